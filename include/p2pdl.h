@@ -46,8 +46,10 @@ extern "C" {
  * 8: adds p2p_fedavg_split_chunks_f32 (a state_dict of separately allocated
  *    tensors on the split kernel, one launch, by 1024-float chunks).
  * 9: adds p2p_aggregate_ex_f32 and P2P_HINT_SHARE_CUS (the FedAvg split
- *    kernel's tile queue vs a kernel running beside it). */
-#define P2P_ABI_VERSION 9
+ *    kernel's tile queue vs a kernel running beside it).
+ * 10: adds the operators of a trainer's local step: p2p_layernorm_*,
+ *    p2p_dropout, p2p_gated_linear_*, p2p_linear_ce_*, P2P_DTYPE_F32. */
+#define P2P_ABI_VERSION 10
 
 typedef void *p2p_stream_t; /* hipStream_t */
 
@@ -209,7 +211,7 @@ int32_t p2p_aggregate_segments_f32(const p2p_segment_t *segs, int32_t nseg, int6
  * to the storage type, as torch runs the reference's ops -- acc = r(acc + u)
  * per update in list order, r(acc / K) (P2P_RULE_FEDAVG) or r(acc * fl(1/K))
  * (P2P_RULE_FEDAVG_TORCH_GPU), w = r(w + r(lr * acc)). */
-enum { P2P_DTYPE_F16 = 1, P2P_DTYPE_BF16 = 2 };
+enum { P2P_DTYPE_F32 = 0 /* K7-K10 only */, P2P_DTYPE_F16 = 1, P2P_DTYPE_BF16 = 2 };
 int32_t p2p_fedavg_apply_16(const uint16_t *const *peers, int32_t k, int64_t n, uint16_t *w, float lr,
                             int32_t dtype, int32_t rule, p2p_stream_t stream);
 
@@ -271,6 +273,81 @@ int32_t p2p_sha256_batch(const uint8_t *const *msgs, const uint64_t *lens, int32
 int32_t p2p_digest_accept(const uint8_t *digests, const uint8_t *expected,
                           const float *const *payloads, int32_t k, const float **accepted,
                           int32_t *count, p2p_stream_t stream);
+
+/* ---- K7-K10: the operators of a trainer's local step --------------------
+ * What a trainer computes between two rounds (reference training/train.py:
+ * 7-22, node/node.py:322-324), forward and backward, before K4 takes the
+ * delta.  `dtype` is P2P_DTYPE_F32 / _F16 / _BF16; sums and statistics are
+ * held in 32 bits, and no result depends on the order of atomics: the same
+ * call gives the same bits.  Tensors need the alignment of their elements
+ * only; an `ld` is a row pitch in elements (>= the row's length), outputs
+ * are dense.  A workspace is 16-byte aligned device memory of at least the
+ * bytes its query returns for the same arguments (< 0: P2P_ERR_*); it holds
+ * nothing between calls, and two calls that may run at once need one each.
+ *
+ * K7, layer norm.  y = (x - mean) * rstd * w + b per row, w / b nullable;
+ * mean and rstd (float, one per row) feed the backward pass, which writes dx
+ * and, where not NULL, dw and db (with rows = 0 it launches nothing: the
+ * caller clears dw and db).  cols <= 16384. */
+int32_t p2p_layernorm_fwd(const void *x, int64_t ldx, const void *w, const void *b, int64_t rows, int64_t cols,
+                          float eps, void *y, float *mean, float *rstd, int32_t dtype, p2p_stream_t stream);
+int64_t p2p_layernorm_bwd_workspace(int64_t rows, int64_t cols, int32_t dtype);
+int32_t p2p_layernorm_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w, const float *mean,
+                          const float *rstd, int64_t rows, int64_t cols, void *dx, void *dw, void *db, void *workspace,
+                          int64_t workspace_bytes, int32_t dtype, p2p_stream_t stream);
+
+/* K8, dropout.  y[i] = (keep(i) ? x[i] / (1 - p) : 0) + residual[i] (nullable),
+ * keep(i): word i % 4 of Philox4x32-10's block offset + *offset_dev + i / 4
+ * (offset_dev nullable; 64-bit counters) under the 64-bit key `seed` is at
+ * least floor(p * 2^32).  0 <= p <= 1.  The gradient is the same call with
+ * x = dy.  n elements use ceil(n / 4) blocks.  y may be x or residual. */
+int32_t p2p_dropout(const void *x, const void *residual, int64_t n, double p, uint64_t seed, uint64_t offset,
+                    const uint64_t *offset_dev, void *y, int32_t dtype, p2p_stream_t stream);
+
+/* K9, the gated linear layer: h = act(x w_gate^T) * (x w_up^T), x [tokens,
+ * hidden], weights [units, hidden].  The forward pass writes h and, where
+ * not NULL, gate and up (float [tokens, units], the products before the
+ * activation), which the backward pass reads with dh [tokens, units] and
+ * turns into dx, dw_gate, dw_up.  With tokens = 0 nothing is launched. */
+enum { P2P_ACT_SILU = 0, P2P_ACT_GELU = 1 /* exact, by erf */, P2P_ACT_RELU = 2 };
+typedef struct p2p_gated_linear_t {
+  const void *x, *w_gate, *w_up;
+  int64_t ldx, ldg, ldu;
+  int64_t tokens, hidden, units;
+  int32_t activation, dtype;
+  void *h;
+  float *gate, *up;
+  const void *dh;
+  int64_t lddh;
+  void *dx, *dw_gate, *dw_up;
+} p2p_gated_linear_t;
+int64_t p2p_gated_linear_workspace(const p2p_gated_linear_t *args, int32_t backward);
+int32_t p2p_gated_linear_fwd(const p2p_gated_linear_t *args, void *workspace, int64_t workspace_bytes,
+                             p2p_stream_t stream);
+int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t *args, void *workspace, int64_t workspace_bytes,
+                             p2p_stream_t stream);
+
+/* K10, softmax cross entropy of the logits x w^T (never stored), x [tokens,
+ * hidden], w [vocab, hidden], over the tokens whose target is not
+ * ignore_index: their mean (mean != 0; 0 where there are none) or sum.  The
+ * forward pass writes loss, lse [tokens] and norm (1 / count, or 1), the
+ * backward pass reads lse and norm and writes dx and dw, times *dloss
+ * (nullable: 1).  A target outside [0, vocab) that is not ignore_index makes
+ * the loss and both gradients NaN.  With tokens = 0 the forward pass writes a
+ * loss of 0, the backward pass launches nothing. */
+typedef struct p2p_linear_ce_t {
+  const void *x, *w;
+  const int64_t *target;
+  int64_t ldx, ldw;
+  int64_t tokens, hidden, vocab, ignore_index;
+  int32_t mean, dtype;
+  float *loss, *lse, *norm;
+  const float *dloss;
+  void *dx, *dw;
+} p2p_linear_ce_t;
+int64_t p2p_linear_ce_workspace(const p2p_linear_ce_t *args, int32_t backward);
+int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t *args, void *workspace, int64_t workspace_bytes, p2p_stream_t stream);
+int32_t p2p_linear_ce_bwd(const p2p_linear_ce_t *args, void *workspace, int64_t workspace_bytes, p2p_stream_t stream);
 
 /* ---- synthetic inputs ---------------------------------
  * out[i] = ((splitmix64(seed ^ (peer << 40) ^ g(i)) >> 40) * 2^-23 - 1) * scale

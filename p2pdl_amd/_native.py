@@ -13,10 +13,11 @@ import threading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # P2P_LIB selects a diagnostic build (csrc/Makefile `diag`); default: the product library
 LIB_PATH = os.environ.get("P2P_LIB") or os.path.join(_HERE, "libp2pdl_hip.so")
-ABI_VERSION = 9  # include/p2pdl.h P2P_ABI_VERSION
+ABI_VERSION = 10  # include/p2pdl.h P2P_ABI_VERSION
 
 P2P_RULE_FEDAVG, P2P_RULE_MEDIAN, P2P_RULE_TRIMMED, P2P_RULE_FEDAVG_TORCH_GPU = 0, 1, 2, 3
-P2P_DTYPE_F16, P2P_DTYPE_BF16 = 1, 2
+P2P_DTYPE_F32, P2P_DTYPE_F16, P2P_DTYPE_BF16 = 0, 1, 2
+P2P_ACT_SILU, P2P_ACT_GELU, P2P_ACT_RELU = 0, 1, 2
 P2P_HINT_SHARE_CUS = 1  # include/p2pdl.h (ABI 9)
 
 # Every symbol include/p2pdl.h declares (tests check the .so exports them).
@@ -28,6 +29,9 @@ EXPORTS = (
     "p2p_fedavg_split_rows_f32", "p2p_fedavg_split_chunks_f32", "p2p_apply_f32",
     "p2p_sha256_batch", "p2p_digest_accept", "p2p_fill_synthetic_f32",
     "p2p_delta_snapshot_f32", "p2p_delta_snapshot_segments_f32", "p2p_land_segments_f32",
+    "p2p_layernorm_fwd", "p2p_layernorm_bwd_workspace", "p2p_layernorm_bwd", "p2p_dropout",
+    "p2p_gated_linear_workspace", "p2p_gated_linear_fwd", "p2p_gated_linear_bwd",
+    "p2p_linear_ce_workspace", "p2p_linear_ce_fwd", "p2p_linear_ce_bwd",
 )
 
 
@@ -61,6 +65,25 @@ _cuda_ok = False  # a ROCm device was seen (checked once)
 _P = ctypes.c_void_p
 _I32, _I64, _U64, _F32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float
 
+
+class GatedLinearArgs(ctypes.Structure):
+    """include/p2pdl.h p2p_gated_linear_t."""
+    _fields_ = [("x", _P), ("w_gate", _P), ("w_up", _P), ("ldx", _I64), ("ldg", _I64), ("ldu", _I64),
+                ("tokens", _I64), ("hidden", _I64), ("units", _I64), ("activation", _I32), ("dtype", _I32),
+                ("h", _P), ("gate", _P), ("up", _P), ("dh", _P), ("lddh", _I64),
+                ("dx", _P), ("dw_gate", _P), ("dw_up", _P)]
+
+
+class LinearCeArgs(ctypes.Structure):
+    """include/p2pdl.h p2p_linear_ce_t."""
+    _fields_ = [("x", _P), ("w", _P), ("target", _P), ("ldx", _I64), ("ldw", _I64),
+                ("tokens", _I64), ("hidden", _I64), ("vocab", _I64), ("ignore_index", _I64),
+                ("mean", _I32), ("dtype", _I32), ("loss", _P), ("lse", _P), ("norm", _P), ("dloss", _P),
+                ("dx", _P), ("dw", _P)]
+
+
+_GATED, _CE = ctypes.POINTER(GatedLinearArgs), ctypes.POINTER(LinearCeArgs)
+
 _SIGS = {
     "p2p_abi_version": ([], _I32),
     "p2p_strerror": ([_I32], ctypes.c_char_p),
@@ -85,6 +108,16 @@ _SIGS = {
     "p2p_delta_snapshot_f32": ([_P, _P, _P, _I64, _I32, _P], _I32),
     "p2p_delta_snapshot_segments_f32": ([_P, _I32, _I64, _I32, _P], _I32),
     "p2p_land_segments_f32": ([_P, _U64, _P, _I32, _I64, _P], _I32),
+    "p2p_layernorm_fwd": ([_P, _I64, _P, _P, _I64, _I64, _F32, _P, _P, _P, _I32, _P], _I32),
+    "p2p_layernorm_bwd_workspace": ([_I64, _I64, _I32], _I64),
+    "p2p_layernorm_bwd": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I32, _P], _I32),
+    "p2p_dropout": ([_P, _P, _I64, ctypes.c_double, _U64, _U64, _P, _P, _I32, _P], _I32),
+    "p2p_gated_linear_workspace": ([_GATED, _I32], _I64),
+    "p2p_gated_linear_fwd": ([_GATED, _P, _I64, _P], _I32),
+    "p2p_gated_linear_bwd": ([_GATED, _P, _I64, _P], _I32),
+    "p2p_linear_ce_workspace": ([_CE, _I32], _I64),
+    "p2p_linear_ce_fwd": ([_CE, _P, _I64, _P], _I32),
+    "p2p_linear_ce_bwd": ([_CE, _P, _I64, _P], _I32),
 }
 
 

@@ -1,0 +1,294 @@
+// K9 -- the gated linear layer of a feed-forward block, forward and backward.
+//
+//   g = x Wg^T, u = x Wu^T, h = act(g) * u            x [T, H], Wg / Wu [F, H]
+//   dg = dh * u * act'(g), du = dh * act(g)
+//   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
+//
+// Matrix-bound: 12 T H F operations over operands that are read once per
+// 256 x 256 tile.  Forward: one kernel, both products (the tile's columns
+// interleave 16 rows of Wg and 16 of Wu, so one lane ends up with g and u of
+// the same unit), the activation and the product in its epilogue.
+//
+// Training keeps g and u in 32 bits (8 bytes a unit): rounded to 16 bits
+// they would put their rounding on top of dg's and du's own and the
+// gradients' error at twice that of one rounding, and computing them again
+// would be two of then eight products (at H = 4096, 2 x 8192 operations per
+// unit against 16 more bytes moved).  dg and du are rounded to the type of x
+// once, as the operands of the matrix instructions (float32: not rounded,
+// three planes), lie side by side in one [T, 2F] buffer, and feed dx as two
+// segments of one sum and dWg, dWu as one product of 2F rows.
+#include "gemm_tile.h"
+
+namespace p2p {
+
+template <int ACT>
+__device__ __forceinline__ void activation(float g, float* a, float* da) {
+  if constexpr (ACT == P2P_ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.f + expf(-g));
+    *a = g * s;
+    *da = s * (1.f + g * (1.f - s));
+  } else if constexpr (ACT == P2P_ACT_GELU) {
+    const float phi = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    *a = g * phi;
+    *da = phi + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+  } else {
+    *a = g < 0.f ? 0.f : g;  // a NaN stays one
+    *da = g > 0.f ? 1.f : 0.f;
+  }
+}
+__device__ __forceinline__ void activation(int act, float g, float* a, float* da) {
+  if (act == P2P_ACT_SILU) activation<P2P_ACT_SILU>(g, a, da);
+  else if (act == P2P_ACT_GELU) activation<P2P_ACT_GELU>(g, a, da);
+  else activation<P2P_ACT_RELU>(g, a, da);
+}
+
+struct GatedEpi {
+  void* h;
+  float *gate, *up;  // nullable
+  int64_t units;
+  int32_t dtype, act;
+
+  template <class Cfg>
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char*) const {
+    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+      const int64_t m = p.m0 + i * 16 + i16;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; j += 2) {
+        const int64_t n = p.n0 / 2 + j * 8 + q4;
+        if (n >= units) continue;
+        const f4 gv = acc[i][j], uv = acc[i][j + 1];
+        f4 hv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float a, da;
+          activation(act, gv[e], &a, &da);
+          hv[e] = a * uv[e];
+        }
+        store4_as(h, dtype, m, units, n, units, hv);
+        if (gate) store4(gate + m * units, n, units, gv);
+        if (up) store4(up + m * units, n, units, uv);
+      }
+    }
+  }
+};
+
+// dg and du of 8 units per lane, into d [T, 2 * pitch]: dg, then du, zeros
+// in the columns past `units`; plane: elements from one plane to the next.
+template <typename T, int ACT>
+__global__ __launch_bounds__(kBlock) void gated_grad_kernel(const T* dh, int64_t lddh, const float* gate, const float* up,
+                                                            int64_t rows, int64_t units, int64_t pitch, uint16_t* d,
+                                                            int64_t plane) {
+  const int64_t per_row = pitch / 8, all = rows * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
+       i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    float g[8], u[8], dhv[8];
+    load_row<float, 8>(gate + r * units, c, units, g);
+    load_row<float, 8>(up + r * units, c, units, u);
+    load_row<T, 8>(dh + r * lddh, c, units, dhv);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float a, da;
+      activation<ACT>(g[e], &a, &da);
+      const float dg = dhv[e] * u[e] * da, du = dhv[e] * a;
+      g[e] = c + e < units ? dg : 0.f;
+      u[e] = c + e < units ? du : 0.f;
+    }
+    uint16_t* to = d + r * 2 * pitch + c;
+    if constexpr (sizeof(T) == 4) {
+      Pack<uint16_t, 8> og[3], ou[3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Planes a = split3(g[e]), b = split3(u[e]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) og[q].v[e] = a.p[q], ou[q].v[e] = b.p[q];
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        store_pack<uint16_t, 8>(to + q * plane, og[q]);
+        store_pack<uint16_t, 8>(to + q * plane + pitch, ou[q]);
+      }
+    } else {
+      store_row<T, 8>(reinterpret_cast<T*>(to), 0, 8, g);
+      store_row<T, 8>(reinterpret_cast<T*>(to) + pitch, 0, 8, u);
+    }
+  }
+}
+
+template <typename T>
+static int32_t gated_grad(const p2p_gated_linear_t& a, int64_t pitch, uint16_t* d, hipStream_t st) {
+  const int64_t items = a.tokens * (pitch / 8), blocks = ceil_div(items, kBlock);
+  const dim3 grid(static_cast<unsigned>(blocks < 256 * 32 ? blocks : 256 * 32)), block(kBlock);
+  const int64_t plane = a.tokens * 2 * pitch;
+  const T* dh = static_cast<const T*>(a.dh);
+  if (a.activation == P2P_ACT_SILU)
+    gated_grad_kernel<T, P2P_ACT_SILU><<<grid, block, 0, st>>>(dh, a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d, plane);
+  else if (a.activation == P2P_ACT_GELU)
+    gated_grad_kernel<T, P2P_ACT_GELU><<<grid, block, 0, st>>>(dh, a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d, plane);
+  else
+    gated_grad_kernel<T, P2P_ACT_RELU><<<grid, block, 0, st>>>(dh, a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d, plane);
+  return launch_status();
+}
+
+static int32_t gated_check(const p2p_gated_linear_t* a) {
+  if (!a || !known_dtype(a->dtype) || a->activation < 0 || a->activation > P2P_ACT_RELU) return P2P_ERR_INVALID;
+  if (a->tokens < 0 || a->hidden < 1 || a->units < 1 || a->ldx < a->hidden || a->ldg < a->hidden || a->ldu < a->hidden)
+    return P2P_ERR_INVALID;
+  const int64_t most = (int64_t(1) << 31) - 256;
+  if (a->hidden > kMaxPitch - 8 || a->units > kMaxPitch / 2 - 8 || a->tokens > most) return P2P_ERR_UNSUPPORTED;
+  if (!a->w_gate || !a->w_up || (a->tokens > 0 && !a->x)) return P2P_ERR_INVALID;
+  const int s = dtype_bytes(a->dtype);
+  if (!aligned_to(a->x, s) || !aligned_to(a->w_gate, s) || !aligned_to(a->w_up, s)) return P2P_ERR_ALIGN;
+  return P2P_OK;
+}
+
+// The workspace, in the order in which both passes carve it.
+struct GatedSpace {
+  uint16_t *x, *wg, *wu, *d;
+  float* parts;
+};
+static int64_t gated_pitch(const p2p_gated_linear_t& a) { return round_up(a.units, 8); }
+static Plan gated_dx_plan(const p2p_gated_linear_t& a) {
+  return gemm_plan(a.tokens, a.hidden, ksteps(a.units, a.dtype == P2P_DTYPE_F32 ? 12 : 2), true);
+}
+static Plan gated_dw_plan(const p2p_gated_linear_t& a) {
+  return gemm_plan(2 * gated_pitch(a), a.hidden, ksteps(a.tokens, a.dtype == P2P_DTYPE_F32 ? 6 : 1), true);
+}
+static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* base, GatedSpace* s) {
+  Carver c{static_cast<char*>(base)};
+  const auto operand = [&](const void* p, int64_t ld, int64_t rows) -> uint16_t* {
+    return in_place(p, ld, a.hidden, a.dtype) ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(rows, a.hidden, a.dtype)));
+  };
+  s->x = operand(a.x, a.ldx, a.tokens);
+  s->wg = operand(a.w_gate, a.ldg, a.units);
+  // both weights share one pitch: packed together or not at all
+  if (in_place(a.w_gate, a.ldg, a.hidden, a.dtype) && in_place(a.w_up, a.ldu, a.hidden, a.dtype) && a.ldg == a.ldu) {
+    s->wu = nullptr;
+  } else {
+    if (!s->wg) s->wg = static_cast<uint16_t*>(c.take(packed_bytes(a.units, a.hidden, a.dtype)));
+    s->wu = static_cast<uint16_t*>(c.take(packed_bytes(a.units, a.hidden, a.dtype)));
+  }
+  s->d = nullptr;
+  s->parts = nullptr;
+  if (backward) {
+    const int64_t rows2 = 2 * gated_pitch(a);
+    s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 2 * planes_of(a.dtype)));
+    const Plan px = gated_dx_plan(a), pw = gated_dw_plan(a);
+    int64_t floats = 0;
+    if (px.split > 1) floats = px.split * a.tokens * a.hidden;
+    if (pw.split > 1) floats = std::max(floats, pw.split * rows2 * a.hidden);
+    if (floats) s->parts = static_cast<float*>(c.take(floats * 4));
+  }
+  return c.used;
+}
+
+static int32_t gated_operand(const void* p, int64_t ld, int64_t rows, int64_t cols, int32_t dtype, uint16_t* space, Mat* m,
+                             hipStream_t st) {
+  if (space) return pack_matrix(p, ld, rows, cols, dtype, space, m, st);
+  m->plane[0] = static_cast<const uint16_t*>(p);
+  m->plane[1] = m->plane[2] = nullptr;
+  m->ld = ld;
+  return P2P_OK;
+}
+
+}  // namespace p2p
+
+using namespace p2p;
+
+extern "C" int64_t p2p_gated_linear_workspace(const p2p_gated_linear_t* a, int32_t backward) {
+  const int32_t rc = gated_check(a);
+  if (rc != P2P_OK) return rc;
+  GatedSpace s;
+  return a->tokens ? gated_carve(*a, backward != 0, nullptr, &s) : 0;
+}
+
+extern "C" int32_t p2p_gated_linear_fwd(const p2p_gated_linear_t* a, void* workspace, int64_t workspace_bytes,
+                                        p2p_stream_t stream) {
+  int32_t rc = gated_check(a);
+  if (rc != P2P_OK || a->tokens == 0) return rc;
+  if (!a->h || !aligned_to(a->h, dtype_bytes(a->dtype)) || !aligned_to(a->gate, 4) || !aligned_to(a->up, 4))
+    return a->h ? P2P_ERR_ALIGN : P2P_ERR_INVALID;
+  GatedSpace s;
+  const int64_t need = gated_carve(*a, false, workspace, &s);
+  if (need > workspace_bytes || (need && !workspace)) return P2P_ERR_INVALID;
+  if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  Mat x, wg, wu;
+  if ((rc = gated_operand(a->x, a->ldx, a->tokens, a->hidden, a->dtype, s.x, &x, st)) != P2P_OK) return rc;
+  if ((rc = gated_operand(a->w_gate, a->ldg, a->units, a->hidden, a->dtype, s.wg, &wg, st)) != P2P_OK) return rc;
+  if ((rc = gated_operand(a->w_up, a->ldu, a->units, a->hidden, a->dtype, s.wu, &wu, st)) != P2P_OK) return rc;
+  GemmArgs g{};
+  add_pairs(&g, x, wg, &wu, a->dtype);
+  g.lda = x.ld, g.ldb = wg.ld;
+  g.M = a->tokens, g.N = 2 * a->units, g.K = a->hidden;
+  g.ksplit = 1;
+  const GatedEpi epi{a->h, a->gate, a->up, a->units, a->dtype, a->activation};
+  const bool big = gemm_plan(g.M, g.N, ksteps(g.K, g.nseg), false).big;
+  return gemm_launch<false, false, true>(g, a->dtype == P2P_DTYPE_F16, big, epi, st);
+}
+
+extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* workspace, int64_t workspace_bytes,
+                                        p2p_stream_t stream) {
+  int32_t rc = gated_check(a);
+  if (rc != P2P_OK || a->tokens == 0) return rc;
+  if (!a->gate || !a->up || !a->dh || a->lddh < a->units || !a->dx || !a->dw_gate || !a->dw_up) return P2P_ERR_INVALID;
+  const int size = dtype_bytes(a->dtype);
+  if (!aligned_to(a->gate, 4) || !aligned_to(a->up, 4) || !aligned_to(a->dh, size) || !aligned_to(a->dx, size) ||
+      !aligned_to(a->dw_gate, size) || !aligned_to(a->dw_up, size))
+    return P2P_ERR_ALIGN;
+  GatedSpace s;
+  const int64_t need = gated_carve(*a, true, workspace, &s);
+  if (need > workspace_bytes || !workspace) return P2P_ERR_INVALID;
+  if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool f16_ = a->dtype == P2P_DTYPE_F16;
+  Mat x, wg, wu;
+  if ((rc = gated_operand(a->x, a->ldx, a->tokens, a->hidden, a->dtype, s.x, &x, st)) != P2P_OK) return rc;
+  if ((rc = gated_operand(a->w_gate, a->ldg, a->units, a->hidden, a->dtype, s.wg, &wg, st)) != P2P_OK) return rc;
+  if ((rc = gated_operand(a->w_up, a->ldu, a->units, a->hidden, a->dtype, s.wu, &wu, st)) != P2P_OK) return rc;
+  const int64_t pitch = gated_pitch(*a), plane = a->tokens * 2 * pitch;
+  rc = a->dtype == P2P_DTYPE_F32 ? gated_grad<float>(*a, pitch, s.d, st)
+       : f16_                    ? gated_grad<f16>(*a, pitch, s.d, st)
+                                 : gated_grad<bf16>(*a, pitch, s.d, st);
+  if (rc != P2P_OK) return rc;
+  Mat dg{{s.d, s.d + plane, s.d + 2 * plane}, 2 * pitch};
+  Mat du{{s.d + pitch, s.d + plane + pitch, s.d + 2 * plane + pitch}, 2 * pitch};
+
+  {  // dx = dg Wg + du Wu
+    GemmArgs g{};
+    add_pairs(&g, dg, wg, nullptr, a->dtype);
+    add_pairs(&g, du, wu, nullptr, a->dtype);
+    g.lda = 2 * pitch, g.ldb = wg.ld;
+    g.M = a->tokens, g.N = a->hidden, g.K = a->units;
+    const Plan plan = gated_dx_plan(*a);
+    g.ksplit = plan.split;
+    StoreEpi e{{a->dx, nullptr}, 0, 0, a->hidden, a->dtype, {nullptr, nullptr}, 1.f, plan.split > 1 ? s.parts : nullptr, 0};
+    if ((rc = gemm_launch<false, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
+    if (plan.split > 1 && (rc = join_parts(s.parts, plan.split, g.M * g.N, g.M * g.N, nullptr, nullptr, 1.f, a->dx, a->dtype,
+                                           st)) != P2P_OK)
+      return rc;
+  }
+  {  // dWg = dg^T x, dWu = du^T x: one product of 2 pitch rows
+    GemmArgs g{};
+    add_pairs(&g, dg, x, nullptr, a->dtype);
+    g.lda = 2 * pitch, g.ldb = x.ld;
+    g.M = 2 * pitch, g.N = a->hidden, g.K = a->tokens;
+    const Plan plan = gated_dw_plan(*a);
+    g.ksplit = plan.split;
+    StoreEpi e{{a->dw_gate, a->dw_up}, pitch, a->units, a->hidden, a->dtype, {nullptr, nullptr}, 1.f,
+               plan.split > 1 ? s.parts : nullptr, 0};
+    if ((rc = gemm_launch<true, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
+    if (plan.split > 1) {
+      const int64_t n = a->units * a->hidden, stride = g.M * g.N;
+      if ((rc = join_parts(s.parts, plan.split, stride, n, nullptr, nullptr, 1.f, a->dw_gate, a->dtype, st)) != P2P_OK)
+        return rc;
+      if ((rc = join_parts(s.parts + pitch * a->hidden, plan.split, stride, n, nullptr, nullptr, 1.f, a->dw_up, a->dtype,
+                           st)) != P2P_OK)
+        return rc;
+    }
+  }
+  return P2P_OK;
+}

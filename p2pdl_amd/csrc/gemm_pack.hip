@@ -1,0 +1,91 @@
+// What surrounds the products of gemm_tile.h: copies of operands that cannot
+// be read in place, and the sum of a product's k-runs.
+#include "gemm_tile.h"
+
+namespace p2p {
+
+// One lane per 8 elements of a packed row.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void pack_kernel(const T* src, int64_t ld, int64_t rows, int64_t cols, int64_t pitch,
+                                                      uint16_t* dst, int64_t plane) {
+  const int64_t per_row = pitch / 8, all = rows * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
+       i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    const T* s = src + r * ld;
+    if constexpr (sizeof(T) == 4) {
+      float v[8];
+      load_row<T, 8>(s, c, cols, v);
+      Pack<uint16_t, 8> o[3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Planes p = split3(v[e]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) o[q].v[e] = p.p[q];
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q) store_pack<uint16_t, 8>(dst + q * plane + r * pitch + c, o[q]);
+    } else {
+      Pack<uint16_t, 8> o;
+      if (c + 8 <= cols) {
+        o = load_pack<uint16_t, 8>(s + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o.v[e] = c + e < cols ? ldg(s + c + e) : 0;
+      }
+      store_pack<uint16_t, 8>(dst + r * pitch + c, o);
+    }
+  }
+}
+
+static unsigned blocks_for(int64_t items) {
+  const int64_t b = ceil_div(items, kBlock);
+  return static_cast<unsigned>(b < 1 ? 1 : b > 256 * 32 ? 256 * 32 : b);
+}
+
+int32_t pack_matrix(const void* src, int64_t ld, int64_t rows, int64_t cols, int32_t dtype, uint16_t* dst, Mat* out,
+                    hipStream_t st) {
+  const int64_t pitch = round_up(cols, 8), plane = rows * pitch;
+  for (int q = 0; q < 3; ++q) out->plane[q] = q < planes_of(dtype) ? dst + q * plane : nullptr;
+  out->ld = pitch;
+  if (rows == 0) return P2P_OK;
+  const unsigned blocks = blocks_for(rows * (pitch / 8));
+  if (dtype == P2P_DTYPE_F32)
+    pack_kernel<float><<<dim3(blocks), dim3(kBlock), 0, st>>>(static_cast<const float*>(src), ld, rows, cols, pitch, dst, plane);
+  else
+    pack_kernel<uint16_t><<<dim3(blocks), dim3(kBlock), 0, st>>>(static_cast<const uint16_t*>(src), ld, rows, cols, pitch, dst, plane);
+  return launch_status();
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void join_kernel(const float* parts, int nparts, int64_t stride, int64_t n,
+                                                      const float* scale0, const float* scale1, float alpha, T* out) {
+  if (scale0) alpha *= ldc(scale0);
+  if (scale1) alpha *= ldc(scale1);
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * 4; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kBlock * 4) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < nparts; ++p) {
+      float v[4];
+      load_row<float, 4>(parts + p * stride, i, n, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] *= alpha;
+    store_row<T, 4>(out, i, n, s);
+  }
+}
+
+int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, const float* scale0, const float* scale1, float alpha,
+                   void* out, int32_t dtype, hipStream_t st) {
+  if (n == 0) return P2P_OK;
+  const dim3 grid(blocks_for(ceil_div(n, 4))), block(kBlock);
+  if (dtype == P2P_DTYPE_F32) join_kernel<float><<<grid, block, 0, st>>>(parts, nparts, stride, n, scale0, scale1, alpha, static_cast<float*>(out));
+  else if (dtype == P2P_DTYPE_F16) join_kernel<f16><<<grid, block, 0, st>>>(parts, nparts, stride, n, scale0, scale1, alpha, static_cast<f16*>(out));
+  else join_kernel<bf16><<<grid, block, 0, st>>>(parts, nparts, stride, n, scale0, scale1, alpha, static_cast<bf16*>(out));
+  return launch_status();
+}
+
+}  // namespace p2p

@@ -1,0 +1,458 @@
+// The matrix product under the gated linear layer and the linear cross
+// entropy: C[m, n] = sum over k of A(m, k) * B(n, k), 16-bit operands,
+// accumulators in 32 bits, the epilogue in the caller's hands.
+//
+// Operands.  An operand is either k-contiguous (A[m][k], what x and a weight
+// [out, in] are in the forward pass) or row-contiguous (A[k][m], what the same
+// tensors are when the gradient sums over tokens or over units); neither is
+// transposed in memory.  Requirements of both: 16-byte aligned base and
+// pitch, contiguous extent a multiple of 8 (pack_kernel makes such a copy of
+// what is not).  A product may be a sum over several (A, B) pairs of equal
+// shape, its segments: the two halves of the gated layer's dx, and float32.
+//
+// float32.  x = hi + mid + lo exactly, three bf16 values of 8 bits each,
+// rounded to nearest: |mid| <= 2^-8 |x|, |lo| <= 2^-16 |x|.  Of the nine
+// products the six of order 2^-16 and above are kept, the small ones first;
+// what is left out is at most 2^-23 + 2^-32 of |a| |b|, the size of one
+// rounding of a 32-bit sum.  Six bf16 products take 6/16 of the time of one on
+// the 32-bit matrix instructions.  A value that is not finite is its own hi.
+//
+// Tile.  BM x BN x 64, double-buffered in LDS (128 KiB for 256 x 256), filled
+// by LDS-DMA: a wave's instruction writes 1 KiB in lane order, so the
+// swizzles are made by choosing each lane's source address.  Lanes whose
+// source lies outside the operand get an offset past the descriptor's range
+// and write zeros.  One barrier per 64 k: the loads of step s + 1 are issued
+// after it and waited for before the next one, under the matrix
+// instructions of step s.
+//
+// LDS images.  k-contiguous: rows of 128 bytes, 16-byte chunk c at position
+// c ^ (row / 2 % 8): the 16 lanes of one k-group, one row each, then hit the 64
+// banks once.  Row-contiguous: one line per k, its 32-byte granule g at
+// position g ^ f(k), f(k) = k % 4 + 4 * (k / 8 % 4), read with
+// ds_read_b64_tr_b16 (a 4 x 16 block of 16-bit elements comes back transposed
+// over 16 lanes); f spreads the 16 lines that one instruction reads.
+#pragma once
+#include <algorithm>
+
+#include "train_common.h"
+
+#define P2P_LDS __attribute__((address_space(3)))
+
+namespace p2p {
+
+constexpr int kGemmK = 64;
+constexpr int kMaxSegs = 12;
+constexpr int64_t kMaxPitch = int64_t(1) << 22;  // 256 rows of 16-bit elements stay below 2^31 bytes
+
+using f4 = float __attribute__((ext_vector_type(4)));
+using s4 = short __attribute__((ext_vector_type(4)));
+using s8 = short __attribute__((ext_vector_type(8)));
+using b8 = __bf16 __attribute__((ext_vector_type(8)));
+using h8 = _Float16 __attribute__((ext_vector_type(8)));
+
+struct GemmArgs {
+  const uint16_t* a[kMaxSegs];
+  const uint16_t* b[kMaxSegs];
+  const uint16_t* b2[kMaxSegs];  // DUAL: the second weight
+  int64_t lda, ldb;
+  int64_t M, N, K;  // K of one segment
+  int nseg;
+  int ksplit;       // grid.y: the k-steps of all segments cut into this many runs
+};
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct GemmCfg {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int TM = BM / WM, TN = BN / WN;  // a wave's part of the tile
+  static constexpr int MI = TM / 16, NJ = TN / 16;
+  static constexpr int A_BYTES = BM * kGemmK * 2, STAGE = (BM + BN) * kGemmK * 2;
+  static constexpr int BLOCKS_PER_CU = 2 * STAGE > 80 * 1024 ? 1 : 2;
+};
+using Big = GemmCfg<256, 256, 2, 4>;
+using Small = GemmCfg<128, 128, 2, 2>;
+
+constexpr uint32_t kOutside = 0x80000000u;
+
+// One operand's part of a stage.  EXT: rows of the tile, INSTS: 1-KiB
+// instructions per wave.
+template <bool ROWMAJOR, int EXT, int INSTS>
+struct TileLoader {
+  uint32_t voff[INSTS];
+  int kpos[INSTS];
+  uint32_t kstep;  // bytes from one k-step to the next
+
+  // Lane addresses relative to the tile's origin; `rows` left from it.
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int64_t rows) {
+#pragma unroll
+    for (int j = 0; j < INSTS; ++j) {
+      const int q = wave * INSTS + j;
+      if constexpr (!ROWMAJOR) {
+        const int r = q * 8 + lane / 8;
+        const int c = (lane & 7) ^ ((r >> 1) & 7);
+        kpos[j] = c * 8;
+        voff[j] = r < rows ? static_cast<uint32_t>(r * ld * 2 + c * 16) : kOutside;
+      } else {
+        constexpr int CPL = EXT / 8;  // 16-byte chunks of a line
+        const int k = q * (64 / CPL) + lane / CPL;
+        const int pos = lane % CPL;
+        const int f = ((k & 3) | (((k >> 3) & 3) << 2)) & (EXT / 16 - 1);
+        const int m = ((pos >> 1) ^ f) * 16 + (pos & 1) * 8;
+        kpos[j] = k;
+        voff[j] = m < rows ? static_cast<uint32_t>(k * ld * 2 + m * 2) : kOutside;
+      }
+    }
+  }
+
+  // The k-step at `base` into the image at dst; `left`: k still in the segment.
+  __device__ __forceinline__ void issue(const uint16_t* base, int64_t left, char* dst, int wave) const {
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, static_cast<int>(kOutside), 0x00020000);
+#pragma unroll
+    for (int j = 0; j < INSTS; ++j) {
+      const uint32_t v = kpos[j] < left ? voff[j] : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (P2P_LDS void*)(dst + (wave * INSTS + j) * 1024), 16, v, 0, 0, 0);
+    }
+  }
+};
+
+template <bool F16>
+__device__ __forceinline__ f4 mfma16(s8 a, s8 b, f4 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// A 16-row fragment of 32 k out of an image: lane l gets row l % 16, k = 8 * (l / 16) ... + 7.
+template <bool ROWMAJOR, int EXT>
+struct FragReader {
+  int base[2];  // k-contiguous: per half of the step
+  int kline, f, part;
+
+  __device__ __forceinline__ void init(int lane) {
+    const int i = lane & 15, q = lane >> 4;
+    if constexpr (!ROWMAJOR) {
+      base[0] = i * 128 + ((q ^ (i >> 1)) & 7) * 16;
+      base[1] = i * 128 + (((4 + q) ^ (i >> 1)) & 7) * 16;
+    } else {
+      kline = (8 * q + (i >> 2)) * EXT * 2;
+      f = ((i >> 2) | (q << 2)) & (EXT / 16 - 1);
+      part = (i & 3) * 8;
+    }
+  }
+  // row0: first row of the fragment in the tile, a multiple of 16
+  __device__ __forceinline__ s8 read(const char* image, int row0, int half) const {
+    if constexpr (!ROWMAJOR) {
+      return *reinterpret_cast<const P2P_LDS s8*>((const P2P_LDS char*)(image) + base[half] + row0 * 128);
+    } else {
+      const P2P_LDS char* p = (const P2P_LDS char*)(image) + kline + half * 32 * EXT * 2 + (((row0 >> 4) ^ f) << 5) + part;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P2P_LDS s4*)(p));
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P2P_LDS s4*)(p + 4 * EXT * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// Blocks go to the eight XCDs in turn; give each XCD a contiguous run of
+// tiles, and order the tiles in groups of 8 rows so that a run shares its
+// operands in that XCD's L2.
+__device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int* tm, int* tn) {
+  const int total = tiles_m * tiles_n;
+  const int pid = blockIdx.x, per = total / 8, extra = total % 8, xcd = pid % 8;
+  const int t = xcd * per + (xcd < extra ? xcd : extra) + pid / 8;
+  constexpr int G = 8;
+  const int group = t / (G * tiles_n), first = group * G;
+  const int rows = tiles_m - first < G ? tiles_m - first : G;
+  const int in = t - group * G * tiles_n;
+  *tm = first + in % rows;
+  *tn = in / rows;
+}
+
+// Where an accumulator element lies: acc[mi][nj][i] is C[m][n] of
+// m = m0 + 16 mi + (lane % 16), n = n0 + 16 nj + 4 (lane / 16) + i
+// (the second operand's rows come out as the register index, so a lane holds
+// four neighbours of one output row).
+struct Place {
+  int64_t m0, n0;  // the wave's first row and column
+  int lane, wave;
+  int tm, tn;      // the tile
+  int wm, wn;      // the wave in it
+  int part;        // the k-run
+};
+
+// DUAL: B's tile interleaves 16 rows of b and 16 of b2; N counts both (the
+// tile's columns [32 j, 32 j + 16) are b's rows [16 j, 16 j + 16)).
+template <bool F16, bool AT, bool BT, bool DUAL, class Cfg, class Epi>
+__global__ __launch_bounds__(Cfg::THREADS, 2) void gemm_kernel(GemmArgs g, Epi epi) {
+  __shared__ __attribute__((aligned(1024))) char lds[2 * Cfg::STAGE];
+  constexpr int A_INSTS = Cfg::BM / 8 / Cfg::WAVES, B_INSTS = Cfg::BN / 8 / Cfg::WAVES;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles_m = static_cast<int>(ceil_div(g.M, Cfg::BM)), tiles_n = static_cast<int>(ceil_div(g.N, Cfg::BN));
+  int tm, tn;
+  tile_of_block(tiles_m, tiles_n, &tm, &tn);
+  const int64_t m0 = static_cast<int64_t>(tm) * Cfg::BM, n0 = static_cast<int64_t>(tn) * Cfg::BN;
+
+  TileLoader<AT, Cfg::BM, A_INSTS> la;
+  TileLoader<BT, Cfg::BN, B_INSTS> lb;
+  la.init(wave, lane, g.lda, g.M - m0);
+  const int64_t a_org = AT ? m0 : m0 * g.lda;
+  int64_t b_org;
+  if constexpr (DUAL) {
+    static_assert(!BT, "two weights: k-contiguous");
+    // tile row r: unit n0 / 2 + 16 (r / 32) + r % 16 of b (r / 16 even) or b2 (odd)
+    const int64_t units = g.N / 2 - n0 / 2;
+#pragma unroll
+    for (int j = 0; j < B_INSTS; ++j) {
+      const int r = (wave * B_INSTS + j) * 8 + lane / 8, u = (r >> 5) * 16 + (r & 15);
+      const int c = (lane & 7) ^ ((r >> 1) & 7);
+      lb.kpos[j] = c * 8;
+      lb.voff[j] = u < units ? static_cast<uint32_t>(u * g.ldb * 2 + c * 16) : kOutside;
+    }
+    b_org = n0 / 2 * g.ldb;
+  } else {
+    lb.init(wave, lane, g.ldb, g.N - n0);
+    b_org = BT ? n0 : n0 * g.ldb;
+  }
+
+  const int per_seg = static_cast<int>(ceil_div(g.K, kGemmK));
+  const int all = per_seg * g.nseg;
+  const int part = blockIdx.y;
+  const int first = static_cast<int>(static_cast<int64_t>(all) * part / g.ksplit);
+  const int last = static_cast<int>(static_cast<int64_t>(all) * (part + 1) / g.ksplit);
+  int seg = first / per_seg, ks = first % per_seg;
+
+  const auto issue = [&](int buf) {
+    const int64_t k0 = static_cast<int64_t>(ks) * kGemmK, left = g.K - k0;
+    char* dst = lds + buf * Cfg::STAGE;
+    la.issue(g.a[seg] + a_org + (AT ? k0 * g.lda : k0), left, dst, wave);
+    if constexpr (DUAL) {
+      const int64_t org = b_org + k0;
+#pragma unroll
+      for (int j = 0; j < B_INSTS; ++j) {
+        const int q = wave * B_INSTS + j;  // rows 8q .. 8q + 7: all of one weight
+        const uint16_t* w = (q >> 1) & 1 ? g.b2[seg] : g.b[seg];
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(w + org), 0,
+                                                                            static_cast<int>(kOutside), 0x00020000);
+        const uint32_t v = lb.kpos[j] < left ? lb.voff[j] : kOutside;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (P2P_LDS void*)(dst + Cfg::A_BYTES + q * 1024), 16, v, 0, 0, 0);
+      }
+    } else {
+      lb.issue(g.b[seg] + b_org + (BT ? k0 * g.ldb : k0), left, dst + Cfg::A_BYTES, wave);
+    }
+    if (++ks == per_seg) ks = 0, ++seg;
+  };
+
+  FragReader<AT, Cfg::BM> ra;
+  FragReader<BT, Cfg::BN> rb;
+  ra.init(lane);
+  rb.init(lane);
+  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  f4 acc[Cfg::MI][Cfg::NJ];
+#pragma unroll
+  for (int i = 0; i < Cfg::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < Cfg::NJ; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+
+  if (first < last) issue(0);
+  for (int s = first; s < last; ++s) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of step s
+    __builtin_amdgcn_s_barrier();                     // everyone's; and step s - 1's image is read
+    asm volatile("" ::: "memory");
+    if (s + 1 < last) issue((s + 1 - first) & 1);
+    const char* image = lds + ((s - first) & 1) * Cfg::STAGE;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      s8 fa[Cfg::MI], fb[Cfg::NJ];
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j) fb[j] = rb.read(image + Cfg::A_BYTES, wn * Cfg::TN + j * 16, half);
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) fa[i] = ra.read(image, wm * Cfg::TM + i * 16, half);
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < Cfg::NJ; ++j) acc[i][j] = mfma16<F16>(fb[j], fa[i], acc[i][j]);
+    }
+  }
+  __syncthreads();  // the images are free: an epilogue may use them
+  Place p;
+  p.m0 = m0 + wm * Cfg::TM, p.n0 = n0 + wn * Cfg::TN;
+  p.lane = lane, p.wave = wave, p.tm = tm, p.tn = tn, p.wm = wm, p.wn = wn, p.part = part;
+  epi.template finish<Cfg>(acc, p, g, lds);
+}
+
+// ------------------------------------------------------------------ epilogues
+// Four neighbours of one row, columns n .. n + 3 of `cols`, as T.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int64_t n, int64_t cols, f4 v) {
+  if (n + 4 <= cols) {
+    Pack<T, 4> p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p.v[i] = static_cast<T>(v[i]);
+    store_pack<T, 4>(row + n, p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < cols) stg(row + n + i, static_cast<T>(v[i]));
+  }
+}
+__device__ __forceinline__ void store4_as(void* base, int32_t dtype, int64_t row, int64_t pitch, int64_t n, int64_t cols,
+                                          f4 v) {
+  if (dtype == P2P_DTYPE_F32) store4(static_cast<float*>(base) + row * pitch, n, cols, v);
+  else if (dtype == P2P_DTYPE_F16) store4(static_cast<f16*>(base) + row * pitch, n, cols, v);
+  else store4(static_cast<bf16*>(base) + row * pitch, n, cols, v);
+}
+
+// A float as three bf16 (their bits): hi + mid + lo == x.
+struct Planes {
+  uint16_t p[3];
+};
+__device__ __forceinline__ uint16_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, static_cast<bf16>(x)); }
+__device__ __forceinline__ Planes split3(float x) {
+  Planes r;
+  const uint32_t b = __float_as_uint(x);
+  const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+  r.p[0] = bf16_bits(x);
+  // the largest floats would round up to an infinity: cut them off instead
+  if (finite && (r.p[0] & 0x7fff) == 0x7f80) r.p[0] = static_cast<uint16_t>(b >> 16);
+  const float rest = finite ? x - __uint_as_float(static_cast<uint32_t>(r.p[0]) << 16) : 0.f;
+  r.p[1] = bf16_bits(rest);
+  r.p[2] = bf16_bits(rest - __uint_as_float(static_cast<uint32_t>(r.p[1]) << 16));
+  return r;
+}
+// The six kept products, small ones first: (plane of A, plane of B).
+constexpr int kSplitA[6] = {0, 2, 1, 0, 1, 0}, kSplitB[6] = {2, 0, 1, 1, 0, 0};
+
+// C = alpha * acc as `dtype`, or the raw sums of one k-run into its own
+// float plane (`partial`; add: on top of what is there).  With `half` > 0
+// the rows from `half` on are a second result's (rows past `rows` of either
+// are padding).
+struct StoreEpi {
+  void* out[2];
+  int64_t half, rows;
+  int64_t pitch;
+  int32_t dtype;
+  const float* scale[2];  // device factors (nullable)
+  float alpha;
+  float* partial;         // [ksplit][M][pitch]
+  int add;
+
+  template <class Cfg>
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char*) const {
+    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+    float a = alpha;
+    if (scale[0]) a *= ldc(scale[0]);
+    if (scale[1]) a *= ldc(scale[1]);
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+      const int64_t m = p.m0 + i * 16 + i16;
+      if (m >= g.M) continue;
+      const bool second = half > 0 && m >= half;
+      const int64_t row = second ? m - half : m;
+      if (!partial && half > 0 && row >= rows) continue;
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j) {
+        const int64_t n = p.n0 + j * 16 + q4;
+        if (n >= g.N) continue;
+        if (partial) {
+          float* to = partial + (p.part * g.M + m) * pitch;
+          f4 v = acc[i][j];
+          if (add) {
+            float o[4];
+            load_row<float, 4>(to, n, g.N, o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += o[e];
+          }
+          store4(to, n, g.N, v);
+        } else {
+          store4_as(out[second], dtype, row, pitch, n, g.N, acc[i][j] * a);
+        }
+      }
+    }
+  }
+};
+
+// ------------------------------------------------------------------ host side
+template <bool F16, bool AT, bool BT, bool DUAL, class Cfg, class Epi>
+static int32_t gemm_launch_cfg(const GemmArgs& g, const Epi& epi, hipStream_t st) {
+  const int64_t tiles = ceil_div(g.M, Cfg::BM) * ceil_div(g.N, Cfg::BN);
+  if (tiles > (int64_t(1) << 31) / Cfg::THREADS) return P2P_ERR_UNSUPPORTED;
+  gemm_kernel<F16, AT, BT, DUAL, Cfg, Epi>
+      <<<dim3(static_cast<unsigned>(tiles), g.ksplit), dim3(Cfg::THREADS), 0, st>>>(g, epi);
+  return launch_status();
+}
+
+template <bool AT, bool BT, bool DUAL, class Epi>
+static int32_t gemm_launch(const GemmArgs& g, bool is_f16, bool big, const Epi& epi, hipStream_t st) {
+  if (is_f16)
+    return big ? gemm_launch_cfg<true, AT, BT, DUAL, Big>(g, epi, st)
+               : gemm_launch_cfg<true, AT, BT, DUAL, Small>(g, epi, st);
+  return big ? gemm_launch_cfg<false, AT, BT, DUAL, Big>(g, epi, st)
+             : gemm_launch_cfg<false, AT, BT, DUAL, Small>(g, epi, st);
+}
+
+// Tile and k-runs of a product.  The large tile where its tiles fill most of
+// the 256 CUs; where they do not and the sum is long, its k-steps are cut into
+// runs of at least kMinRun steps; what is still short of blocks takes the
+// small tile (two blocks per CU).
+constexpr int kMinRun = 8, kMaxSplit = 16;
+struct Plan {
+  bool big;
+  int split;
+};
+static inline Plan gemm_plan(int64_t M, int64_t N, int64_t steps, bool may_split) {
+  const int64_t tb = ceil_div(M, Big::BM) * ceil_div(N, Big::BN), ts = ceil_div(M, Small::BM) * ceil_div(N, Small::BN);
+  if (tb >= 192) return Plan{true, 1};
+  const int64_t most = may_split ? std::min<int64_t>(kMaxSplit, std::max<int64_t>(1, steps / kMinRun)) : 1;
+  const int64_t sb = std::min(most, 256 / tb);
+  if (tb * sb >= 192) return Plan{true, static_cast<int>(sb)};
+  return Plan{false, static_cast<int>(std::max<int64_t>(1, std::min(most, 512 / ts)))};
+}
+static inline int64_t ksteps(int64_t K, int nseg) { return ceil_div(K, kGemmK) * nseg; }
+
+// An operand as the product reads it: 16-bit planes (one, or three of a float32 tensor).
+struct Mat {
+  const uint16_t* plane[3];
+  int64_t ld;
+};
+
+// Whether a 16-bit tensor can be read where it is.
+static inline bool in_place(const void* p, int64_t ld, int64_t cols, int32_t dtype) {
+  return dtype != P2P_DTYPE_F32 && aligned_to(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld <= kMaxPitch;
+}
+static inline int64_t round_up(int64_t n, int64_t to) { return ceil_div(n, to) * to; }
+static inline int planes_of(int32_t dtype) { return dtype == P2P_DTYPE_F32 ? 3 : 1; }
+static inline int64_t packed_bytes(int64_t rows, int64_t cols, int32_t dtype) {
+  return round_up(rows * round_up(cols, 8) * 2 * planes_of(dtype), 256);
+}
+
+// src [rows, cols], pitch ld, as 16-bit planes of pitch round_up(cols, 8), zeros in the added columns.
+P2P_INTERNAL int32_t pack_matrix(const void* src, int64_t ld, int64_t rows, int64_t cols, int32_t dtype, uint16_t* dst, Mat* out,
+                                 hipStream_t st);
+// out[i] = alpha * (parts[i] + parts[stride + i] + ...) in that order
+P2P_INTERNAL int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, const float* scale0,
+                                const float* scale1, float alpha, void* out, int32_t dtype, hipStream_t st);
+
+// The pairs of a product of two operands, appended to g (DUAL: b2 too).
+static inline void add_pairs(GemmArgs* g, const Mat& a, const Mat& b, const Mat* b2, int32_t dtype) {
+  const int n = dtype == P2P_DTYPE_F32 ? 6 : 1;
+  for (int i = 0; i < n; ++i) {
+    const int pa = n == 1 ? 0 : kSplitA[i], pb = n == 1 ? 0 : kSplitB[i];
+    g->a[g->nseg] = a.plane[pa];
+    g->b[g->nseg] = b.plane[pb];
+    g->b2[g->nseg] = b2 ? b2->plane[pb] : nullptr;
+    ++g->nseg;
+  }
+}
+
+// Bytes handed out of a workspace; with base null it only counts them.
+struct Carver {
+  char* base;
+  int64_t used = 0;
+  void* take(int64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += round_up(bytes, 256);
+    return p;
+  }
+};
+
+}  // namespace p2p

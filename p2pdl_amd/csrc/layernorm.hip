@@ -1,0 +1,322 @@
+// K7 -- layer norm of a trainer's local step, forward and backward.
+//
+//   y  = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   dx = rstd * (g - mean(g) - xh * mean(g * xh)),  g = dy * w, xh = (x - mean) * rstd
+//   dw = sum over rows of dy * xh,  db = sum over rows of dy
+//
+// HBM-bound (about 20 operations for 8 bytes of a 16-bit element), so every
+// element is moved once: a team of lanes holds a whole row in registers, 16
+// bytes per lane and load, and takes the mean and then the squared
+// deviations from what it holds (the two-pass variance, without a second
+// read and without the cancellation of E[x^2] - mean^2).  The backward pass
+// keeps dw and db of its columns in registers over all rows of a block and
+// writes one partial row per block; a second kernel adds the partials in
+// their order, so the gradients' bits do not depend on timing.
+#include "train_common.h"
+
+namespace p2p {
+
+constexpr int kLnMaxCols = 16384;
+constexpr int kLnFwdBlock = 256;
+constexpr int kLnBwdBlock = 512;
+constexpr int kLnMaxParts = 512;  // partial rows of dw / db: two blocks of 512 lanes per CU
+
+// Sum over a team of TEAM lanes (one wave, or several through LDS: then every
+// lane of the block must call it).
+template <int TEAM, int BLOCK>
+__device__ __forceinline__ float team_sum(float v, float* scratch) {
+  v = wave_sum(v);
+  if constexpr (TEAM > 64) {
+    constexpr int W = TEAM / 64;
+    const int wave = threadIdx.x / 64;
+    __syncthreads();  // the scratch of the last sum has been read
+    if ((threadIdx.x & 63) == 0) scratch[wave] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v += scratch[(wave / W) * W + i];
+  }
+  return v;
+}
+
+template <typename T, int TEAM, int NV>
+__global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layernorm_fwd_kernel(
+    const T* x, int64_t ldx, const T* w, const T* b, int64_t rows, int cols, float eps, T* y, float* mean_out,
+    float* rstd_out) {
+  constexpr int BLOCK = kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock;
+  constexpr int V = Vec16<T>::N;
+  __shared__ float scratch[BLOCK / 64];
+  const int lane = threadIdx.x % TEAM;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (BLOCK / TEAM) + threadIdx.x / TEAM;
+  const int have = row < rows ? cols : 0;  // surplus teams of the last block hold an empty row
+  const T* xr = x + row * ldx;
+  float v[NV][V];
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_row<T, V>(xr, (i * TEAM + lane) * V, have, v[i]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s += v[i][e];
+  }
+  const float mean = team_sum<TEAM, BLOCK>(s, scratch) / static_cast<float>(cols);
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float d = (i * TEAM + lane) * V + e < have ? v[i][e] - mean : 0.f;
+      v[i][e] = d;
+      s += d * d;
+    }
+  const float rstd = 1.f / sqrtf(team_sum<TEAM, BLOCK>(s, scratch) / static_cast<float>(cols) + eps);
+  if (row >= rows) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TEAM + lane) * V;
+    if (c >= cols) continue;
+    float wv[V], bv[V], o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) wv[e] = 1.f, bv[e] = 0.f;
+    if (w) load_row<T, V>(w, c, cols, wv);
+    if (b) load_row<T, V>(b, c, cols, bv);
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = v[i][e] * rstd * wv[e] + bv[e];
+    store_row<T, V>(y + row * cols, c, cols, o);
+  }
+  if (lane == 0) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+}
+
+// Block q takes the rows (it * gridDim.x + q) * teams + team; parts[q] is its
+// row of 2 * cols sums: dw, then db.
+template <typename T, int TEAM, int NV>
+__global__ __launch_bounds__(kLnBwdBlock) void layernorm_bwd_kernel(const T* dy, int64_t lddy, const T* x, int64_t ldx,
+                                                                    const T* w, const float* mean_in,
+                                                                    const float* rstd_in, int64_t rows, int cols,
+                                                                    T* dx, float* parts) {
+  constexpr int V = Vec16<T>::N;
+  constexpr int TEAMS = kLnBwdBlock / TEAM;
+  __shared__ float scratch[2][kLnBwdBlock / 64];
+  __shared__ float joined[TEAMS > 1 ? TEAM * V : 1];
+  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  float dwv[NV][V], dbv[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) dwv[i][e] = 0.f, dbv[i][e] = 0.f;
+  const float inv = 1.f / static_cast<float>(cols);
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * TEAMS; first < rows;
+       first += static_cast<int64_t>(gridDim.x) * TEAMS) {
+    const int64_t row = first + team;
+    const int have = row < rows ? cols : 0;
+    const float mean = have ? ldg(mean_in + row) : 0.f, rstd = have ? ldg(rstd_in + row) : 0.f;
+    float xh[NV][V], g[NV][V];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TEAM + lane) * V;
+      load_row<T, V>(x + row * ldx, c, have, xh[i]);
+      load_row<T, V>(dy + row * lddy, c, have, g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TEAM + lane) * V;
+      float wv[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) wv[e] = 1.f;
+      if (w) load_row<T, V>(w, c, cols, wv);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float h = c + e < have ? (xh[i][e] - mean) * rstd : 0.f;
+        const float d = g[i][e];
+        dwv[i][e] += d * h;
+        dbv[i][e] += d;
+        xh[i][e] = h;
+        g[i][e] = d * wv[e];
+        s1 += g[i][e];
+        s2 += g[i][e] * h;
+      }
+    }
+    s1 = team_sum<TEAM, kLnBwdBlock>(s1, scratch[0]) * inv;
+    s2 = team_sum<TEAM, kLnBwdBlock>(s2, scratch[1]) * inv;
+    if (have) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TEAM + lane) * V;
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = rstd * (g[i][e] - s1 - xh[i][e] * s2);
+        if (c < cols) store_row<T, V>(dx + row * cols, c, cols, o);
+      }
+    }
+  }
+  if (!parts) return;
+  float* out = parts + static_cast<int64_t>(blockIdx.x) * 2 * cols;
+  // the teams' sums of each column, added in team order by the first team
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float (&v)[V] = which ? dbv[i] : dwv[i];
+      if constexpr (TEAMS > 1) {
+        for (int t = 1; t < TEAMS; ++t) {
+          __syncthreads();
+          if (team == t)
+#pragma unroll
+            for (int e = 0; e < V; ++e) joined[e * TEAM + lane] = v[e];
+          __syncthreads();
+          if (team == 0)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += joined[e * TEAM + lane];
+        }
+      }
+      const int c = (i * TEAM + lane) * V;
+      if (team == 0 && c < cols) store_row<float, V>(out + which * cols, c, cols, v);
+    }
+}
+
+// dw / db from the partial rows: 64 columns per block, 16 groups of rows.
+template <typename T>
+__global__ __launch_bounds__(1024) void layernorm_parts_kernel(const float* parts, int nparts, int cols, T* dw, T* db) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float s = 0.f;
+  if (c < 2 * static_cast<int64_t>(cols)) {
+#pragma unroll 8
+    for (int p = group; p < nparts; p += 16) s += ldg(parts + static_cast<int64_t>(p) * 2 * cols + c);
+  }
+  sums[group][lane] = s;
+  __syncthreads();
+  if (group || c >= 2 * static_cast<int64_t>(cols)) return;
+#pragma unroll
+  for (int q = 1; q < 16; ++q) s += sums[q][lane];
+  if (c < cols) {
+    if (dw) dw[c] = static_cast<T>(s);
+  } else if (db) {
+    db[c - cols] = static_cast<T>(s);
+  }
+}
+
+// Team and vectors per lane by the row's 16-byte vectors: one wave up to 128
+// of them, then 256 lanes, then 512 -- the registers of the backward pass
+// (4 floats per element) stay under 256 per lane.
+template <typename T, typename F>
+static void ln_team(int cols, F&& go) {
+  const int vecs = static_cast<int>(ceil_div(cols, Vec16<T>::N));
+  if (vecs <= 64) go(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+  else if (vecs <= 128) go(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+  else if (vecs <= 256) go(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+  else if (vecs <= 512) go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+  else if (vecs <= 1024) go(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
+  else if (vecs <= 2048) go(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
+  else if constexpr (sizeof(T) == 4) go(std::integral_constant<int, 512>(), std::integral_constant<int, 8>());
+}
+
+static int ln_parts(int64_t rows, int cols, int32_t dtype) {
+  const int vecs = static_cast<int>(ceil_div(cols, 16 / dtype_bytes(dtype)));
+  const int teams = kLnBwdBlock / (vecs <= 128 ? 64 : vecs <= 512 ? 256 : 512);
+  const int64_t blocks = ceil_div(rows, teams);
+  return static_cast<int>(blocks < kLnMaxParts ? blocks : kLnMaxParts);
+}
+
+template <typename T>
+static int32_t ln_fwd(const T* x, int64_t ldx, const T* w, const T* b, int64_t rows, int cols, float eps, T* y,
+                      float* mean, float* rstd, hipStream_t st) {
+  ln_team<T>(cols, [&](auto team, auto nv) {
+    constexpr int TEAM = decltype(team)::value, BLOCK = kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock;
+    layernorm_fwd_kernel<T, TEAM, decltype(nv)::value>
+        <<<dim3(static_cast<unsigned>(ceil_div(rows, BLOCK / TEAM))), dim3(BLOCK), 0, st>>>(x, ldx, w, b, rows, cols, eps,
+                                                                                           y, mean, rstd);
+  });
+  return launch_status();
+}
+
+template <typename T>
+static int32_t ln_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, const float* mean,
+                      const float* rstd, int64_t rows, int cols, T* dx, T* dw, T* db, float* parts, int32_t dtype,
+                      hipStream_t st) {
+  const int n = ln_parts(rows, cols, dtype);
+  float* const to = dw || db ? parts : nullptr;
+  ln_team<T>(cols, [&](auto team, auto nv) {
+    layernorm_bwd_kernel<T, decltype(team)::value, decltype(nv)::value>
+        <<<dim3(n), dim3(kLnBwdBlock), 0, st>>>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, to);
+  });
+  const int32_t rc = launch_status();
+  if (rc != P2P_OK || !to) return rc;
+  layernorm_parts_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(2 * static_cast<int64_t>(cols), 64))), dim3(1024), 0, st>>>(
+      parts, n, cols, dw, db);
+  return launch_status();
+}
+
+static int32_t ln_check(const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t dtype) {
+  if (!known_dtype(dtype) || rows < 0 || cols < 1 || ldx < cols) return P2P_ERR_INVALID;
+  if (cols > kLnMaxCols || rows > (int64_t(1) << 31) - 1) return P2P_ERR_UNSUPPORTED;
+  if (rows > 0 && !x) return P2P_ERR_INVALID;
+  if (!aligned_to(x, dtype_bytes(dtype))) return P2P_ERR_ALIGN;
+  return P2P_OK;
+}
+
+}  // namespace p2p
+
+using namespace p2p;
+
+extern "C" int32_t p2p_layernorm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int64_t rows,
+                                     int64_t cols, float eps, void* y, float* mean, float* rstd, int32_t dtype,
+                                     p2p_stream_t stream) {
+  const int32_t rc = ln_check(x, ldx, rows, cols, dtype);
+  if (rc != P2P_OK || rows == 0) return rc;
+  if (!y || !mean || !rstd) return P2P_ERR_INVALID;
+  if (!aligned_to(y, dtype_bytes(dtype)) || !aligned_to(w, dtype_bytes(dtype)) || !aligned_to(b, dtype_bytes(dtype)) ||
+      !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+    return P2P_ERR_ALIGN;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int c = static_cast<int>(cols);
+  if (dtype == P2P_DTYPE_F32)
+    return ln_fwd(static_cast<const float*>(x), ldx, static_cast<const float*>(w), static_cast<const float*>(b), rows, c,
+                  eps, static_cast<float*>(y), mean, rstd, st);
+  if (dtype == P2P_DTYPE_F16)
+    return ln_fwd(static_cast<const f16*>(x), ldx, static_cast<const f16*>(w), static_cast<const f16*>(b), rows, c, eps,
+                  static_cast<f16*>(y), mean, rstd, st);
+  return ln_fwd(static_cast<const bf16*>(x), ldx, static_cast<const bf16*>(w), static_cast<const bf16*>(b), rows, c, eps,
+                static_cast<bf16*>(y), mean, rstd, st);
+}
+
+extern "C" int64_t p2p_layernorm_bwd_workspace(int64_t rows, int64_t cols, int32_t dtype) {
+  if (!known_dtype(dtype) || rows < 0 || cols < 1 || cols > kLnMaxCols) return P2P_ERR_INVALID;
+  return static_cast<int64_t>(ln_parts(rows, static_cast<int>(cols), dtype)) * 2 * cols * 4;
+}
+
+extern "C" int32_t p2p_layernorm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
+                                     const float* mean, const float* rstd, int64_t rows, int64_t cols, void* dx,
+                                     void* dw, void* db, void* workspace, int64_t workspace_bytes, int32_t dtype,
+                                     p2p_stream_t stream) {
+  int32_t rc = ln_check(x, ldx, rows, cols, dtype);
+  if (rc == P2P_OK) rc = ln_check(dy, lddy, rows, cols, dtype);
+  if (rc != P2P_OK) return rc;
+  // no rows: dw and db are empty sums, which the caller clears (nothing is launched)
+  if (rows == 0) return P2P_OK;
+  if (!mean || !rstd || !dx) return P2P_ERR_INVALID;
+  if (dw || db) {
+    if (!workspace || workspace_bytes < p2p_layernorm_bwd_workspace(rows, cols, dtype)) return P2P_ERR_INVALID;
+    if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
+  }
+  const int s = dtype_bytes(dtype);
+  if (!aligned_to(dx, s) || !aligned_to(w, s) || !aligned_to(dw, s) || !aligned_to(db, s) || !aligned_to(mean, 4) ||
+      !aligned_to(rstd, 4))
+    return P2P_ERR_ALIGN;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int c = static_cast<int>(cols);
+  float* parts = static_cast<float*>(workspace);
+  if (dtype == P2P_DTYPE_F32)
+    return ln_bwd(static_cast<const float*>(dy), lddy, static_cast<const float*>(x), ldx, static_cast<const float*>(w),
+                  mean, rstd, rows, c, static_cast<float*>(dx), static_cast<float*>(dw), static_cast<float*>(db), parts,
+                  dtype, st);
+  if (dtype == P2P_DTYPE_F16)
+    return ln_bwd(static_cast<const f16*>(dy), lddy, static_cast<const f16*>(x), ldx, static_cast<const f16*>(w), mean,
+                  rstd, rows, c, static_cast<f16*>(dx), static_cast<f16*>(dw), static_cast<f16*>(db), parts, dtype, st);
+  return ln_bwd(static_cast<const bf16*>(dy), lddy, static_cast<const bf16*>(x), ldx, static_cast<const bf16*>(w), mean,
+                rstd, rows, c, static_cast<bf16*>(dx), static_cast<bf16*>(dw), static_cast<bf16*>(db), parts, dtype, st);
+}

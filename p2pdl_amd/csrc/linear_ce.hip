@@ -1,0 +1,394 @@
+// K10 -- softmax cross entropy of a linear head over a large vocabulary, its
+// logits never kept, with its gradient.
+//
+//   z = x W^T                                  x [T, H], W [V, H]
+//   lse_t = log sum_v exp(z_tv),  loss = norm * sum_t (lse_t - z_t,target(t))
+//   d_tv = exp(z_tv - lse_t) - [v = target(t)]
+//   dx = s * d W,  dW = s * d^T x,  s = dloss * norm
+// over the tokens whose target is not `ignore_index`; norm = 1 / their count
+// (mean; 0 where there is none) or 1 (sum).
+//
+// Matrix-bound.  Forward: the product's epilogue keeps, per token and 256
+// columns, the maximum and the sum of exponentials of its accumulators and
+// the target's logit; a second kernel joins those in column order.
+// Backward: the vocabulary in pieces, each piece's logits computed again
+// (one product of then four), turned in the epilogue into d in the operand
+// type, and read by the two gradient products out of one buffer of at most
+// half a gigabyte.  dx is summed over the pieces in 32 bits; dW's rows belong
+// to one piece each.
+//
+// d is rounded to x's type once (float32: not, three planes).  It lies in
+// [-1, 1]; for float16 it is held times 2^14, else the 1 / V of a
+// large vocabulary would sit among float16's subnormal numbers; s and 2^-14
+// are applied to the 32-bit sums.  A target outside [0, V) that is not
+// ignore_index makes the loss and both gradients NaN and reads nothing.
+#include "gemm_tile.h"
+
+namespace p2p {
+
+constexpr int64_t kPieceBytes = int64_t(512) << 20;
+constexpr float kHalfScale = 16384.f;
+
+// Per token and tile of columns: (maximum, sum of exp(z - maximum)).
+struct StatsEpi {
+  float2* part;        // [column tile][T]
+  float* at_target;    // [T]
+  const int64_t* target;
+  int64_t first;       // vocabulary index of column 0
+  int precise;
+
+  template <class Cfg>
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
+    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+    float2* rows = reinterpret_cast<float2*>(lds);  // [WN][BM]
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+      const int64_t m = p.m0 + i * 16 + i16;
+      const int64_t t = m < g.M ? ldg(target + m) - first - p.n0 : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = j * 16 + q4 + e;
+          if (p.n0 + n >= g.N) acc[i][j][e] = -INFINITY;
+          else if (n == t) stg(at_target + m, acc[i][j][e]);
+          top = fmaxf(top, acc[i][j][e]);  // passes over a NaN, which the sum below takes up
+        }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float base = top == -INFINITY ? 0.f : top;  // -inf throughout: a sum of zeros
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = acc[i][j][e] - base;
+          s += p.n0 + j * 16 + q4 + e < g.N ? (precise ? expf(x) : __expf(x)) : 0.f;
+        }
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      if (p.lane < 16) rows[p.wn * Cfg::BM + p.wm * Cfg::TM + i * 16 + i16] = make_float2(top, s);
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < Cfg::BM; r += Cfg::THREADS) {
+      const int64_t m = static_cast<int64_t>(p.tm) * Cfg::BM + r;
+      if (m >= g.M) continue;
+      float2 a = rows[r];
+#pragma unroll
+      for (int w = 1; w < Cfg::WN; ++w) {
+        const float2 b = rows[w * Cfg::BM + r];
+        a = join_stats(a, b);
+      }
+      part[p.tn * g.M + m] = a;
+    }
+  }
+
+  // A part without a finite logit is (-inf, 0) and adds nothing.
+  static __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
+    if (b.y == 0.f && b.x == -INFINITY) return a;
+    if (a.y == 0.f && a.x == -INFINITY) return b;
+    const float top = fmaxf(a.x, b.x);
+    return make_float2(top, a.y * expf(a.x - top) + b.y * expf(b.x - top));
+  }
+};
+
+// Joins the column tiles of a piece, and with what earlier pieces left in
+// `state`; after the last piece, lse and the token's loss.  64 tokens per
+// block, 4 lanes of column tiles each.
+__global__ __launch_bounds__(kBlock) void ce_join_kernel(const float2* part, int tiles, int64_t T, float2* state, int first,
+                                                         int last, const int64_t* target, int64_t V, int64_t ignore,
+                                                         const float* at_target, float* lse, float* row_loss) {
+  __shared__ float2 groups[4][64];
+  const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float2 a = make_float2(-INFINITY, 0.f);
+  if (t < T) {
+    const int from = tiles * group / 4, to = tiles * (group + 1) / 4;
+#pragma unroll 4
+    for (int i = from; i < to; ++i) a = StatsEpi::join_stats(a, part[i * T + t]);
+  }
+  groups[group][lane] = a;
+  __syncthreads();
+  if (group || t >= T) return;
+#pragma unroll
+  for (int q = 1; q < 4; ++q) a = StatsEpi::join_stats(a, groups[q][lane]);
+  if (!first) a = StatsEpi::join_stats(state[t], a);
+  if (!last) {
+    state[t] = a;
+    return;
+  }
+  const float l = a.x + logf(a.y);
+  lse[t] = l;
+  const int64_t y = target[t];
+  // z - max and log(sum) apart: lse - z would lose the digits of a large maximum
+  row_loss[t] = y == ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at_target[t] - a.x);
+}
+
+// loss and norm, by one block in a fixed order, in 64 bits.
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* row_loss, const int64_t* target, int64_t T, int64_t ignore,
+                                                       int mean, float* loss, float* norm) {
+  __shared__ double sums[1024];
+  __shared__ int64_t counts[1024];
+  double s = 0.0;
+  int64_t n = 0;
+  for (int64_t t = threadIdx.x; t < T; t += 1024) {
+    s += static_cast<double>(row_loss[t]);
+    n += target[t] != ignore;
+  }
+  sums[threadIdx.x] = s;
+  counts[threadIdx.x] = n;
+  for (int o = 512; o > 0; o >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < o) {
+      sums[threadIdx.x] += sums[threadIdx.x + o];
+      counts[threadIdx.x] += counts[threadIdx.x + o];
+    }
+  }
+  if (threadIdx.x == 0) {
+    const double f = !mean ? 1.0 : counts[0] ? 1.0 / static_cast<double>(counts[0]) : 0.0;
+    *loss = static_cast<float>(mean && counts[0] ? sums[0] / static_cast<double>(counts[0]) : sums[0]);
+    *norm = static_cast<float>(f);
+  }
+}
+
+// d of a piece into its buffer [T, pitch] (planes `plane` elements apart).
+struct GradEpi {
+  uint16_t* d;
+  int64_t pitch, plane;
+  const float* lse;
+  const int64_t* target;
+  int64_t first, vocab, ignore;
+  int32_t dtype;
+
+  template <class Cfg>
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char*) const {
+    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+      const int64_t m = p.m0 + i * 16 + i16;
+      if (m >= g.M) continue;
+      const int64_t y = ldg(target + m);
+      const bool counts = y != ignore;
+      const float l = y >= 0 && y < vocab ? ldg(lse + m) : NAN;
+      const int64_t t = y - first;
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j) {
+        const int64_t n = p.n0 + j * 16 + q4;
+        if (n >= pitch) continue;
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = acc[i][j][e] - l;
+          const float pr = dtype == P2P_DTYPE_F32 ? expf(x) : __expf(x);
+          v[e] = counts && n + e < g.N ? (n + e == t ? pr - 1.f : pr) : 0.f;
+        }
+        uint16_t* to = d + m * pitch + n;
+        if (dtype == P2P_DTYPE_F32) {
+          Pack<uint16_t, 4> o[3];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const Planes s = split3(v[e]);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) o[q].v[e] = s.p[q];
+          }
+#pragma unroll
+          for (int q = 0; q < 3; ++q) store_pack<uint16_t, 4>(to + q * plane, o[q]);
+        } else if (dtype == P2P_DTYPE_F16) {
+          store4(reinterpret_cast<f16*>(to), 0, 4, v * kHalfScale);
+        } else {
+          store4(reinterpret_cast<bf16*>(to), 0, 4, v);
+        }
+      }
+    }
+  }
+};
+
+static int32_t ce_check(const p2p_linear_ce_t* a) {
+  if (!a || !known_dtype(a->dtype) || a->tokens < 0 || a->hidden < 1 || a->vocab < 1 || a->ldx < a->hidden ||
+      a->ldw < a->hidden)
+    return P2P_ERR_INVALID;
+  const int64_t most = (int64_t(1) << 31) - 256;
+  if (a->hidden > kMaxPitch - 8 || a->vocab > most || a->tokens > most) return P2P_ERR_UNSUPPORTED;
+  if (!a->w || (a->tokens > 0 && (!a->x || !a->target || !a->lse)) || !a->norm) return P2P_ERR_INVALID;
+  const int s = dtype_bytes(a->dtype);
+  if (!aligned_to(a->x, s) || !aligned_to(a->w, s) || !aligned_to(a->target, 8) || !aligned_to(a->lse, 4) ||
+      !aligned_to(a->norm, 4))
+    return P2P_ERR_ALIGN;
+  return P2P_OK;
+}
+
+struct CeSpace {
+  bool x_here, w_here;
+  int64_t piece;      // vocabulary rows per piece
+  uint16_t *x, *w;    // packed x; packed rows of one piece of W
+  // forward
+  float2 *part, *state;
+  float *at_target, *row_loss;
+  // backward
+  uint16_t* d;
+  float* dx_parts;
+  Plan dx_plan;
+  int64_t dw_floats;
+  float* dw_parts;
+};
+
+static Plan ce_dw_plan(const p2p_linear_ce_t& a, int64_t rows) {
+  return gemm_plan(rows, a.hidden, ksteps(a.tokens, a.dtype == P2P_DTYPE_F32 ? 6 : 1), true);
+}
+
+static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeSpace* s) {
+  Carver c{static_cast<char*>(base)};
+  const int planes = planes_of(a.dtype);
+  s->x_here = in_place(a.x, a.ldx, a.hidden, a.dtype);
+  s->w_here = in_place(a.w, a.ldw, a.hidden, a.dtype);
+  // pieces: the buffers that grow with one stay under kPieceBytes (one tile's columns at least)
+  int64_t per_row = backward ? a.tokens * 2 * planes : ceil_div(a.tokens * 8, Small::BN);
+  if (!s->w_here) per_row = std::max(per_row, round_up(a.hidden, 8) * 2 * planes);
+  int64_t piece = std::max<int64_t>(1, kPieceBytes / per_row / Big::BN) * Big::BN;
+  if (piece >= a.vocab) piece = a.vocab;
+  else piece = round_up(ceil_div(a.vocab, ceil_div(a.vocab, piece)), Big::BN);  // pieces of about one size
+  s->piece = piece;
+  s->x = s->x_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(a.tokens, a.hidden, a.dtype)));
+  s->w = s->w_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(piece, a.hidden, a.dtype)));
+  if (!backward) {
+    s->part = static_cast<float2*>(c.take(ceil_div(piece, Small::BN) * a.tokens * 8));
+    s->state = static_cast<float2*>(c.take(a.tokens * 8));
+    s->at_target = static_cast<float*>(c.take(a.tokens * 4));
+    s->row_loss = static_cast<float*>(c.take(a.tokens * 4));
+    return c.used;
+  }
+  const int nseg = a.dtype == P2P_DTYPE_F32 ? 6 : 1;
+  s->d = static_cast<uint16_t*>(c.take(a.tokens * round_up(piece, 8) * 2 * planes));
+  s->dx_plan = gemm_plan(a.tokens, a.hidden, ksteps(piece, nseg), true);
+  const bool parts = s->dx_plan.split > 1 || piece < a.vocab;
+  s->dx_parts = parts ? static_cast<float*>(c.take(s->dx_plan.split * a.tokens * a.hidden * 4)) : nullptr;
+  s->dw_floats = 0;
+  for (const int64_t rows : {piece, a.vocab - (ceil_div(a.vocab, piece) - 1) * piece}) {
+    const Plan pw = ce_dw_plan(a, rows);
+    if (pw.split > 1) s->dw_floats = std::max(s->dw_floats, pw.split * rows * a.hidden);
+  }
+  s->dw_parts = s->dw_floats ? static_cast<float*>(c.take(s->dw_floats * 4)) : nullptr;
+  return c.used;
+}
+
+static int32_t ce_x(const p2p_linear_ce_t& a, const CeSpace& s, Mat* x, hipStream_t st) {
+  if (!s.x_here) return pack_matrix(a.x, a.ldx, a.tokens, a.hidden, a.dtype, s.x, x, st);
+  *x = Mat{{static_cast<const uint16_t*>(a.x), nullptr, nullptr}, a.ldx};
+  return P2P_OK;
+}
+static int32_t ce_w(const p2p_linear_ce_t& a, const CeSpace& s, int64_t v0, int64_t rows, Mat* w, hipStream_t st) {
+  const char* p = static_cast<const char*>(a.w) + v0 * a.ldw * dtype_bytes(a.dtype);
+  if (!s.w_here) return pack_matrix(p, a.ldw, rows, a.hidden, a.dtype, s.w, w, st);
+  *w = Mat{{reinterpret_cast<const uint16_t*>(p), nullptr, nullptr}, a.ldw};
+  return P2P_OK;
+}
+
+}  // namespace p2p
+
+using namespace p2p;
+
+extern "C" int64_t p2p_linear_ce_workspace(const p2p_linear_ce_t* a, int32_t backward) {
+  const int32_t rc = ce_check(a);
+  if (rc != P2P_OK) return rc;
+  CeSpace s;
+  return a->tokens ? ce_carve(*a, backward != 0, nullptr, &s) : 0;
+}
+
+extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, int64_t workspace_bytes,
+                                     p2p_stream_t stream) {
+  int32_t rc = ce_check(a);
+  if (rc != P2P_OK) return rc;
+  if (!a->loss) return P2P_ERR_INVALID;
+  if (!aligned_to(a->loss, 4)) return P2P_ERR_ALIGN;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a->tokens == 0) {  // the empty sum
+    ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(nullptr, nullptr, 0, a->ignore_index, a->mean, a->loss, a->norm);
+    return launch_status();
+  }
+  CeSpace s;
+  if (ce_carve(*a, false, workspace, &s) > workspace_bytes || !workspace) return P2P_ERR_INVALID;
+  if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
+  Mat x, w;
+  if ((rc = ce_x(*a, s, &x, st)) != P2P_OK) return rc;
+  for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
+    const int64_t rows = std::min(s.piece, a->vocab - v0);
+    if ((rc = ce_w(*a, s, v0, rows, &w, st)) != P2P_OK) return rc;
+    GemmArgs g{};
+    add_pairs(&g, x, w, nullptr, a->dtype);
+    g.lda = x.ld, g.ldb = w.ld;
+    g.M = a->tokens, g.N = rows, g.K = a->hidden;
+    g.ksplit = 1;
+    const StatsEpi e{s.part, s.at_target, a->target, v0, a->dtype == P2P_DTYPE_F32};
+    const bool big = gemm_plan(g.M, g.N, ksteps(g.K, g.nseg), false).big;
+    if ((rc = gemm_launch<false, false, false>(g, a->dtype == P2P_DTYPE_F16, big, e, st)) != P2P_OK) return rc;
+    const int tiles = static_cast<int>(ceil_div(rows, big ? Big::BN : Small::BN));
+    ce_join_kernel<<<dim3(static_cast<unsigned>(ceil_div(a->tokens, 64))), dim3(kBlock), 0, st>>>(
+        s.part, tiles, a->tokens, s.state, v0 == 0, v0 + rows == a->vocab, a->target, a->vocab, a->ignore_index, s.at_target,
+        a->lse, s.row_loss);
+    if ((rc = launch_status()) != P2P_OK) return rc;
+  }
+  ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, a->target, a->tokens, a->ignore_index, a->mean, a->loss, a->norm);
+  return launch_status();
+}
+
+extern "C" int32_t p2p_linear_ce_bwd(const p2p_linear_ce_t* a, void* workspace, int64_t workspace_bytes,
+                                     p2p_stream_t stream) {
+  int32_t rc = ce_check(a);
+  if (rc != P2P_OK || a->tokens == 0) return rc;
+  const int size = dtype_bytes(a->dtype);
+  if (!a->dx || !a->dw) return P2P_ERR_INVALID;
+  if (!aligned_to(a->dx, size) || !aligned_to(a->dw, size) || !aligned_to(a->dloss, 4)) return P2P_ERR_ALIGN;
+  CeSpace s;
+  if (ce_carve(*a, true, workspace, &s) > workspace_bytes || !workspace) return P2P_ERR_INVALID;
+  if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool f16_ = a->dtype == P2P_DTYPE_F16;
+  const float alpha = f16_ ? 1.f / kHalfScale : 1.f;
+  Mat x, w;
+  if ((rc = ce_x(*a, s, &x, st)) != P2P_OK) return rc;
+  for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
+    const int64_t rows = std::min(s.piece, a->vocab - v0), pitch = round_up(rows, 8), plane = a->tokens * pitch;
+    if ((rc = ce_w(*a, s, v0, rows, &w, st)) != P2P_OK) return rc;
+    {
+      GemmArgs g{};
+      add_pairs(&g, x, w, nullptr, a->dtype);
+      g.lda = x.ld, g.ldb = w.ld;
+      g.M = a->tokens, g.N = rows, g.K = a->hidden;
+      g.ksplit = 1;
+      const GradEpi e{s.d, pitch, plane, a->lse, a->target, v0, a->vocab, a->ignore_index, a->dtype};
+      const bool big = gemm_plan(g.M, g.N, ksteps(g.K, g.nseg), false).big;
+      if ((rc = gemm_launch<false, false, false>(g, f16_, big, e, st)) != P2P_OK) return rc;
+    }
+    const Mat d{{s.d, s.d + plane, s.d + 2 * plane}, pitch};
+    {  // dx += d W
+      GemmArgs g{};
+      add_pairs(&g, d, w, nullptr, a->dtype);
+      g.lda = pitch, g.ldb = w.ld;
+      g.M = a->tokens, g.N = a->hidden, g.K = rows;
+      g.ksplit = s.dx_plan.split;
+      const StoreEpi e{{a->dx, nullptr}, 0, 0, a->hidden, a->dtype, {a->norm, a->dloss}, alpha, s.dx_parts, v0 > 0};
+      if ((rc = gemm_launch<false, true, false>(g, f16_, s.dx_plan.big, e, st)) != P2P_OK) return rc;
+    }
+    {  // dW of the piece = d^T x
+      GemmArgs g{};
+      add_pairs(&g, d, x, nullptr, a->dtype);
+      g.lda = pitch, g.ldb = x.ld;
+      g.M = rows, g.N = a->hidden, g.K = a->tokens;
+      const Plan plan = ce_dw_plan(*a, rows);
+      g.ksplit = plan.split;
+      void* out = static_cast<char*>(a->dw) + v0 * a->hidden * size;
+      const StoreEpi e{{out, nullptr}, 0, 0, a->hidden, a->dtype, {a->norm, a->dloss}, alpha,
+                       plan.split > 1 ? s.dw_parts : nullptr, 0};
+      if ((rc = gemm_launch<true, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
+      if (plan.split > 1 && (rc = join_parts(s.dw_parts, plan.split, g.M * g.N, g.M * g.N, a->norm, a->dloss, alpha, out,
+                                             a->dtype, st)) != P2P_OK)
+        return rc;
+    }
+  }
+  if (s.dx_parts) {
+    const int64_t n = a->tokens * a->hidden;
+    return join_parts(s.dx_parts, s.dx_plan.split, n, n, a->norm, a->dloss, alpha, a->dx, a->dtype, st);
+  }
+  return P2P_OK;
+}

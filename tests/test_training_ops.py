@@ -1,0 +1,1005 @@
+"""The operators of a trainer's local step (p2pdl_amd/training.py) against plain 64-bit forms.
+
+Tolerances are bounds, element by element, derived from how the kernels round: u(T) =
+eps(T) / 2 for each rounding to the type T, U = 2^-24 for each 32-bit operation, and for
+a sum of n terms n * U * (the sum of their magnitudes).  A float32 product on three
+bf16 planes leaves out at most 2^-22 of |a| |b|.
+"""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from p2pdl_amd import _native as N
+from p2pdl_amd import training as T
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+gpu = pytest.mark.gpu
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    """Half a step among the subnormal numbers."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+def check(got, want, bound, what):
+    """|got - want| <= bound everywhere, where both are finite; the same elsewhere."""
+    got, want, bound = got.detach().double().cpu(), want.double().cpu(), bound.double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert not torch.isnan(got).any() or torch.equal(torch.isnan(got), torch.isnan(want)), what
+    over = (got - want).abs() - bound
+    bad = over > 0
+    assert not bad.any(), (what, int(bad.sum()), float((got - want).abs()[bad].max()), float(bound[bad].min()))
+
+
+def rounded(want, err, dtype):
+    """The bound after a value with error `err` is rounded to `dtype`."""
+    return err + u(dtype) * (want.abs() + err) + tiny(dtype)
+
+
+def randn(shape, dtype, seed, scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g, dtype=torch.float64) * scale + shift).to(dtype).cuda()
+
+
+def same_bits(a, b):
+    return a.dtype == b.dtype and a.shape == b.shape and torch.equal(
+        a.detach().reshape(-1).contiguous().view(torch.uint8), b.detach().reshape(-1).contiguous().view(torch.uint8))
+
+
+def replayed(step, keep, times=3):
+    """Runs step() eagerly, captures it and replays it with eager work between: every replay's outputs
+    have the eager bits.  keep: what step() returns, copied."""
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(times):
+        for t in out:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert same_bits(a, b), keep
+        for a, b in zip(step(), want):
+            assert same_bits(a, b), keep
+
+
+# ------------------------------------------------------------------ the C ABI's refusals (no GPU)
+def test_layernorm_arguments_without_gpu():
+    L = N.load_library()
+    ok = 1 << 12  # an address that no refused call reads
+    assert L.p2p_layernorm_fwd(ok, 8, None, None, 1, 8, 1e-5, ok, ok, ok, 3, None) == -1  # no such type
+    assert L.p2p_layernorm_fwd(ok, 7, None, None, 1, 8, 1e-5, ok, ok, ok, 0, None) == -1  # pitch < row
+    assert L.p2p_layernorm_fwd(None, 8, None, None, 1, 8, 1e-5, ok, ok, ok, 0, None) == -1
+    assert L.p2p_layernorm_fwd(ok, 8, None, None, 1, 8, 1e-5, None, ok, ok, 0, None) == -1
+    assert L.p2p_layernorm_fwd(ok, 16385, None, None, 1, 16385, 1e-5, ok, ok, ok, 0, None) == -2
+    assert L.p2p_layernorm_fwd(ok + 2, 8, None, None, 1, 8, 1e-5, ok, ok, ok, 0, None) == -3
+    assert L.p2p_layernorm_fwd(None, 8, None, None, 0, 8, 1e-5, None, None, None, 0, None) == 0  # no rows: nothing
+    need = L.p2p_layernorm_bwd_workspace(100, 8, 0)
+    assert need > 0 and L.p2p_layernorm_bwd_workspace(1, 0, 0) < 0
+    assert L.p2p_layernorm_bwd(ok, 8, ok, 8, ok, ok, ok, 100, 8, ok, ok, ok, ok, need - 1, 0, None) == -1
+    assert L.p2p_layernorm_bwd(ok, 8, ok, 8, ok, ok, ok, 100, 8, ok, ok, ok, None, need, 0, None) == -1
+    assert L.p2p_layernorm_bwd(ok, 8, ok, 8, ok, ok, ok, 100, 8, None, ok, ok, ok, need, 0, None) == -1
+
+
+def test_dropout_arguments_without_gpu():
+    L = N.load_library()
+    ok = 1 << 12
+    for p in (-0.1, 1.1, float("nan")):
+        assert L.p2p_dropout(ok, None, 8, p, 1, 0, None, ok, 0, None) == -1
+    assert L.p2p_dropout(ok, None, 8, 0.5, 1, 0, None, ok, 9, None) == -1
+    assert L.p2p_dropout(None, None, 8, 0.5, 1, 0, None, ok, 0, None) == -1
+    assert L.p2p_dropout(ok + 1, None, 8, 0.5, 1, 0, None, ok, 1, None) == -3
+    assert L.p2p_dropout(ok, None, 8, 0.5, 1, 0, ok + 4, ok, 1, None) == -3
+    assert L.p2p_dropout(None, None, 0, 0.5, 1, 0, None, None, 0, None) == 0
+
+
+def gated_args(**more):
+    ok = 1 << 12
+    a = N.GatedLinearArgs(x=ok, w_gate=ok, w_up=ok, ldx=64, ldg=64, ldu=64, tokens=4, hidden=64, units=32, activation=0,
+                          dtype=2, h=ok, gate=ok, up=ok, dh=ok, lddh=32, dx=ok, dw_gate=ok, dw_up=ok)
+    for k, v in more.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_gated_linear_arguments_without_gpu():
+    L = N.load_library()
+    ok = 1 << 12
+    big = 1 << 40
+    for bad, rc in (({"dtype": 5}, -1), ({"activation": 3}, -1), ({"hidden": 0}, -1), ({"units": 0}, -1), ({"ldx": 63}, -1),
+                    ({"ldu": 63}, -1), ({"x": None}, -1), ({"w_up": None}, -1), ({"tokens": -1}, -1),
+                    ({"hidden": 1 << 22, "ldx": 1 << 22, "ldg": 1 << 22, "ldu": 1 << 22}, -2), ({"tokens": 1 << 31}, -2),
+                    ({"x": ok + 1}, -3)):
+        a = gated_args(**bad)
+        assert L.p2p_gated_linear_workspace(a, 1) == rc, bad
+        assert L.p2p_gated_linear_fwd(a, ok, big, None) == rc, bad
+        assert L.p2p_gated_linear_bwd(a, ok, big, None) == rc, bad
+    assert L.p2p_gated_linear_fwd(gated_args(h=None), ok, big, None) == -1
+    assert L.p2p_gated_linear_bwd(gated_args(gate=None), ok, big, None) == -1
+    assert L.p2p_gated_linear_bwd(gated_args(lddh=31), ok, big, None) == -1
+    assert L.p2p_gated_linear_bwd(gated_args(dw_up=None), ok, big, None) == -1
+    # aligned 16-bit operands are read in place; float32 and odd ones need their copies
+    assert L.p2p_gated_linear_workspace(gated_args(), 0) == 0
+    assert L.p2p_gated_linear_workspace(gated_args(dtype=0), 0) >= 3 * 2 * 64 * (4 + 32 + 32)
+    assert L.p2p_gated_linear_workspace(gated_args(x=ok + 2), 0) >= 2 * 64 * 4
+    need = L.p2p_gated_linear_workspace(gated_args(), 1)
+    assert need >= 4 * 64 * 2
+    assert L.p2p_gated_linear_bwd(gated_args(), ok, need - 1, None) == -1
+    assert L.p2p_gated_linear_bwd(gated_args(), None, need, None) == -1
+    assert L.p2p_gated_linear_bwd(gated_args(), ok + 8, need, None) == -3
+    assert L.p2p_gated_linear_fwd(gated_args(tokens=0, x=None), None, 0, None) == 0
+
+
+def ce_args(**more):
+    ok = 1 << 12
+    a = N.LinearCeArgs(x=ok, w=ok, target=ok, ldx=64, ldw=64, tokens=4, hidden=64, vocab=32, ignore_index=-100, mean=1,
+                       dtype=2, loss=ok, lse=ok, norm=ok, dloss=None, dx=ok, dw=ok)
+    for k, v in more.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_linear_ce_arguments_without_gpu():
+    L = N.load_library()
+    ok = 1 << 12
+    big = 1 << 50
+    for bad, rc in (({"dtype": 5}, -1), ({"vocab": 0}, -1), ({"hidden": 0}, -1), ({"ldw": 63}, -1), ({"w": None}, -1),
+                    ({"target": None}, -1), ({"lse": None}, -1), ({"norm": None}, -1), ({"vocab": 1 << 31}, -2),
+                    ({"hidden": 1 << 22, "ldx": 1 << 22, "ldw": 1 << 22}, -2), ({"target": ok + 4}, -3), ({"w": ok + 1}, -3)):
+        a = ce_args(**bad)
+        assert L.p2p_linear_ce_workspace(a, 0) == rc, bad
+        assert L.p2p_linear_ce_fwd(a, ok, big, None) == rc, bad
+        assert L.p2p_linear_ce_bwd(a, ok, big, None) == rc, bad
+    assert L.p2p_linear_ce_fwd(ce_args(loss=None), ok, big, None) == -1
+    assert L.p2p_linear_ce_bwd(ce_args(dw=None), ok, big, None) == -1
+    for backward, run in ((0, L.p2p_linear_ce_fwd), (1, L.p2p_linear_ce_bwd)):
+        need = L.p2p_linear_ce_workspace(ce_args(), backward)
+        assert need > 0
+        assert run(ce_args(), ok, need - 1, None) == -1
+        assert run(ce_args(), None, need, None) == -1
+        assert run(ce_args(), ok + 8, need, None) == -3
+    # the buffer of a piece of the vocabulary is bounded, whatever the vocabulary
+    assert L.p2p_linear_ce_workspace(ce_args(tokens=8192, vocab=1 << 20), 1) < (1 << 30)
+    assert L.p2p_linear_ce_workspace(ce_args(tokens=8192, vocab=1 << 20, dtype=0), 1) < (2 << 30)
+
+
+def test_struct_sizes_match_the_header():
+    """The binding's structs as the C compiler lays them out: natural alignment, no holes but the last."""
+    assert ctypes.sizeof(N.GatedLinearArgs) == 9 * 8 + 2 * 4 + 3 * 8 + 2 * 8 + 3 * 8
+    assert ctypes.sizeof(N.LinearCeArgs) == 9 * 8 + 2 * 4 + 6 * 8
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    calls = [lambda: T.layer_norm_forward(x), lambda: T.dropout_forward(x, 0.5, 1), lambda: T.gated_linear_forward(x, w, w),
+             lambda: T.linear_cross_entropy_forward(x, w, torch.zeros(2, dtype=torch.int64))]
+    for call in calls:
+        with pytest.raises(RuntimeError):
+            call()
+
+
+# ------------------------------------------------------------------ references in 64 bits
+def norm_reference(x, w, b, dy, eps):
+    """(values, error bounds before the last rounding) of y, dx, dw, db."""
+    x, dy = x.double().cpu(), dy.double().cpu()
+    cols, rows = x.shape[1], x.shape[0]
+    w64 = torch.ones(cols, dtype=torch.float64) if w is None else w.double().cpu()
+    b64 = torch.zeros(cols, dtype=torch.float64) if b is None else b.double().cpu()
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    xh = (x - mean) * rstd
+    g = dy * w64
+    s1, s2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+    # a lane adds at most 64 of a row's elements, then 6 steps of its wave and 8 waves
+    n = 80 * U
+    e_mean = n * x.abs().mean(1, keepdim=True)
+    # the variance around the computed mean: its own sum, and the (second-order) mean error
+    r_rstd = (0.5 * n + 8 * U) + 0.5 * (e_mean * rstd) ** 2
+    e_xh = rstd * (e_mean + 2 * U * (x - mean).abs()) + xh.abs() * r_rstd
+    y = xh * w64 + b64
+    e_y = w64.abs() * e_xh + 4 * U * ((xh * w64).abs() + b64.abs())
+    dx = rstd * (g - s1 - xh * s2)
+    e_s1 = n * g.abs().mean(1, keepdim=True)
+    e_s2 = (g.abs() * e_xh).mean(1, keepdim=True) + n * (g * xh).abs().mean(1, keepdim=True)
+    e_dx = rstd * (e_s1 + e_xh * s2.abs() + (xh.abs() + e_xh) * e_s2) \
+        + (6 * U + r_rstd) * rstd * (g.abs() + s1.abs() + (xh * s2).abs())
+    # rows of one block's lane, then the teams of a block, then 16 groups of at most 32 parts
+    adds = (math.ceil(rows / 512) + 8 + 32 + 16) * U
+    dw, e_dw = (dy * xh).sum(0), (dy.abs() * e_xh).sum(0) + (adds + 2 * U) * (dy * xh).abs().sum(0)
+    db, e_db = dy.sum(0), adds * dy.abs().sum(0)
+    return (y, dx, dw, db), (e_y, e_dx, e_dw, e_db)
+
+
+NORM_SHAPES = [(1, 1), (1, 8), (3, 5), (32, 512), (7, 513), (65, 1001), (33, 1024), (9, 2048), (5, 2049), (4, 4096),
+               (6, 4099), (3, 8192), (2, 16384), (3, 16383), (1500, 24)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES)
+def test_layer_norm(cuda, dtype, rows, cols):
+    x = randn((rows, cols), dtype, 1, 1.5, 0.25)
+    w, b, dy = randn((cols,), dtype, 2, 0.2, 1.0), randn((cols,), dtype, 3), randn((rows, cols), dtype, 4)
+    eps = 1e-5
+    for weight, bias in ((w, b), (None, None), (w, None)):
+        y, mean, rstd = T.layer_norm_forward(x, weight, bias, eps)
+        dx, dw, db = T.layer_norm_backward(dy, x, mean, rstd, weight)
+        want, err = norm_reference(x, weight, bias, dy, eps)
+        for got, v, e, name in zip((y, dx, dw, db), want, err, ("y", "dx", "dw", "db")):
+            if got is None:
+                assert weight is None and name in ("dw", "db")
+                continue
+            check(got, v, rounded(v, e, dtype), (name, rows, cols, weight is not None, bias is not None))
+        again = T.layer_norm_backward(dy, x, mean, rstd, weight)
+        assert all(a is b_ or same_bits(a, b_) for a, b_ in zip((dx, dw, db), again))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layer_norm_layouts(cuda, dtype):
+    """Pitched rows are read in place, other layouts copied: the bits of the dense call."""
+    wide = randn((40, 300), dtype, 5, 1.0, 3.0)
+    w, b = randn((129,), dtype, 6), randn((129,), dtype, 7)
+    views = [wide[:, 3:132], wide[::2, 1:130], wide.t()[:129].t(), wide[:, :258:2], wide[5, :129].expand(7, 129),
+             wide[:, :258].reshape(4, 10, 258)[:, :, 100:229]]
+    for v in views:
+        dense = v.clone(memory_format=torch.contiguous_format)
+        y, mean, rstd = T.layer_norm_forward(v, w, b)
+        y0, mean0, rstd0 = T.layer_norm_forward(dense, w, b)
+        assert y.shape == v.shape and mean.shape == v.shape[:-1]
+        assert same_bits(y, y0) and same_bits(mean, mean0) and same_bits(rstd, rstd0)
+        for g, g0 in zip(T.layer_norm_backward(v, v, mean, rstd, w), T.layer_norm_backward(dense, dense, mean0, rstd0, w)):
+            assert same_bits(g, g0)
+    x = wide[0, :129]
+    assert T.layer_norm_forward(x, w, b)[0].shape == (129,)
+
+
+@gpu
+def test_layer_norm_empty_and_not_finite(cuda):
+    w = randn((16,), torch.float32, 8)
+    y, mean, rstd = T.layer_norm_forward(torch.empty(0, 16, device="cuda"), w, w)
+    dx, dw, db = T.layer_norm_backward(y, y, mean, rstd, w)
+    assert y.shape == dx.shape == (0, 16) and torch.equal(dw, torch.zeros_like(w)) and torch.equal(db, torch.zeros_like(w))
+    x = randn((5, 16), torch.float32, 9)
+    clean = T.layer_norm_forward(x, w, w)[0]
+    x[1, 3], x[3, 0] = float("nan"), float("inf")
+    y, mean, rstd = T.layer_norm_forward(x, w, w)
+    assert torch.isnan(y[[1, 3]]).all() and same_bits(y[[0, 2, 4]], clean[[0, 2, 4]])  # rows do not mix
+    same = torch.full((3, 16), 7.0, device="cuda")  # no variance: eps alone
+    y, mean, rstd = T.layer_norm_forward(same, w, w, 1e-5)
+    assert torch.equal(y, w.expand(3, 16))
+
+
+@gpu
+def test_layer_norm_large_offset(cuda):
+    """A mean far from 0 costs the variance no digits (two passes over the held row)."""
+    x = randn((8, 512), torch.float32, 10, 1.0, 4096.0)
+    dy = randn((8, 512), torch.float32, 11)
+    y, mean, rstd = T.layer_norm_forward(x)
+    dx, _, _ = T.layer_norm_backward(dy, x, mean, rstd)
+    want, err = norm_reference(x, None, None, dy, 1e-5)
+    check(y, want[0], rounded(want[0], err[0], torch.float32), "y")
+    check(dx, want[1], rounded(want[1], err[1], torch.float32), "dx")
+
+
+@gpu
+def test_layer_norm_many_rows(cuda):
+    """More rows than partial sums, so that a block keeps several; rows past 2^16."""
+    x, dy = randn((70001, 40), torch.bfloat16, 12), randn((70001, 40), torch.bfloat16, 13)
+    w = randn((40,), torch.bfloat16, 14)
+    y, mean, rstd = T.layer_norm_forward(x, w)
+    got = T.layer_norm_backward(dy, x, mean, rstd, w)
+    want, err = norm_reference(x, w, None, dy, 1e-5)
+    for g, v, e, name in zip((y,) + got, want, err, ("y", "dx", "dw", "db")):
+        check(g, v, rounded(v, e, torch.bfloat16), name)
+
+
+# ------------------------------------------------------------------ dropout
+def philox_words(seed, blocks):
+    """Philox4x32-10 in Python integers: the four words of each block."""
+    out = []
+    for block in blocks:
+        c = [block & 0xFFFFFFFF, (block >> 32) & 0xFFFFFFFF, 0, 0]
+        k = [seed & 0xFFFFFFFF, seed >> 32]
+        for _ in range(10):
+            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+        out.append(c)
+    return out
+
+
+def kept(seed, offset, n, p):
+    words = [w for c in philox_words(seed, [(offset + i) % (1 << 64) for i in range((n + 3) // 4)]) for w in c][:n]
+    return torch.tensor([w >= int(p * 2 ** 32) and p < 1 for w in words], dtype=torch.bool)
+
+
+def test_philox_known_answers():
+    """The generator's published vectors (Random123's kat_vectors, philox4x32 10 rounds): zero counter and key."""
+    assert philox_words(0, [0]) == [[0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,p,seed,offset", [(1, 0.5, 0, 0), (3, 0.5, 1, 5), (4, 0.25, 2, 0), (1000, 0.1, 0xDEADBEEFCAFEF00D, (1 << 32) - 3),
+                                             (4099, 0.9, (1 << 64) - 1, (1 << 64) - 7), (777, 0.0, 3, 4), (777, 1.0, 3, 4),
+                                             (2051, 1 - 2.0 ** -33, 3, 4)])
+def test_dropout(cuda, dtype, n, p, seed, offset):
+    x, r = randn((n,), dtype, 20), randn((n,), dtype, 21)
+    keep = kept(seed, offset, n, p)
+    scale = 1 / (1 - p) if p < 1 else 0.0
+    want = torch.where(keep, x.double().cpu() * scale, 0.0)
+    y = T.dropout_forward(x, p, seed, offset)
+    assert torch.equal(y.cpu()[~keep], torch.zeros(int((~keep).sum()), dtype=dtype))
+    ok = want.abs() < torch.finfo(dtype).max  # a scale of 2^33 leaves float16
+    check(y.cpu()[ok], want[ok], rounded(want, 3 * U * want.abs(), dtype)[ok], "y")  # scale's and the product's rounding
+    assert same_bits(T.dropout_backward(x, p, seed, offset), y)
+    yr = T.dropout_forward(x, p, seed, offset, residual=r)
+    total = want + r.double().cpu()
+    ok = total.abs() < torch.finfo(dtype).max
+    check(yr.cpu()[ok], total[ok], rounded(total, 4 * U * (want.abs() + r.double().cpu().abs()), dtype)[ok], "y + residual")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dropout_layouts_and_values(cuda, dtype):
+    """The mask goes by the element's place in row-major order, whatever the memory; what is dropped is 0."""
+    x = randn((37, 50), dtype, 22)
+    y = T.dropout_forward(x, 0.3, 9, 100)
+    assert same_bits(T.dropout_forward(x.t().contiguous().t(), 0.3, 9, 100), y)
+    assert same_bits(T.dropout_forward(x.reshape(-1), 0.3, 9, 100).view(37, 50), y)
+    buf = torch.zeros(37 * 50 + 1, dtype=dtype, device="cuda")
+    buf[1:] = x.reshape(-1)
+    assert same_bits(T.dropout_forward(buf[1:], 0.3, 9, 100).view(37, 50), y)  # element-aligned only
+    # the counters of the second half of the elements
+    assert same_bits(T.dropout_forward(x.reshape(-1)[1000:], 0.3, 9, 100 + T.dropout_blocks(1000)), y.reshape(-1)[1000:])
+    bad = torch.full((2000,), float("nan"), dtype=dtype, device="cuda")
+    keep = kept(9, 100, 2000, 0.3)
+    y = T.dropout_forward(bad, 0.3, 9, 100).cpu()
+    assert torch.isnan(y[keep]).all() and (y[~keep] == 0).all()
+    at = torch.tensor([100], dtype=torch.int64, device="cuda")
+    assert same_bits(T.dropout_forward(x, 0.3, 9, at), T.dropout_forward(x, 0.3, 9, 100))
+    assert T.dropout_forward(x[:0], 0.3, 9).shape == (0, 50)
+
+
+@gpu
+def test_dropout_share(cuda):
+    """2^24 elements: the share kept is 1 - p within five standard deviations, and of pairs of neighbours too."""
+    x = torch.ones(1 << 24, device="cuda")
+    for p in (0.1, 0.5, 0.9):
+        m = T.dropout_forward(x, p, 77, 1 << 40) != 0
+        share, pairs = m.double().mean().item(), (m[1:] & m[:-1]).double().mean().item()
+        q = 1 - p
+        assert abs(share - q) < 5 * math.sqrt(p * q / x.numel())
+        # neighbouring pairs overlap: their mean's variance is at most 3 q^2 (1 - q^2) / n
+        assert abs(pairs - q * q) < 5 * math.sqrt(3 * q * q * (1 - q * q) / x.numel())
+
+
+# ------------------------------------------------------------------ products
+def product(a, b, k, dtype):
+    """(a @ b, bound of its 32-bit sum over k terms); float32 on planes leaves out 2^-22."""
+    c = a @ b
+    return c, ((k + 8) * U + (2.0 ** -22 if dtype == torch.float32 else 0)) * (a.abs() @ b.abs())
+
+
+def act64(name, g):
+    if name == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if name == "gelu":
+        phi = 0.5 * (1 + torch.erf(g / math.sqrt(2)))
+        return g * phi, phi + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    return torch.relu(g), (g > 0).double()
+
+
+# |act'| and |act''| at most, and the 32-bit evaluation's error as a multiple of U * (1 + |g|)
+SLOPE = {"silu": (1.1, 0.5), "gelu": (1.13, 0.8), "relu": (1.0, 0.0)}
+
+
+def gated_reference(x, wg, wu, dh, act):
+    """Values and bounds (before the last rounding) of h, dx, dwg, dwu; no g within its bound of relu's corner."""
+    dtype = x.dtype
+    x, wg, wu, dh = (t.double().cpu() for t in (x, wg, wu, dh))
+    rows, cols = x.shape
+    units = wg.shape[0]
+    g, e_g = product(x, wg.t(), cols, dtype)
+    v, e_v = product(x, wu.t(), cols, dtype)
+    a, da = act64(act, g)
+    s1, s2 = SLOPE[act]
+    e_a = s1 * e_g + 16 * U * (1 + g.abs())
+    e_da = s2 * e_g + 16 * U * (1 + g.abs())
+    if act == "relu":
+        e_da = (g.abs() <= e_g).double()
+    h, e_h = a * v, a.abs() * e_v + v.abs() * e_a + e_a * e_v + 2 * U * (a * v).abs()
+    dg, du = dh * v * da, dh * a
+    e_dg = dh.abs() * (e_v * da.abs() + v.abs() * e_da + e_v * e_da) + 4 * U * dg.abs()
+    e_du = dh.abs() * e_a + 4 * U * du.abs()
+    if dtype != torch.float32:  # rounded once as operands
+        e_dg, e_du = rounded(dg, e_dg, dtype), rounded(du, e_du, dtype)
+
+    def grad(p, q, e_p, n):
+        c, e = product(p, q, n, dtype)
+        return c, e + (e_p @ q.abs()) * (1 + 1e-3)
+
+    dx1, e1 = grad(dg, wg, e_dg, 2 * units)
+    dx2, e2 = grad(du, wu, e_du, 2 * units)
+    dwg, e_dwg = grad(dg.t(), x, e_dg.t(), rows)
+    dwu, e_dwu = grad(du.t(), x, e_du.t(), rows)
+    return (h, dx1 + dx2, dwg, dwu), (e_h, e1 + e2, e_dwg, e_dwu)
+
+
+GATED_SHAPES = [(1, 1, 1), (1, 64, 16), (2, 8, 8), (5, 7, 3), (32, 784, 512), (65, 100, 33), (128, 128, 64), (129, 136, 72),
+                (300, 257, 130), (1, 1000, 777), (257, 72, 1000), (40, 2048, 24)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,units", GATED_SHAPES)
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_linear(cuda, dtype, rows, cols, units, act):
+    x, dh = randn((rows, cols), dtype, 30), randn((rows, units), dtype, 31)
+    wg, wu = randn((units, cols), dtype, 32, cols ** -0.5), randn((units, cols), dtype, 33, cols ** -0.5)
+    h, gate, up = T.gated_linear_forward(x, wg, wu, act)
+    got = (h,) + T.gated_linear_backward(dh, x, wg, wu, gate, up, act)
+    want, err = gated_reference(x, wg, wu, dh, act)
+    for o, v, e, name in zip(got, want, err, ("h", "dx", "dwg", "dwu")):
+        check(o, v, rounded(v, e, dtype), (name, rows, cols, units))
+    h2, none, none2 = T.gated_linear_forward(x, wg, wu, act, save=False)
+    assert none is None and none2 is None and same_bits(h, h2)
+    for a, b in zip(got[1:], T.gated_linear_backward(dh, x, wg, wu, gate, up, act)):
+        assert same_bits(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,units", [(2048, 2048, 1024), (4100, 520, 264), (96, 512, 8192), (3000, 256, 128)])
+def test_gated_linear_large_tiles(cuda, dtype, rows, cols, units):
+    """Sizes whose products take the large tile, several tiles in each direction, or runs of the sum."""
+    x, dh = randn((rows, cols), dtype, 34), randn((rows, units), dtype, 35)
+    wg, wu = randn((units, cols), dtype, 36, cols ** -0.5), randn((units, cols), dtype, 37, cols ** -0.5)
+    h, gate, up = T.gated_linear_forward(x, wg, wu)
+    got = (h,) + T.gated_linear_backward(dh, x, wg, wu, gate, up)
+    want, err = gated_reference(x, wg, wu, dh, "silu")
+    for o, v, e, name in zip(got, want, err, ("h", "dx", "dwg", "dwu")):
+        check(o, v, rounded(v, e, dtype), name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_linear_layouts(cuda, dtype):
+    """Pitches, element-aligned bases, expanded gradients, more dimensions: the bits of the dense call."""
+    rows, cols, units = 30, 72, 40
+    wide = randn((rows, 3 * cols + 8), dtype, 38)
+    ww = randn((2 * units, cols + 16), dtype, 39, 0.1)
+    dh = randn((rows, units), dtype, 40)
+    for x, wg, wu in ((wide[:, 8:8 + cols], ww[:units, :cols], ww[units:, :cols]),
+                      (wide[:, 3:3 + cols], ww[:units, 5:5 + cols], ww[units:, 8:8 + cols]),
+                      (wide[:, :2 * cols:2], ww[::2, :cols], ww[1::2, :cols])):
+        dense = [t.clone(memory_format=torch.contiguous_format) for t in (x, wg, wu)]
+        h, gate, up = T.gated_linear_forward(x, wg, wu)
+        h0, gate0, up0 = T.gated_linear_forward(*dense)
+        assert same_bits(h, h0) and same_bits(gate, gate0) and same_bits(up, up0)
+        for a, b in zip(T.gated_linear_backward(dh, x, wg, wu, gate, up),
+                        T.gated_linear_backward(dh, *dense, gate0, up0)):
+            assert same_bits(a, b)
+        one = dh[0].expand(rows, units)
+        for a, b in zip(T.gated_linear_backward(one, x, wg, wu, gate, up),
+                        T.gated_linear_backward(one.contiguous(), *dense, gate0, up0)):
+            assert same_bits(a, b)
+        h3, _, _ = T.gated_linear_forward(dense[0].view(5, 6, cols), wg, wu)
+        assert h3.shape == (5, 6, units) and same_bits(h3.view(rows, units), h)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_linear_guards(cuda, dtype):
+    """NaN all round the operands, in the pitch and behind the last row, reaches no result."""
+    rows, cols, units = 21, 40, 24
+    for cols_ in (cols, 37):
+        xs = torch.full((rows + 3, cols + 24), float("nan"), dtype=dtype, device="cuda")
+        ws = torch.full((2 * units + 3, cols + 24), float("nan"), dtype=dtype, device="cuda")
+        x, wg, wu = xs[1:1 + rows, 8:8 + cols_], ws[1:1 + units, 8:8 + cols_], ws[2 + units:2 + 2 * units, 8:8 + cols_]
+        for t, seed in ((x, 41), (wg, 42), (wu, 43)):
+            t.copy_(randn(t.shape, dtype, seed, 0.2))
+        dh = randn((rows, units), dtype, 44)
+        h, gate, up = T.gated_linear_forward(x, wg, wu)
+        out = (h, gate, up) + T.gated_linear_backward(dh, x, wg, wu, gate, up)
+        assert all(torch.isfinite(t).all() for t in out)
+    e = T.gated_linear_forward(x[:0], wg, wu)
+    assert e[0].shape == (0, units)
+    dx, dwg, dwu = T.gated_linear_backward(dh[:0], x[:0], wg, wu, e[1], e[2])
+    assert dx.shape == (0, 37) and not dwg.any() and not dwu.any()
+
+
+@gpu
+def test_gated_linear_float32_range(cuda):
+    """Planes of values at the ends of float32's range: finite ones stay so, others stay in their row."""
+    x = torch.zeros(4, 16, device="cuda")
+    w = torch.zeros(8, 16, device="cuda")
+    x[0, 0], x[1, 1], x[2, 2], x[3, 3] = torch.finfo(torch.float32).max, 1e-30, float("inf"), 2.0 ** -140
+    w[:, :4] = torch.tensor([0.5, 1.0, 1.0, 1.0], device="cuda")
+    h, gate, up = T.gated_linear_forward(x, w, w, "relu")
+    assert gate[0, 0].item() == np.float32(3.4028235e38) * np.float32(0.5)
+    assert abs(gate[1, 0].item() - 1e-30) <= 1e-30 * 2.0 ** -22
+    assert not torch.isfinite(gate[2]).any() and torch.isfinite(gate[[0, 1, 3]]).all()
+
+
+# ------------------------------------------------------------------ linear cross entropy
+def ce_reference(x, w, target, dloss, ignore, reduction):
+    """Values and bounds (before the last rounding) of loss, dx, dw."""
+    dtype = x.dtype
+    x, w, target = x.double().cpu(), w.double().cpu(), target.cpu()
+    rows, cols, vocab = x.shape[0], x.shape[1], w.shape[0]
+    z, e_z = product(x, w.t(), cols, dtype)
+    seen = target != ignore
+    t = torch.where(seen, target, 0)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p = torch.exp(z - lse)
+    # sums of exponentials: a lane's 16, its wave, 4 waves, then the column tiles and pieces, each
+    # with an exponential (its argument rounded: U * |argument|, and 2 U of its own)
+    spread = (z.amax(1, keepdim=True) - z.amin(1, keepdim=True)) + 1
+    e_lse = (p * e_z).sum(1, keepdim=True) * 1.01 + (32 + vocab / 64) * U + 4 * U * (spread * p).sum(1, keepdim=True) \
+        + 4 * U * lse.abs() + 8 * U
+    e_lse = e_lse + 4 * U * spread.amax()
+    count = int(seen.sum())
+    norm = (1.0 / count if count else 0.0) if reduction == "mean" else 1.0
+    row = torch.where(seen, lse[:, 0] - z.gather(1, t[:, None])[:, 0], 0.0)
+    e_row = torch.where(seen, e_lse[:, 0] + e_z.gather(1, t[:, None])[:, 0] + 4 * U * (row.abs() + spread[:, 0]), 0.0)
+    loss, e_loss = row.sum() * norm, e_row.sum() * norm
+    d = p.clone()
+    d[torch.arange(rows), t] -= 1
+    d *= seen[:, None]
+    e_d = (p * (e_z + e_lse + 4 * U * (z - lse).abs() + 8 * U) * 1.01 + 2 * U * d.abs()) * seen[:, None]
+    if dtype != torch.float32:  # rounded once as an operand; float16 holds it times 2^14
+        e_d = e_d + u(dtype) * (d.abs() + e_d) + tiny(dtype) * (2.0 ** -14 if dtype == torch.float16 else 1)
+    s = norm * dloss
+    out = []
+    for a, b, e_a, n in ((d, w, e_d, vocab), (d.t(), x, e_d.t(), rows)):
+        c, e = product(a, b, n, dtype)
+        out.append((c * s, (e + (e_a @ b.abs()) * (1 + 1e-3)) * abs(s) + 6 * U * c.abs() * abs(s)))
+    return (loss, out[0][0], out[1][0]), (e_loss, out[0][1], out[1][1])
+
+
+CE_SHAPES = [(1, 1, 1), (1, 64, 10), (3, 5, 2), (32, 256, 10), (33, 72, 1000), (65, 100, 333), (130, 128, 129), (257, 65, 513),
+             (7, 1001, 2050), (600, 96, 700)]
+
+
+def ce_inputs(rows, cols, vocab, dtype, seed, skip=0.25):
+    x, w = randn((rows, cols), dtype, seed), randn((vocab, cols), dtype, seed + 1, 2 * cols ** -0.5)
+    g = torch.Generator().manual_seed(seed + 2)
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    t[torch.rand(rows, generator=g) < skip] = -100
+    t[0] = vocab - 1
+    return x, w, t.cuda()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,vocab", CE_SHAPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_linear_cross_entropy(cuda, dtype, rows, cols, vocab, reduction):
+    x, w, t = ce_inputs(rows, cols, vocab, dtype, 50)
+    scale = 8.0 * rows if reduction == "mean" else 8.0
+    dloss = torch.tensor(scale, device="cuda")
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t, reduction=reduction)
+    got = (loss,) + T.linear_cross_entropy_backward(x, w, t, lse, norm, dloss)
+    want, err = ce_reference(x, w, t, scale, -100, reduction)
+    assert loss.dtype == torch.float32 and loss.dim() == 0
+    check(loss, want[0], rounded(want[0], err[0], torch.float32), "loss")
+    for o, v, e, name in zip(got[1:], want[1:], err[1:], ("dx", "dw")):
+        check(o, v, rounded(v, e, dtype), (name, rows, cols, vocab))
+    again = T.linear_cross_entropy_backward(x, w, t, lse, norm, dloss)
+    assert all(same_bits(a, b) for a, b in zip(got[1:], again))
+    assert (got[1][t == -100] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,vocab", [(2300, 256, 5000), (64, 264, 20001), (4096, 24, 40)])
+def test_linear_cross_entropy_large_tiles(cuda, dtype, rows, cols, vocab):
+    x, w, t = ce_inputs(rows, cols, vocab, dtype, 53)
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    dloss = torch.tensor(8.0 * rows, device="cuda")
+    got = T.linear_cross_entropy_backward(x, w, t, lse, norm, dloss)
+    want, err = ce_reference(x, w, t, 8.0 * rows, -100, "mean")
+    check(loss, want[0], rounded(want[0], err[0], torch.float32), "loss")
+    for o, v, e, name in zip(got, want[1:], err[1:], ("dx", "dw")):
+        check(o, v, rounded(v, e, dtype), name)
+
+
+@gpu
+def test_linear_cross_entropy_pieces(cuda):
+    """A vocabulary that the backward pass takes in several pieces, the last one short."""
+    rows, cols, vocab = 40000, 16, 14000
+    L = N.lib()
+    x, w, t = ce_inputs(rows, cols, vocab, torch.bfloat16, 56)
+    a, keep = T._ce_args(x, w, t, -100)
+    a.lse = a.norm = x.data_ptr()
+    assert L.p2p_linear_ce_workspace(a, 1) < 2 * rows * vocab  # fewer bytes than all of d: more than one piece
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    dx, dw = T.linear_cross_entropy_backward(x, w, t, lse, norm, torch.tensor(float(rows), device="cuda"))
+    z = x.double() @ w.double().t()
+    ref = torch.logsumexp(z, 1)
+    seen = t != -100
+    p = torch.exp(z - ref[:, None])
+    want_loss = ((ref - z.gather(1, t.clamp_min(0)[:, None])[:, 0]) * seen).sum() / seen.sum()
+    assert abs(loss.item() - want_loss.item()) <= 64 * U * want_loss.item()
+    p[torch.arange(rows, device="cuda"), t.clamp_min(0)] -= 1
+    p *= seen[:, None] * (rows / seen.sum())
+    ub = u(torch.bfloat16)
+    want = p @ w.double()
+    # d's rounding, the 32-bit sum and the last rounding
+    check(dx, want, rounded(want, (ub * 1.02 + vocab * U) * (p.abs() @ w.double().abs()), torch.bfloat16), "dx")
+    want = p.t() @ x.double()
+    check(dw, want, rounded(want, (ub * 1.02 + rows * U) * (p.t().abs() @ x.double().abs()), torch.bfloat16), "dw")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_cross_entropy_targets(cuda, dtype):
+    x, w, t = ce_inputs(40, 32, 50, dtype, 60)
+    # no token counts: a loss of 0 and gradients of 0
+    none = torch.full_like(t, -100)
+    for reduction in ("mean", "sum"):
+        loss, lse, norm = T.linear_cross_entropy_forward(x, w, none, reduction=reduction)
+        dx, dw = T.linear_cross_entropy_backward(x, w, none, lse, norm)
+        assert loss.item() == 0 and not dx.any() and not dw.any()
+    # an ignored token's row may hold anything
+    bad = x.clone()
+    t[3] = t[7] = -100
+    bad[3], bad[7, 5] = float("nan"), float("inf")
+    a, b = T.linear_cross_entropy_forward(x, w, t), T.linear_cross_entropy_forward(bad, w, t)
+    assert same_bits(a[0], b[0]) and torch.isfinite(b[0])
+    # (the NaN of such a row meets a d of 0 in dW's sum: 0 * NaN)
+    dx, _ = T.linear_cross_entropy_backward(bad, w, t, b[1], b[2])
+    assert same_bits(dx, T.linear_cross_entropy_backward(x, w, t, a[1], a[2])[0])
+    # ignore_index among the classes
+    c = t.clamp_min(0)
+    c[5] = 7
+    la, lb = (T.linear_cross_entropy_forward(x, w, v, ignore_index=i)[0] for v, i in ((c, 7), (torch.where(c == 7, -1, c), -1)))
+    assert same_bits(la, lb)
+    # a target outside the vocabulary: NaN, nothing read
+    for wrong in (50, -1, 1 << 40):
+        o = t.clone()
+        o[11] = wrong
+        loss, lse, norm = T.linear_cross_entropy_forward(x, w, o)
+        dx, dw = T.linear_cross_entropy_backward(x, w, o, lse, norm)
+        assert torch.isnan(loss) and torch.isnan(dx[11]).all() and torch.isfinite(dx[:11]).all() and torch.isnan(dw).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_cross_entropy_extreme_logits(cuda, dtype):
+    """Logits far apart, a class at minus infinity, large common offsets."""
+    x = torch.zeros(4, 16, dtype=dtype, device="cuda")
+    w = torch.zeros(300, 16, dtype=dtype, device="cuda")
+    x[:, 0] = 1
+    x[1, 1], x[2, 2] = 1, 1
+    w[5, 0], w[290, 1] = 28672.0, -28672.0
+    w[:, 2] = 1024.0
+    t = torch.tensor([5, 5, 4, 290], device="cuda")
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t, reduction="sum")
+    assert loss.item() == 57344.0  # 0, 0, and 28672 twice
+    dx, dw = T.linear_cross_entropy_backward(x, w, t, lse, norm)
+    assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+    if dtype == torch.float32:
+        return  # an infinity times a plane that is 0: NaN (documented)
+    w[:200, 0] = float("-inf")  # whole column parts without a finite logit
+    t = torch.tensor([250, 250, 250, -100], device="cuda")
+    loss, lse, norm = T.linear_cross_entropy_forward(x[:, :1], w[:, :1], t, reduction="sum")
+    assert abs(loss.item() - 3 * math.log(100)) <= 3 * 16 * U * math.log(100)
+    loss, _, _ = T.linear_cross_entropy_forward(x[:1, :1], w[:, :1], torch.tensor([0], device="cuda"))
+    assert loss.item() == float("inf")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_cross_entropy_layouts_and_guards(cuda, dtype):
+    rows, cols, vocab = 37, 48, 100
+    for cols_, shift in ((cols, 8), (45, 3)):
+        xs = torch.full((rows + 2, cols + 32), float("nan"), dtype=dtype, device="cuda")
+        ws = torch.full((vocab + 2, cols + 32), float("nan"), dtype=dtype, device="cuda")
+        x, w = xs[1:1 + rows, shift:shift + cols_], ws[1:1 + vocab, shift:shift + cols_]
+        x.copy_(randn(x.shape, dtype, 61))
+        w.copy_(randn(w.shape, dtype, 62, 0.3))
+        t = (torch.arange(2 * rows, device="cuda") % vocab)[::2]
+        dense = [v.clone(memory_format=torch.contiguous_format) for v in (x, w, t)]
+        a, b = T.linear_cross_entropy_forward(x, w, t), T.linear_cross_entropy_forward(*dense)
+        assert all(same_bits(p, q) for p, q in zip(a, b)) and torch.isfinite(a[0])
+        ga, gb = T.linear_cross_entropy_backward(x, w, t, *a[1:]), T.linear_cross_entropy_backward(*dense, *b[1:])
+        assert all(same_bits(p, q) for p, q in zip(ga, gb)) and all(torch.isfinite(g).all() for g in ga)
+    empty = T.linear_cross_entropy_forward(x[:0], w, t[:0])
+    assert empty[0].item() == 0
+    dx, dw = T.linear_cross_entropy_backward(x[:0], w, t[:0], *empty[1:])
+    assert dx.shape == (0, 45) and not dw.any()
+
+
+# ------------------------------------------------------------------ refusals of the Python entry points
+@gpu
+def test_refusals(cuda):
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    half, stat = x.half(), torch.zeros(4, device="cuda")
+    v = torch.zeros(8, device="cuda")
+    for err, call in [
+        (TypeError, lambda: T.layer_norm_forward(x.double())), (TypeError, lambda: T.layer_norm_forward(t.view(2, 2))),
+        (ValueError, lambda: T.layer_norm_forward(torch.zeros(2, 0, device="cuda"))),
+        (ValueError, lambda: T.layer_norm_forward(torch.zeros(2, 16385, device="cuda"))),
+        (ValueError, lambda: T.layer_norm_forward(x, None, v)), (ValueError, lambda: T.layer_norm_forward(x, v[:7])),
+        (TypeError, lambda: T.layer_norm_forward(half, v)), (RuntimeError, lambda: T.layer_norm_forward(x, v.cpu())),
+        (ValueError, lambda: T.layer_norm_backward(x[:3], x, stat, stat)),
+        (TypeError, lambda: T.layer_norm_backward(x, x, stat.double(), stat)),
+        (ValueError, lambda: T.layer_norm_backward(x, x, stat[:3], stat)),
+        (ValueError, lambda: T.dropout_forward(x, 1.5, 0)), (ValueError, lambda: T.dropout_forward(x, float("nan"), 0)),
+        (ValueError, lambda: T.dropout_forward(x, 0.5, -1)), (ValueError, lambda: T.dropout_forward(x, 0.5, 1 << 64)),
+        (ValueError, lambda: T.dropout_forward(x, 0.5, 0, -1)), (ValueError, lambda: T.dropout_forward(x, 0.5, 0, stat[:1])),
+        (ValueError, lambda: T.dropout_forward(x, 0.5, 0, t)), (ValueError, lambda: T.dropout_forward(x, 0.5, 0, t[:1].cpu())),
+        (ValueError, lambda: T.dropout_forward(x, 0.5, 0, residual=x[:3])),
+        (TypeError, lambda: T.dropout_forward(x, 0.5, 0, residual=half)),
+        (ValueError, lambda: T.gated_linear_forward(x, w, w, "tanh")), (ValueError, lambda: T.gated_linear_forward(x, w, w[:5])),
+        (ValueError, lambda: T.gated_linear_forward(x, w[:, :7], w[:, :7])), (TypeError, lambda: T.gated_linear_forward(x, w.half(), w)),
+        (ValueError, lambda: T.gated_linear_forward(x, w[:0], w[:0])), (RuntimeError, lambda: T.gated_linear_forward(x, w, w.cpu())),
+        (ValueError, lambda: T.gated_linear_backward(x, x, w, w, x, x)),
+        (TypeError, lambda: T.linear_cross_entropy_forward(x, w, t.int())),
+        (ValueError, lambda: T.linear_cross_entropy_forward(x, w, t[:3])),
+        (ValueError, lambda: T.linear_cross_entropy_forward(x, w, t, reduction="none")),
+        (ValueError, lambda: T.linear_cross_entropy_forward(x, w[0], t)), (RuntimeError, lambda: T.linear_cross_entropy_forward(x, w, t.cpu())),
+        (TypeError, lambda: T.linear_cross_entropy_forward(x, w.bfloat16(), t)),
+        (ValueError, lambda: T.linear_cross_entropy_backward(x, w, t, stat, stat[0], torch.tensor(1.0))),
+        (ValueError, lambda: T.linear_cross_entropy_backward(x, w, t, stat, stat)),
+    ]:
+        with pytest.raises(err):
+            call()
+
+
+# ------------------------------------------------------------------ graphs, streams, autograd
+def step_calls(dtype, rows=150, cols=264, units=136, vocab=1000):
+    x, w, b, dy = randn((rows, cols), dtype, 70), randn((cols,), dtype, 71), randn((cols,), dtype, 72), randn((rows, cols), dtype, 73)
+    wg, wu, dh = randn((units, cols), dtype, 74, 0.06), randn((units, cols), dtype, 75, 0.06), randn((rows, units), dtype, 76)
+    _, head, t = ce_inputs(rows, cols, vocab, dtype, 77)
+
+    def step():
+        y, mean, rstd = T.layer_norm_forward(x, w, b)
+        out = [y, *T.layer_norm_backward(dy, x, mean, rstd, w)]
+        out += [T.dropout_forward(x, 0.2, 5, 6, residual=dy), T.dropout_backward(dy, 0.2, 5, 6)]
+        h, gate, up = T.gated_linear_forward(x, wg, wu)
+        out += [h, *T.gated_linear_backward(dh, x, wg, wu, gate, up)]
+        loss, lse, norm = T.linear_cross_entropy_forward(x, head, t)
+        return out + [loss, *T.linear_cross_entropy_backward(x, head, t, lse, norm)]
+
+    return step
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_captured_step(cuda, dtype):
+    replayed(step_calls(dtype), str(dtype))
+
+
+@gpu
+def test_captured_dropout_advances(cuda):
+    """A counter on the device: each replay draws the next mask."""
+    x = randn((999,), torch.float32, 80)
+    at = torch.tensor([40], dtype=torch.int64, device="cuda")
+    T.dropout_forward(x, 0.5, 3, at)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = T.dropout_forward(x, 0.5, 3, at)
+        at.add_(T.dropout_blocks(x.numel()))
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same_bits(y, T.dropout_forward(x, 0.5, 3, 40 + 250 * k))
+
+
+@gpu
+def test_differentiable_forms_refuse_capture(cuda):
+    x, w = torch.zeros(4, 8, device="cuda", requires_grad=True), torch.zeros(6, 8, device="cuda")
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    keep = torch.zeros(1, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep.add_(1)
+        for call in (lambda: T.layer_norm(x), lambda: T.dropout(x, 0.5, 1), lambda: T.gated_linear(x, w, w),
+                     lambda: T.linear_cross_entropy(x, w, t)):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+        with torch.no_grad():
+            T.layer_norm(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert keep.item() == 1
+
+
+@gpu
+def test_side_stream(cuda):
+    """Calls on another stream than the default one, two at once, each with its own workspace."""
+    step = step_calls(torch.bfloat16)
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(step())
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for out in got:
+        assert all(same_bits(a, b) for a, b in zip(out, want))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_autograd_forms(cuda, dtype):
+    """The differentiable forms give what their pairs give; gradients of shared leaves add up."""
+    rows, cols, units, vocab = 20, 40, 24, 30
+    x = randn((rows, cols), dtype, 90).requires_grad_()
+    w, b = randn((cols,), dtype, 91).requires_grad_(), randn((cols,), dtype, 92).requires_grad_()
+    dy = randn((rows, cols), dtype, 93)
+    T.layer_norm(x, w, b).backward(dy)
+    _, mean, rstd = T.layer_norm_forward(x.detach(), w.detach(), b.detach())
+    for g, v in zip((x.grad, w.grad, b.grad), T.layer_norm_backward(dy, x.detach(), mean, rstd, w.detach())):
+        assert same_bits(g, v)
+    x.grad = None
+    at = torch.tensor([11], dtype=torch.int64, device="cuda")
+    r = randn((rows, cols), dtype, 94).requires_grad_()
+    y = T.dropout(x, 0.4, 8, at, residual=r)
+    at.add_(100)  # the counter moves on before the backward pass
+    y.backward(dy)
+    assert same_bits(x.grad, T.dropout_backward(dy, 0.4, 8, 11)) and same_bits(r.grad, dy)
+    x.grad = None
+    wg, wu = randn((units, cols), dtype, 95, 0.2).requires_grad_(), randn((units, cols), dtype, 96, 0.2).requires_grad_()
+    T.gated_linear(x, wg, wu, "gelu").sum().backward()  # an expanded gradient
+    _, gate, up = T.gated_linear_forward(x.detach(), wg.detach(), wu.detach(), "gelu")
+    one = torch.ones(rows, units, dtype=dtype, device="cuda")
+    for g, v in zip((x.grad, wg.grad, wu.grad),
+                    T.gated_linear_backward(one, x.detach(), wg.detach(), wu.detach(), gate, up, "gelu")):
+        assert same_bits(g, v)
+    x.grad = None
+    _, head, t = ce_inputs(rows, cols, vocab, dtype, 97)
+    head.requires_grad_()
+    (T.linear_cross_entropy(x, head, t) * 4.0).backward()
+    _, lse, norm = T.linear_cross_entropy_forward(x.detach(), head.detach(), t)
+    four = torch.tensor(4.0, device="cuda")
+    for g, v in zip((x.grad, head.grad), T.linear_cross_entropy_backward(x.detach(), head.detach(), t, lse, norm, four)):
+        assert same_bits(g, v)
+    # the same weight twice
+    wg.grad = None
+    T.gated_linear(x.detach(), wg, wg).backward(one)
+    _, gate, up = T.gated_linear_forward(x.detach(), wg.detach(), wg.detach())
+    _, a, c = T.gated_linear_backward(one, x.detach(), wg.detach(), wg.detach(), gate, up)
+    assert same_bits(wg.grad, a + c)
+
+
+@gpu
+def test_gradients_against_differences(cuda):
+    """float32: the directional derivative by central differences of the forward pass, summed in 64 bits.
+
+    f is a mean of squares or a loss near 1; a step of h = 2^-6 along a unit-sized direction: the
+    third-order term is h^2 / 6 times a third derivative, the rounding term 2^-22 / h of the terms' size."""
+    h = 2.0 ** -6
+    rows, cols, units, vocab = 16, 48, 32, 40
+    x, d = randn((rows, cols), torch.float32, 100), randn((rows, cols), torch.float32, 101)
+    d /= d.norm()
+    wn, bn = randn((cols,), torch.float32, 102), randn((cols,), torch.float32, 103)
+    wg, wu = randn((units, cols), torch.float32, 104, 0.15), randn((units, cols), torch.float32, 105, 0.15)
+    _, head, t = ce_inputs(rows, cols, vocab, torch.float32, 106)
+    c1, c2 = randn((rows, cols), torch.float32, 107), randn((rows, units), torch.float32, 108)
+    forms = {"layer_norm": lambda v: (T.layer_norm(v, wn, bn), c1), "dropout": lambda v: (T.dropout(v, 0.3, 4), c1),
+             "gated_linear": lambda v: (T.gated_linear(v, wg, wu), c2),
+             "linear_cross_entropy": lambda v: (T.linear_cross_entropy(v, head, t), torch.ones((), device="cuda"))}
+    for name, form in forms.items():
+        leaf = x.clone().requires_grad_()
+        y, c = form(leaf)
+        y.backward(c)
+        slope = (leaf.grad.double() * d.double()).sum().item()
+        ends = []
+        for s in (h, -h):
+            y, c = form(x + s * d)
+            ends.append((y.double() * c.double()).sum().item())
+        size = (y.double() * c.double()).abs().sum().item()
+        diff = (ends[0] - ends[1]) / (2 * h)
+        assert abs(diff - slope) <= h * h * 4 * (1 + abs(slope)) + 2.0 ** -22 * (size + 1) / h, (name, diff, slope)
+
+
+# ------------------------------------------------------------------ together, as a trainer uses them
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_local_step_to_aggregation(cuda, dtype):
+    """Three trainers run two steps of a small block and head on these operators, send their local updates
+    (K4), a tester aggregates them: every trainer's step run again gives the same bits, the gradients are
+    those of the same model in 64 bits, and the global model is the reference's op sequence on the deltas."""
+    import types
+
+    from p2pdl_amd.aggregator import aggregation as agg
+    from p2pdl_amd.node.local_update import compute_local_update
+
+    rows, cols, units, vocab = 96, 64, 80, 50
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            g = torch.Generator().manual_seed(5)
+            for name, shape, scale in (("norm_w", (cols,), 0.0), ("norm_b", (cols,), 0.0), ("gate", (units, cols), 0.12),
+                                       ("up", (units, cols), 0.12), ("down", (cols, units), 0.11), ("head", (vocab, cols), 0.12)):
+                v = torch.randn(shape, generator=g) * scale + (1.0 if name == "norm_w" else 0.0)
+                self.register_parameter(name, torch.nn.Parameter(v))
+
+        def loss(self, x, t, seed):
+            p = {k: v.to(dtype) for k, v in self.named_parameters()}
+            x = x.to(dtype)
+            h = T.gated_linear(T.layer_norm(x, p["norm_w"], p["norm_b"]), p["gate"], p["up"])
+            x = T.dropout(h @ p["down"].t(), 0.1, seed, residual=x)
+            return T.linear_cross_entropy(x, p["head"], t)
+
+        def loss64(self, x, t, seed):
+            p = {k: v.detach().double().cpu().requires_grad_() for k, v in self.named_parameters()}
+            x, t = x.double().cpu(), t.cpu()
+            n = torch.nn.functional.layer_norm(x, (cols,), p["norm_w"], p["norm_b"])
+            h = torch.nn.functional.silu(n @ p["gate"].t()) * (n @ p["up"].t())
+            m = kept(seed, 0, rows * cols, 0.1).reshape(rows, cols).double() / 0.9
+            loss = torch.nn.functional.cross_entropy((h @ p["down"].t() * m + x) @ p["head"].t(), t)
+            loss.backward()
+            return loss, {k: v.grad for k, v in p.items()}
+
+    def train(seed):
+        model = Block().cuda()
+        node = types.SimpleNamespace(model=model, previous_model_state={k: v.clone() for k, v in model.state_dict().items()})
+        opt = torch.optim.SGD(model.parameters(), lr=0.05)
+        g = torch.Generator().manual_seed(seed)
+        first = None
+        for step in range(2):
+            x = torch.randn(rows, cols, generator=g).cuda()
+            t = torch.randint(0, vocab, (rows,), generator=g).cuda()
+            opt.zero_grad()
+            want = model.loss64(x, t, seed * 10 + step) if step == 0 else None
+            loss = model.loss(x, t, seed * 10 + step)
+            loss.backward()
+            if step == 0:
+                first = (loss.item(), {k: v.grad.double().cpu() for k, v in model.named_parameters()}, want)
+            opt.step()
+        return compute_local_update(node), first
+
+    updates = []
+    # the whole chain rounds a handful of times per value: 2-norm errors of a few roundings of the type
+    few = 24 * u(dtype) if dtype == torch.bfloat16 else 256 * U
+    for seed in (1, 2, 3):
+        update, (loss, grads, (loss64, grads64)) = train(seed)
+        again, _ = train(seed)
+        assert all(same_bits(update[k], again[k]) for k in update)
+        assert abs(loss - loss64.item()) <= few * loss64.item()
+        for k, v in grads64.items():
+            assert (grads[k] - v).norm() <= few * v.norm(), (k, float((grads[k] - v).norm() / v.norm()))
+        updates.append({"model": update, "sender": ("127.0.0.1", seed)})
+    model = Block().cuda()
+    want = {k: v.clone() for k, v in model.state_dict().items()}
+    for k, v in want.items():
+        acc = torch.zeros_like(v).cpu()
+        for up in updates:
+            acc += up["model"][k].cpu()
+        acc /= 3
+        want[k] = v.cpu() + 0.1 * acc
+    node = types.SimpleNamespace(model=model, trainers_list=[0] * 3, addr="127.0.0.1", port=7000, neighbors=[],
+                                 received_models=updates)
+    agg.aggregate_models(node)
+    torch.cuda.synchronize()
+    for k, v in model.state_dict().items():
+        assert same_bits(v.cpu(), want[k]), k
