@@ -53,11 +53,11 @@ struct GatedEpi {
     const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + i * 16 + i16;
+      const int64_t m = p.m0 + Cfg::row(i) + i16;
       if (m >= g.M) continue;
 #pragma unroll
       for (int j = 0; j < Cfg::NJ; j += 2) {
-        const int64_t n = p.n0 / 2 + j * 8 + q4;
+        const int64_t n = (p.n0 + Cfg::col(j)) / 2 + q4;
         if (n >= units) continue;
         const f4 gv = acc[i][j], uv = acc[i][j + 1];
         f4 hv;

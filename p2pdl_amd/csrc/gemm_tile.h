@@ -17,13 +17,25 @@
 // rounding of a 32-bit sum.  Six bf16 products take 6/16 of the time of one on
 // the 32-bit matrix instructions.  A value that is not finite is its own hi.
 //
-// Tile.  BM x BN x 64, double-buffered in LDS (128 KiB for 256 x 256), filled
-// by LDS-DMA: a wave's instruction writes 1 KiB in lane order, so the
-// swizzles are made by choosing each lane's source address.  Lanes whose
-// source lies outside the operand get an offset past the descriptor's range
-// and write zeros.  One barrier per 64 k: the loads of step s + 1 are issued
-// after it and waited for before the next one, under the matrix
-// instructions of step s.
+// Tile.  BM x BN x 64 per k-step, the operands of two steps in LDS (128 KiB
+// for 256 x 256), filled by LDS-DMA: a wave's instruction writes 1 KiB in
+// lane order, so the swizzles are made by choosing each lane's source
+// address.  Lanes whose source lies outside the operand get an offset past
+// the descriptor's range and write zeros.
+//
+// Schedule.  Each operand's tile has two halves (rows), a wave owns a part of
+// every quadrant, and a k-step is four phases, one quadrant each:
+//   phase   products   reads into registers   requests (LDS-DMA)
+//     0     A0 B0      B1 of this step        B0 of the step after next
+//     1     A0 B1      A1 of this step        B1 of the step after next
+//     2     A1 B0      A0 of the next step    A1 of the step after next
+//     3     A1 B1      B0 of the next step    A0 of the third step on
+// A half is requested as soon as the last wave has read the one it replaces
+// (one barrier per phase) and is read seven phases later, so a request has
+// almost two k-steps to come back, and what is read in a phase is multiplied in
+// the next: the matrix instructions wait for neither.  Six halves stay in
+// flight over every wait.  Steps past the end request zeros, so that the
+// counts hold throughout.
 //
 // LDS images.  k-contiguous: rows of 128 bytes, 16-byte chunk c at position
 // c ^ (row / 2 % 8): the 16 lanes of one k-group, one row each, then hit the 64
@@ -64,15 +76,37 @@ template <int BM_, int BN_, int WM_, int WN_>
 struct GemmCfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-  static constexpr int TM = BM / WM, TN = BN / WN;  // a wave's part of the tile
-  static constexpr int MI = TM / 16, NJ = TN / 16;
-  static constexpr int A_BYTES = BM * kGemmK * 2, STAGE = (BM + BN) * kGemmK * 2;
+  static constexpr int HM = BM / 2, HN = BN / 2;          // the tile's halves
+  static constexpr int QM = HM / WM, QN = HN / WN;        // a wave's part of a half
+  static constexpr int MI = 2 * QM / 16, NJ = 2 * QN / 16;
+  static constexpr int A_HALF = HM * kGemmK * 2, B_HALF = HN * kGemmK * 2, STAGE = 2 * (A_HALF + B_HALF);
   static constexpr int BLOCKS_PER_CU = 2 * STAGE > 80 * 1024 ? 1 : 2;
+  static __host__ __device__ constexpr int row(int i) { return i / (MI / 2) * HM + i % (MI / 2) * 16; }
+  static __host__ __device__ constexpr int col(int j) { return j / (NJ / 2) * HN + j % (NJ / 2) * 16; }
 };
 using Big = GemmCfg<256, 256, 2, 4>;
 using Small = GemmCfg<128, 128, 2, 2>;
 
 constexpr uint32_t kOutside = 0x80000000u;
+using i4 = int __attribute__((ext_vector_type(4)));
+// 16 bytes per lane from base + voff to dst + 16 * lane (dst wave-uniform).  In
+// assembly: for the builtin the compiler waits for all requests before any
+// LDS read (970 against 1216 TFLOP/s at 8192 x 4096 x 32768).  The kernel
+// counts and waits itself; no register is written.  (Four idle cycles: the
+// compiler does not look into the block for an address that a vector
+// instruction has just made scalar.)
+__device__ __forceinline__ void lds_dma(const void* base, uint32_t voff, char* dst) {
+  const uint64_t b = uniform_u64(reinterpret_cast<uint64_t>(base));
+  const i4 rs = {static_cast<int>(b), static_cast<int>(b >> 32), static_cast<int>(kOutside), 0x00020000};
+  const uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((P2P_LDS void*)(dst))));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(voff), "s"(rs) : "memory");
+}
+
+template <int EXT>
+__device__ __forceinline__ int line_swizzle(int k) {
+  if constexpr (EXT >= 128) return ((k & 3) | (((k >> 3) & 3) << 2)) & (EXT / 16 - 1);
+  else return ((k >> 3) + (k & 2)) & 3;
+}
 
 // One operand's part of a stage.  EXT: rows of the tile, INSTS: 1-KiB
 // instructions per wave.
@@ -96,7 +130,7 @@ struct TileLoader {
         constexpr int CPL = EXT / 8;  // 16-byte chunks of a line
         const int k = q * (64 / CPL) + lane / CPL;
         const int pos = lane % CPL;
-        const int f = ((k & 3) | (((k >> 3) & 3) << 2)) & (EXT / 16 - 1);
+        const int f = line_swizzle<EXT>(k);
         const int m = ((pos >> 1) ^ f) * 16 + (pos & 1) * 8;
         kpos[j] = k;
         voff[j] = m < rows ? static_cast<uint32_t>(k * ld * 2 + m * 2) : kOutside;
@@ -106,12 +140,10 @@ struct TileLoader {
 
   // The k-step at `base` into the image at dst; `left`: k still in the segment.
   __device__ __forceinline__ void issue(const uint16_t* base, int64_t left, char* dst, int wave) const {
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, static_cast<int>(kOutside), 0x00020000);
 #pragma unroll
     for (int j = 0; j < INSTS; ++j) {
       const uint32_t v = kpos[j] < left ? voff[j] : kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (P2P_LDS void*)(dst + (wave * INSTS + j) * 1024), 16, v, 0, 0, 0);
+      lds_dma(base, v, dst + (wave * INSTS + j) * 1024);
     }
   }
 };
@@ -135,7 +167,7 @@ struct FragReader {
       base[1] = i * 128 + (((4 + q) ^ (i >> 1)) & 7) * 16;
     } else {
       kline = (8 * q + (i >> 2)) * EXT * 2;
-      f = ((i >> 2) | (q << 2)) & (EXT / 16 - 1);
+      f = line_swizzle<EXT>(8 * q + (i >> 2));
       part = (i & 3) * 8;
     }
   }
@@ -182,9 +214,10 @@ struct Place {
 // DUAL: B's tile interleaves 16 rows of b and 16 of b2; N counts both (the
 // tile's columns [32 j, 32 j + 16) are b's rows [16 j, 16 j + 16)).
 template <bool F16, bool AT, bool BT, bool DUAL, class Cfg, class Epi>
-__global__ __launch_bounds__(Cfg::THREADS, 2) void gemm_kernel(GemmArgs g, Epi epi) {
+__global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) void gemm_kernel(GemmArgs g, Epi epi) {
   __shared__ __attribute__((aligned(1024))) char lds[2 * Cfg::STAGE];
-  constexpr int A_INSTS = Cfg::BM / 8 / Cfg::WAVES, B_INSTS = Cfg::BN / 8 / Cfg::WAVES;
+  constexpr int A_INSTS = Cfg::HM / 8 / Cfg::WAVES, B_INSTS = Cfg::HN / 8 / Cfg::WAVES;  // per half and wave
+  static_assert(A_INSTS == B_INSTS, "the counts of the waits below");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_m = static_cast<int>(ceil_div(g.M, Cfg::BM)), tiles_n = static_cast<int>(ceil_div(g.N, Cfg::BN));
@@ -192,26 +225,29 @@ __global__ __launch_bounds__(Cfg::THREADS, 2) void gemm_kernel(GemmArgs g, Epi e
   tile_of_block(tiles_m, tiles_n, &tm, &tn);
   const int64_t m0 = static_cast<int64_t>(tm) * Cfg::BM, n0 = static_cast<int64_t>(tn) * Cfg::BN;
 
-  TileLoader<AT, Cfg::BM, A_INSTS> la;
-  TileLoader<BT, Cfg::BN, B_INSTS> lb;
-  la.init(wave, lane, g.lda, g.M - m0);
-  const int64_t a_org = AT ? m0 : m0 * g.lda;
-  int64_t b_org;
-  if constexpr (DUAL) {
-    static_assert(!BT, "two weights: k-contiguous");
-    // tile row r: unit n0 / 2 + 16 (r / 32) + r % 16 of b (r / 16 even) or b2 (odd)
-    const int64_t units = g.N / 2 - n0 / 2;
+  TileLoader<AT, Cfg::HM, A_INSTS> la[2];
+  TileLoader<BT, Cfg::HN, B_INSTS> lb[2];
+  int64_t a_org[2], b_org[2];
 #pragma unroll
-    for (int j = 0; j < B_INSTS; ++j) {
-      const int r = (wave * B_INSTS + j) * 8 + lane / 8, u = (r >> 5) * 16 + (r & 15);
-      const int c = (lane & 7) ^ ((r >> 1) & 7);
-      lb.kpos[j] = c * 8;
-      lb.voff[j] = u < units ? static_cast<uint32_t>(u * g.ldb * 2 + c * 16) : kOutside;
+  for (int h = 0; h < 2; ++h) {
+    const int64_t m = m0 + h * Cfg::HM, n = n0 + h * Cfg::HN;
+    la[h].init(wave, lane, g.lda, g.M - m);
+    a_org[h] = AT ? m : m * g.lda;
+    if constexpr (DUAL) {
+      static_assert(!BT, "two weights: k-contiguous");
+      const int64_t units = g.N / 2 - n / 2;
+#pragma unroll
+      for (int j = 0; j < B_INSTS; ++j) {
+        const int r = (wave * B_INSTS + j) * 8 + lane / 8, u = (r >> 5) * 16 + (r & 15);
+        const int c = (lane & 7) ^ ((r >> 1) & 7);
+        lb[h].kpos[j] = c * 8;
+        lb[h].voff[j] = u < units ? static_cast<uint32_t>(u * g.ldb * 2 + c * 16) : kOutside;
+      }
+      b_org[h] = n / 2 * g.ldb;
+    } else {
+      lb[h].init(wave, lane, g.ldb, g.N - n);
+      b_org[h] = BT ? n : n * g.ldb;
     }
-    b_org = n0 / 2 * g.ldb;
-  } else {
-    lb.init(wave, lane, g.ldb, g.N - n0);
-    b_org = BT ? n0 : n0 * g.ldb;
   }
 
   const int per_seg = static_cast<int>(ceil_div(g.K, kGemmK));
@@ -219,63 +255,128 @@ __global__ __launch_bounds__(Cfg::THREADS, 2) void gemm_kernel(GemmArgs g, Epi e
   const int part = blockIdx.y;
   const int first = static_cast<int>(static_cast<int64_t>(all) * part / g.ksplit);
   const int last = static_cast<int>(static_cast<int64_t>(all) * (part + 1) / g.ksplit);
-  int seg = first / per_seg, ks = first % per_seg;
+  int seg = first / per_seg, ks = first % per_seg, left_steps = last - first;
 
-  const auto issue = [&](int buf) {
-    const int64_t k0 = static_cast<int64_t>(ks) * kGemmK, left = g.K - k0;
-    char* dst = lds + buf * Cfg::STAGE;
-    la.issue(g.a[seg] + a_org + (AT ? k0 * g.lda : k0), left, dst, wave);
+  int64_t k0 = 0;
+  int left = 0;
+  const uint16_t *pa = nullptr, *pb = nullptr, *pb2 = nullptr;
+  const auto point = [&]() {
+    k0 = static_cast<int64_t>(ks) * kGemmK;
+    const bool in = left_steps > 0;
+    const int sg = in ? seg : 0;
+    left = in ? static_cast<int>(g.K - k0 < kGemmK ? g.K - k0 : kGemmK) : 0;
+    if (!in) k0 = 0;
+    pa = g.a[sg] + (AT ? k0 * g.lda : k0);
+    pb = g.b[sg] + (BT ? k0 * g.ldb : k0);
+    if constexpr (DUAL) pb2 = g.b2[sg] + k0;
+  };
+  const auto next = [&]() {
+    --left_steps;
+    if (++ks == per_seg) ks = 0, ++seg;
+    point();
+  };
+  const auto issue_a = [&](int h, char* stage) { la[h].issue(pa + a_org[h], left, stage + h * Cfg::A_HALF, wave); };
+  const auto issue_b = [&](int h, char* stage) {
+    char* dst = stage + 2 * Cfg::A_HALF + h * Cfg::B_HALF;
     if constexpr (DUAL) {
-      const int64_t org = b_org + k0;
 #pragma unroll
       for (int j = 0; j < B_INSTS; ++j) {
-        const int q = wave * B_INSTS + j;  // rows 8q .. 8q + 7: all of one weight
-        const uint16_t* w = (q >> 1) & 1 ? g.b2[seg] : g.b[seg];
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(w + org), 0,
-                                                                            static_cast<int>(kOutside), 0x00020000);
-        const uint32_t v = lb.kpos[j] < left ? lb.voff[j] : kOutside;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (P2P_LDS void*)(dst + Cfg::A_BYTES + q * 1024), 16, v, 0, 0, 0);
+        const int q = wave * B_INSTS + j;
+        const uint32_t v = lb[h].kpos[j] < left ? lb[h].voff[j] : kOutside;
+        lds_dma(((q >> 1) & 1 ? pb2 : pb) + b_org[h], v, dst + q * 1024);
       }
     } else {
-      lb.issue(g.b[seg] + b_org + (BT ? k0 * g.ldb : k0), left, dst + Cfg::A_BYTES, wave);
+      lb[h].issue(pb + b_org[h], left, dst, wave);
     }
-    if (++ks == per_seg) ks = 0, ++seg;
   };
 
-  FragReader<AT, Cfg::BM> ra;
-  FragReader<BT, Cfg::BN> rb;
+  FragReader<AT, Cfg::HM> ra;
+  FragReader<BT, Cfg::HN> rb;
   ra.init(lane);
   rb.init(lane);
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  constexpr int AI = Cfg::MI / 2, BJ = Cfg::NJ / 2;
   f4 acc[Cfg::MI][Cfg::NJ];
 #pragma unroll
   for (int i = 0; i < Cfg::MI; ++i)
 #pragma unroll
     for (int j = 0; j < Cfg::NJ; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+  s8 fa[2][AI][2], fb[2][BJ][2];
+  const auto read_a = [&](int h, const char* stage) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < AI; ++i) fa[h][i][half] = ra.read(stage + h * Cfg::A_HALF, wm * Cfg::QM + i * 16, half);
+  };
+  const auto read_b = [&](int h, const char* stage) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int j = 0; j < BJ; ++j) fb[h][j][half] = rb.read(stage + 2 * Cfg::A_HALF + h * Cfg::B_HALF, wn * Cfg::QN + j * 16, half);
+  };
+  const auto mma = [&](int ha, int hb) {
+    
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < AI; ++i)
+#pragma unroll
+        for (int j = 0; j < BJ; ++j)
+          acc[ha * AI + i][hb * BJ + j] = mfma16<F16>(fb[hb][j][half], fa[ha][i][half], acc[ha * AI + i][hb * BJ + j]);
+    
+  };
+  // this wave's reads are done, its oldest half has landed; then everyone's
+  const auto phase = [&] {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(6 * (Cfg::HM / 8 / Cfg::WAVES)) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
 
-  if (first < last) issue(0);
+  char* cur = lds;
+  char* nxt = lds + Cfg::STAGE;
+  point();
+  issue_a(0, cur);
+  issue_b(0, cur);
+  issue_b(1, cur);
+  issue_a(1, cur);
+  next();
+  issue_a(0, nxt);
+  issue_b(0, nxt);
+  issue_b(1, nxt);
+  issue_a(1, nxt);
+  phase();
+  read_a(0, cur);
+  read_b(0, cur);
+  next();
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  issue_a(0, cur);
   for (int s = first; s < last; ++s) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of step s
-    __builtin_amdgcn_s_barrier();                     // everyone's; and step s - 1's image is read
-    asm volatile("" ::: "memory");
-    if (s + 1 < last) issue((s + 1 - first) & 1);
-    const char* image = lds + ((s - first) & 1) * Cfg::STAGE;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      s8 fa[Cfg::MI], fb[Cfg::NJ];
-#pragma unroll
-      for (int j = 0; j < Cfg::NJ; ++j) fb[j] = rb.read(image + Cfg::A_BYTES, wn * Cfg::TN + j * 16, half);
-#pragma unroll
-      for (int i = 0; i < Cfg::MI; ++i) fa[i] = ra.read(image, wm * Cfg::TM + i * 16, half);
-#pragma unroll
-      for (int i = 0; i < Cfg::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < Cfg::NJ; ++j) acc[i][j] = mfma16<F16>(fb[j], fa[i], acc[i][j]);
-    }
+    phase();
+    issue_b(0, cur);
+    read_b(1, cur);
+    mma(0, 0);
+    phase();
+    issue_b(1, cur);
+    read_a(1, cur);
+    mma(0, 1);
+    phase();
+    issue_a(1, cur);
+    read_a(0, nxt);
+    mma(1, 0);
+    phase();
+    next();
+    issue_a(0, nxt);
+    read_b(0, nxt);
+    mma(1, 1);
+    char* const t = cur;
+    cur = nxt;
+    nxt = t;
   }
-  __syncthreads();  // the images are free: an epilogue may use them
+  // the last requests (zeros) land before the epilogue uses the images or the block ends
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
   Place p;
-  p.m0 = m0 + wm * Cfg::TM, p.n0 = n0 + wn * Cfg::TN;
+  p.m0 = m0 + wm * Cfg::QM, p.n0 = n0 + wn * Cfg::QN;
   p.lane = lane, p.wave = wave, p.tm = tm, p.tn = tn, p.wm = wm, p.wn = wn, p.part = part;
   epi.template finish<Cfg>(acc, p, g, lds);
 }
@@ -344,14 +445,14 @@ struct StoreEpi {
     if (scale[1]) a *= ldc(scale[1]);
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + i * 16 + i16;
+      const int64_t m = p.m0 + Cfg::row(i) + i16;
       if (m >= g.M) continue;
       const bool second = half > 0 && m >= half;
       const int64_t row = second ? m - half : m;
       if (!partial && half > 0 && row >= rows) continue;
 #pragma unroll
       for (int j = 0; j < Cfg::NJ; ++j) {
-        const int64_t n = p.n0 + j * 16 + q4;
+        const int64_t n = p.n0 + Cfg::col(j) + q4;
         if (n >= g.N) continue;
         if (partial) {
           float* to = partial + (p.part * g.M + m) * pitch;

@@ -43,14 +43,14 @@ struct StatsEpi {
     float2* rows = reinterpret_cast<float2*>(lds);  // [WN][BM]
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + i * 16 + i16;
+      const int64_t m = p.m0 + Cfg::row(i) + i16;
       const int64_t t = m < g.M ? ldg(target + m) - first - p.n0 : -1;
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < Cfg::NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int n = j * 16 + q4 + e;
+          const int n = Cfg::col(j) + q4 + e;
           if (p.n0 + n >= g.N) acc[i][j][e] = -INFINITY;
           else if (n == t) stg(at_target + m, acc[i][j][e]);
           top = fmaxf(top, acc[i][j][e]);  // passes over a NaN, which the sum below takes up
@@ -64,11 +64,11 @@ struct StatsEpi {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = acc[i][j][e] - base;
-          s += p.n0 + j * 16 + q4 + e < g.N ? (precise ? expf(x) : __expf(x)) : 0.f;
+          s += p.n0 + Cfg::col(j) + q4 + e < g.N ? (precise ? expf(x) : __expf(x)) : 0.f;
         }
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
-      if (p.lane < 16) rows[p.wn * Cfg::BM + p.wm * Cfg::TM + i * 16 + i16] = make_float2(top, s);
+      if (p.lane < 16) rows[p.wn * Cfg::BM + p.wm * Cfg::QM + Cfg::row(i) + i16] = make_float2(top, s);
     }
     __syncthreads();
     for (int r = threadIdx.x; r < Cfg::BM; r += Cfg::THREADS) {
@@ -166,7 +166,7 @@ struct GradEpi {
     const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + i * 16 + i16;
+      const int64_t m = p.m0 + Cfg::row(i) + i16;
       if (m >= g.M) continue;
       const int64_t y = ldg(target + m);
       const bool counts = y != ignore;
@@ -174,7 +174,7 @@ struct GradEpi {
       const int64_t t = y - first;
 #pragma unroll
       for (int j = 0; j < Cfg::NJ; ++j) {
-        const int64_t n = p.n0 + j * 16 + q4;
+        const int64_t n = p.n0 + Cfg::col(j) + q4;
         if (n >= pitch) continue;
         f4 v;
 #pragma unroll
