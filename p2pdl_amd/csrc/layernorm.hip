@@ -12,6 +12,9 @@
 // keeps dw and db of its columns in registers over all rows of a block and
 // writes one partial row per block; a second kernel adds the partials in
 // their order, so the gradients' bits do not depend on timing.
+#include <algorithm>
+#include <type_traits>
+
 #include "train_common.h"
 
 namespace p2p {
@@ -90,65 +93,99 @@ __global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layer
 }
 
 // Block q takes the rows (it * gridDim.x + q) * teams + team; parts[q] is its
-// row of 2 * cols sums: dw, then db.
-template <typename T, int TEAM, int NV>
-__global__ __launch_bounds__(kLnBwdBlock) void layernorm_bwd_kernel(const T* dy, int64_t lddy, const T* x, int64_t ldx,
-                                                                    const T* w, const float* mean_in,
-                                                                    const float* rstd_in, int64_t rows, int cols,
-                                                                    T* dx, float* parts) {
+// row of 2 * cols sums: dw, then db.  The next row's x and dy are requested
+// before this one is worked on (rows of up to 4096) and rows are held as they
+// lie, two registers per four 16-bit elements, so that two blocks fit a CU:
+// 16384 x 4096 bf16 in 143.6 us without either, 91 us (4.4 TB/s) with.
+template <typename T, int TEAM, int NV, bool DENSE>
+__global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void layernorm_bwd_kernel(
+    const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, const float* mean_in, const float* rstd_in, int64_t rows,
+    int cols, T* dx, float* parts) {
   constexpr int V = Vec16<T>::N;
-  constexpr int TEAMS = kLnBwdBlock / TEAM;
-  __shared__ float scratch[2][kLnBwdBlock / 64];
+  constexpr int TEAMS = kLnBwdBlock / TEAM, WAVES = TEAM / 64;
+  __shared__ float2 sums[2][kLnBwdBlock / 64];
   __shared__ float joined[TEAMS > 1 ? TEAM * V : 1];
-  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, wave = threadIdx.x / 64;
   float dwv[NV][V], dbv[NV][V];
+  Raw wv[NV], xv[NV], gv[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
 #pragma unroll
     for (int e = 0; e < V; ++e) dwv[i][e] = 0.f, dbv[i][e] = 0.f;
+    if (w) wv[i] = load_raw<T, DENSE>(w, (i * TEAM + lane) * V, cols);
+  }
   const float inv = 1.f / static_cast<float>(cols);
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * TEAMS; first < rows;
-       first += static_cast<int64_t>(gridDim.x) * TEAMS) {
-    const int64_t row = first + team;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * TEAMS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * TEAMS + team;
+  float mean = 0.f, rstd = 0.f;
+  const auto request = [&](int64_t r) {
+    const int have = r < rows ? cols : 0;
+    mean = have ? ldg(mean_in + r) : 0.f;
+    rstd = have ? ldg(rstd_in + r) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TEAM + lane) * V;
+      xv[i] = load_raw<T, DENSE>(x + r * ldx, c, have);
+      gv[i] = load_raw<T, DENSE>(dy + r * lddy, c, have);
+    }
+  };
+  constexpr bool AHEAD = NV * V <= 8;
+  if (AHEAD) request(row);
+  int parity = 0;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * TEAMS; first < rows; first += step, row += step, parity ^= 1) {
     const int have = row < rows ? cols : 0;
-    const float mean = have ? ldg(mean_in + row) : 0.f, rstd = have ? ldg(rstd_in + row) : 0.f;
-    float xh[NV][V], g[NV][V];
+    if (!AHEAD) request(row);
+    const float mu = mean, rs = rstd;
+    Raw xc[NV], gc[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) xc[i] = xv[i], gc[i] = gv[i];
+    if (AHEAD) request(row + step);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TEAM + lane) * V;
-      load_row<T, V>(x + row * ldx, c, have, xh[i]);
-      load_row<T, V>(dy + row * lddy, c, have, g[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TEAM + lane) * V;
-      float wv[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) wv[e] = 1.f;
-      if (w) load_row<T, V>(w, c, cols, wv);
+      forget(wv[i]);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float h = c + e < have ? (xh[i][e] - mean) * rstd : 0.f;
-        const float d = g[i][e];
+        const float h = (DENSE ? (i * TEAM + lane) * V : (i * TEAM + lane) * V + e) < have ? (raw_at<T>(xc[i], e) - mu) * rs : 0.f;
+        const float d = raw_at<T>(gc[i], e);
+        const float g = w ? d * raw_at<T>(wv[i], e) : d;
         dwv[i][e] += d * h;
         dbv[i][e] += d;
-        xh[i][e] = h;
-        g[i][e] = d * wv[e];
-        s1 += g[i][e];
-        s2 += g[i][e] * h;
+        s1 += g;
+        s2 += g * h;
+      }
+      forget(wv[i]);
+      forget(xc[i]);
+      forget(gc[i]);
+    }
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if constexpr (WAVES > 1) {
+      // one barrier per row: the sums of the row after next go to the same place, behind the next one's barrier
+      if ((threadIdx.x & 63) == 0) sums[parity][wave] = make_float2(s1, s2);
+      __syncthreads();
+      s1 = s2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        const float2 v = sums[parity][wave / WAVES * WAVES + i];
+        s1 += v.x;
+        s2 += v.y;
       }
     }
-    s1 = team_sum<TEAM, kLnBwdBlock>(s1, scratch[0]) * inv;
-    s2 = team_sum<TEAM, kLnBwdBlock>(s2, scratch[1]) * inv;
+    s1 *= inv;
+    s2 *= inv;
     if (have) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TEAM + lane) * V;
         float o[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = rstd * (g[i][e] - s1 - xh[i][e] * s2);
-        if (c < cols) store_row<T, V>(dx + row * cols, c, cols, o);
+        for (int e = 0; e < V; ++e) {
+          const float h = (raw_at<T>(xc[i], e) - mu) * rs;
+          const float d = raw_at<T>(gc[i], e);
+          o[e] = rs * ((w ? d * raw_at<T>(wv[i], e) : d) - s1 - h * s2);
+        }
+        if (c < cols) store_row<T, V, DENSE>(dx + row * cols, c, cols, o);
       }
     }
   }
@@ -200,32 +237,58 @@ __global__ __launch_bounds__(1024) void layernorm_parts_kernel(const float* part
   }
 }
 
-// Team and vectors per lane by the row's 16-byte vectors: one wave up to 128
-// of them, then 256 lanes, then 512 -- the registers of the backward pass
-// (4 floats per element) stay under 256 per lane.
+// Team and vectors per lane of the backward pass by the row's 16-byte
+// vectors: as few elements per lane as there are lanes for (8, so that the
+// next row's fit beside them in 128 registers), teams of up to 512.
 template <typename T, typename F>
 static void ln_team(int cols, F&& go) {
+  using std::integral_constant;
   const int vecs = static_cast<int>(ceil_div(cols, Vec16<T>::N));
-  if (vecs <= 64) go(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-  else if (vecs <= 128) go(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-  else if (vecs <= 256) go(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
-  else if (vecs <= 512) go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-  else if (vecs <= 1024) go(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
-  else if (vecs <= 2048) go(std::integral_constant<int, 512>(), std::integral_constant<int, 4>());
-  else if constexpr (sizeof(T) == 4) go(std::integral_constant<int, 512>(), std::integral_constant<int, 8>());
+  if constexpr (sizeof(T) == 4) {
+    if (vecs <= 128) go(integral_constant<int, 64>(), integral_constant<int, 2>());
+    else if (vecs <= 512) go(integral_constant<int, 256>(), integral_constant<int, 2>());
+    else if (vecs <= 1024) go(integral_constant<int, 512>(), integral_constant<int, 2>());
+    else if (vecs <= 2048) go(integral_constant<int, 512>(), integral_constant<int, 4>());
+    else go(integral_constant<int, 512>(), integral_constant<int, 8>());
+  } else {
+    if (vecs <= 64) go(integral_constant<int, 64>(), integral_constant<int, 1>());
+    else if (vecs <= 128) go(integral_constant<int, 128>(), integral_constant<int, 1>());
+    else if (vecs <= 256) go(integral_constant<int, 256>(), integral_constant<int, 1>());
+    else if (vecs <= 512) go(integral_constant<int, 512>(), integral_constant<int, 1>());
+    else if (vecs <= 1024) go(integral_constant<int, 512>(), integral_constant<int, 2>());
+    else go(integral_constant<int, 512>(), integral_constant<int, 4>());
+  }
 }
 
+// Forward: teams of 256 from 128 vectors up (16384 x 4096 bf16: 56 us, 64 us
+// with teams of 512, which wait for each other's sums).
+template <typename T, typename F>
+static void ln_fwd_team(int cols, F&& go) {
+  using std::integral_constant;
+  const int vecs = static_cast<int>(ceil_div(cols, Vec16<T>::N));
+  if (vecs <= 64) go(integral_constant<int, 64>(), integral_constant<int, 1>());
+  else if (vecs <= 128) go(integral_constant<int, 64>(), integral_constant<int, 2>());
+  else if (vecs <= 256) go(integral_constant<int, 256>(), integral_constant<int, 1>());
+  else if (vecs <= 512) go(integral_constant<int, 256>(), integral_constant<int, 2>());
+  else if (vecs <= 1024) go(integral_constant<int, 512>(), integral_constant<int, 2>());
+  else if (vecs <= 2048) go(integral_constant<int, 512>(), integral_constant<int, 4>());
+  else if constexpr (sizeof(T) == 4) go(integral_constant<int, 512>(), integral_constant<int, 8>());
+}
+
+template <typename T>
+static int ln_parts_of(int64_t rows, int cols) {
+  int teams = 1;
+  ln_team<T>(cols, [&](auto team, auto) { teams = kLnBwdBlock / decltype(team)::value; });
+  return static_cast<int>(std::min<int64_t>(ceil_div(rows, teams), kLnMaxParts));
+}
 static int ln_parts(int64_t rows, int cols, int32_t dtype) {
-  const int vecs = static_cast<int>(ceil_div(cols, 16 / dtype_bytes(dtype)));
-  const int teams = kLnBwdBlock / (vecs <= 128 ? 64 : vecs <= 512 ? 256 : 512);
-  const int64_t blocks = ceil_div(rows, teams);
-  return static_cast<int>(blocks < kLnMaxParts ? blocks : kLnMaxParts);
+  return dtype == P2P_DTYPE_F32 ? ln_parts_of<float>(rows, cols) : ln_parts_of<f16>(rows, cols);
 }
 
 template <typename T>
 static int32_t ln_fwd(const T* x, int64_t ldx, const T* w, const T* b, int64_t rows, int cols, float eps, T* y,
                       float* mean, float* rstd, hipStream_t st) {
-  ln_team<T>(cols, [&](auto team, auto nv) {
+  ln_fwd_team<T>(cols, [&](auto team, auto nv) {
     constexpr int TEAM = decltype(team)::value, BLOCK = kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock;
     layernorm_fwd_kernel<T, TEAM, decltype(nv)::value>
         <<<dim3(static_cast<unsigned>(ceil_div(rows, BLOCK / TEAM))), dim3(BLOCK), 0, st>>>(x, ldx, w, b, rows, cols, eps,
@@ -241,8 +304,9 @@ static int32_t ln_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const 
   const int n = ln_parts(rows, cols, dtype);
   float* const to = dw || db ? parts : nullptr;
   ln_team<T>(cols, [&](auto team, auto nv) {
-    layernorm_bwd_kernel<T, decltype(team)::value, decltype(nv)::value>
-        <<<dim3(n), dim3(kLnBwdBlock), 0, st>>>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, to);
+    constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
+    const auto kernel = cols % Vec16<T>::N == 0 ? layernorm_bwd_kernel<T, TEAM, NV, true> : layernorm_bwd_kernel<T, TEAM, NV, false>;
+    kernel<<<dim3(n), dim3(kLnBwdBlock), 0, st>>>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, to);
   });
   const int32_t rc = launch_status();
   if (rc != P2P_OK || !to) return rc;

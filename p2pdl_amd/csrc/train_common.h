@@ -56,6 +56,40 @@ struct Vec16 {
   static constexpr int N = 16 / sizeof(T);  // elements of a 16-byte vector
 };
 
+// A 16-byte vector x[c ..) as it lies, in four registers; elements at and past `cols` are 0.
+struct Raw {
+  uint32_t w[4];
+};
+// DENSE: cols is a multiple of the vector.
+template <typename T, bool DENSE>
+__device__ __forceinline__ Raw load_raw(const T* row, int64_t c, int64_t cols) {
+  constexpr int N = 16 / sizeof(T);
+  if (c + N <= cols) return __builtin_bit_cast(Raw, *(const P2P_GLOBAL raw4*)(row + c));
+  if (DENSE) return Raw{{0u, 0u, 0u, 0u}};
+  Raw r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      r.w[i] = c + i < cols ? ldg(reinterpret_cast<const uint32_t*>(row) + c + i) : 0u;
+    } else {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + c + 2 * i;
+      const uint32_t lo = c + 2 * i < cols ? ldg(p) : 0u, hi = c + 2 * i + 1 < cols ? ldg(p + 1) : 0u;
+      r.w[i] = lo | (hi << 16);
+    }
+  }
+  return r;
+}
+// Keeps the compiler from holding values that it derived from r across this point (as floats
+// they take twice the registers and are two instructions to make again).
+__device__ __forceinline__ void forget(Raw& r) {
+  asm volatile("" : "+v"(r.w[0]), "+v"(r.w[1]), "+v"(r.w[2]), "+v"(r.w[3]));
+}
+// Its element e as a float.
+template <typename T>
+__device__ __forceinline__ float raw_at(const Raw& r, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[e]);
+  else return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(r.w[e / 2] >> (e & 1) * 16)));
+}
 // x[c .. c + N) as floats; elements at and past `cols` read as 0.
 template <typename T, int N>
 __device__ __forceinline__ void load_row(const T* row, int64_t c, int64_t cols, float (&out)[N]) {
@@ -68,9 +102,9 @@ __device__ __forceinline__ void load_row(const T* row, int64_t c, int64_t cols, 
     for (int e = 0; e < N; ++e) out[e] = c + e < cols ? static_cast<float>(ldg(row + c + e)) : 0.f;
   }
 }
-template <typename T, int N>
+template <typename T, int N, bool DENSE = false>
 __device__ __forceinline__ void store_row(T* row, int64_t c, int64_t cols, const float (&x)[N]) {
-  if (c + N <= cols) {
+  if (DENSE || c + N <= cols) {
     Pack<T, N> p;
 #pragma unroll
     for (int e = 0; e < N; ++e) p.v[e] = static_cast<T>(x[e]);
