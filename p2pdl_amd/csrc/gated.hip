@@ -185,13 +185,15 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
   return c.used;
 }
 
-static int32_t gated_operand(const void* p, int64_t ld, int64_t rows, int64_t cols, int32_t dtype, uint16_t* space, Mat* m,
-                             hipStream_t st) {
-  if (space) return pack_matrix(p, ld, rows, cols, dtype, space, m, st);
-  m->plane[0] = static_cast<const uint16_t*>(p);
-  m->plane[1] = m->plane[2] = nullptr;
-  m->ld = ld;
-  return P2P_OK;
+// x, w_gate and w_up as the products read them, copied (in one launch) where the workspace has a place for it.
+static int32_t gated_operands(const p2p_gated_linear_t& a, const GatedSpace& s, Mat* x, Mat* wg, Mat* wu, hipStream_t st) {
+  const PackJob jobs[3] = {{a.x, a.ldx, a.tokens, a.hidden, s.x},
+                           {a.w_gate, a.ldg, a.units, a.hidden, s.wg},
+                           {a.w_up, a.ldu, a.units, a.hidden, s.wu}};
+  *x = mat_of(jobs[0], a.dtype);
+  *wg = mat_of(jobs[1], a.dtype);
+  *wu = mat_of(jobs[2], a.dtype);
+  return pack_matrices(jobs, 3, a.dtype, st);
 }
 
 }  // namespace p2p
@@ -217,9 +219,7 @@ extern "C" int32_t p2p_gated_linear_fwd(const p2p_gated_linear_t* a, void* works
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   Mat x, wg, wu;
-  if ((rc = gated_operand(a->x, a->ldx, a->tokens, a->hidden, a->dtype, s.x, &x, st)) != P2P_OK) return rc;
-  if ((rc = gated_operand(a->w_gate, a->ldg, a->units, a->hidden, a->dtype, s.wg, &wg, st)) != P2P_OK) return rc;
-  if ((rc = gated_operand(a->w_up, a->ldu, a->units, a->hidden, a->dtype, s.wu, &wu, st)) != P2P_OK) return rc;
+  if ((rc = gated_operands(*a, s, &x, &wg, &wu, st)) != P2P_OK) return rc;
   GemmArgs g{};
   add_pairs(&g, x, wg, &wu, a->dtype);
   g.lda = x.ld, g.ldb = wg.ld;
@@ -246,9 +246,7 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool f16_ = a->dtype == P2P_DTYPE_F16;
   Mat x, wg, wu;
-  if ((rc = gated_operand(a->x, a->ldx, a->tokens, a->hidden, a->dtype, s.x, &x, st)) != P2P_OK) return rc;
-  if ((rc = gated_operand(a->w_gate, a->ldg, a->units, a->hidden, a->dtype, s.wg, &wg, st)) != P2P_OK) return rc;
-  if ((rc = gated_operand(a->w_up, a->ldu, a->units, a->hidden, a->dtype, s.wu, &wu, st)) != P2P_OK) return rc;
+  if ((rc = gated_operands(*a, s, &x, &wg, &wu, st)) != P2P_OK) return rc;
   const int64_t pitch = gated_pitch(*a), plane = a->tokens * 2 * pitch;
   rc = a->dtype == P2P_DTYPE_F32 ? gated_grad<float>(*a, pitch, s.d, st)
        : f16_                    ? gated_grad<f16>(*a, pitch, s.d, st)

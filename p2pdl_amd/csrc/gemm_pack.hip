@@ -4,11 +4,17 @@
 
 namespace p2p {
 
-// One lane per 8 elements of a packed row.
+// One lane per 8 elements of a packed row; grid.y: the matrix.
+struct PackJobs {
+  PackJob job[kMaxPack];
+};
 template <typename T>
-__global__ __launch_bounds__(kBlock) void pack_kernel(const T* src, int64_t ld, int64_t rows, int64_t cols, int64_t pitch,
-                                                      uint16_t* dst, int64_t plane) {
-  const int64_t per_row = pitch / 8, all = rows * per_row;
+__global__ __launch_bounds__(kBlock) void pack_kernel(PackJobs jobs) {
+  const PackJob& job = jobs.job[blockIdx.y];
+  const T* src = static_cast<const T*>(job.src);
+  uint16_t* dst = job.dst;
+  const int64_t ld = job.ld, cols = job.cols, pitch = (cols + 7) / 8 * 8, plane = job.rows * pitch;
+  const int64_t per_row = pitch / 8, all = job.rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
        i += static_cast<int64_t>(gridDim.x) * kBlock) {
     const int64_t r = i / per_row, c = (i - r * per_row) * 8;
@@ -43,17 +49,19 @@ static unsigned blocks_for(int64_t items) {
   return static_cast<unsigned>(b < 1 ? 1 : b > 256 * 32 ? 256 * 32 : b);
 }
 
-int32_t pack_matrix(const void* src, int64_t ld, int64_t rows, int64_t cols, int32_t dtype, uint16_t* dst, Mat* out,
-                    hipStream_t st) {
-  const int64_t pitch = round_up(cols, 8), plane = rows * pitch;
-  for (int q = 0; q < 3; ++q) out->plane[q] = q < planes_of(dtype) ? dst + q * plane : nullptr;
-  out->ld = pitch;
-  if (rows == 0) return P2P_OK;
-  const unsigned blocks = blocks_for(rows * (pitch / 8));
-  if (dtype == P2P_DTYPE_F32)
-    pack_kernel<float><<<dim3(blocks), dim3(kBlock), 0, st>>>(static_cast<const float*>(src), ld, rows, cols, pitch, dst, plane);
-  else
-    pack_kernel<uint16_t><<<dim3(blocks), dim3(kBlock), 0, st>>>(static_cast<const uint16_t*>(src), ld, rows, cols, pitch, dst, plane);
+int32_t pack_matrices(const PackJob* jobs, int n, int32_t dtype, hipStream_t st) {
+  PackJobs all{};
+  int64_t most = 0;
+  int used = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!jobs[i].dst || jobs[i].rows == 0) continue;
+    all.job[used++] = jobs[i];
+    most = std::max(most, jobs[i].rows * (round_up(jobs[i].cols, 8) / 8));
+  }
+  if (!used) return P2P_OK;
+  const dim3 grid(blocks_for(most), used);
+  if (dtype == P2P_DTYPE_F32) pack_kernel<float><<<grid, dim3(kBlock), 0, st>>>(all);
+  else pack_kernel<uint16_t><<<grid, dim3(kBlock), 0, st>>>(all);
   return launch_status();
 }
 

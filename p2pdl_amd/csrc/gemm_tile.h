@@ -526,9 +526,23 @@ static inline int64_t packed_bytes(int64_t rows, int64_t cols, int32_t dtype) {
   return round_up(rows * round_up(cols, 8) * 2 * planes_of(dtype), 256);
 }
 
-// src [rows, cols], pitch ld, as 16-bit planes of pitch round_up(cols, 8), zeros in the added columns.
-P2P_INTERNAL int32_t pack_matrix(const void* src, int64_t ld, int64_t rows, int64_t cols, int32_t dtype, uint16_t* dst, Mat* out,
-                                 hipStream_t st);
+// src [rows, cols], pitch ld, as 16-bit planes of pitch round_up(cols, 8) at dst, zeros in the
+// added columns.  Up to kMaxPack of them in one launch; those without a dst are left out.
+constexpr int kMaxPack = 3;
+struct PackJob {
+  const void* src;
+  int64_t ld, rows, cols;
+  uint16_t* dst;
+};
+P2P_INTERNAL int32_t pack_matrices(const PackJob* jobs, int n, int32_t dtype, hipStream_t st);
+
+// What the product reads of a job: its copy, or src in place where it has none.
+static inline Mat mat_of(const PackJob& j, int32_t dtype) {
+  if (!j.dst) return Mat{{static_cast<const uint16_t*>(j.src), nullptr, nullptr}, j.ld};
+  const int64_t pitch = round_up(j.cols, 8), plane = j.rows * pitch;
+  const bool three = planes_of(dtype) == 3;
+  return Mat{{j.dst, three ? j.dst + plane : nullptr, three ? j.dst + 2 * plane : nullptr}, pitch};
+}
 // out[i] = alpha * (parts[i] + parts[stride + i] + ...) in that order
 P2P_INTERNAL int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, const float* scale0,
                                 const float* scale1, float alpha, void* out, int32_t dtype, hipStream_t st);

@@ -219,7 +219,6 @@ static int32_t ce_check(const p2p_linear_ce_t* a) {
 }
 
 struct CeSpace {
-  bool x_here, w_here;
   int64_t piece;      // vocabulary rows per piece
   uint16_t *x, *w;    // packed x; packed rows of one piece of W
   // forward
@@ -240,17 +239,16 @@ static Plan ce_dw_plan(const p2p_linear_ce_t& a, int64_t rows) {
 static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeSpace* s) {
   Carver c{static_cast<char*>(base)};
   const int planes = planes_of(a.dtype);
-  s->x_here = in_place(a.x, a.ldx, a.hidden, a.dtype);
-  s->w_here = in_place(a.w, a.ldw, a.hidden, a.dtype);
+  const bool x_here = in_place(a.x, a.ldx, a.hidden, a.dtype), w_here = in_place(a.w, a.ldw, a.hidden, a.dtype);
   // pieces: the buffers that grow with one stay under kPieceBytes (one tile's columns at least)
   int64_t per_row = backward ? a.tokens * 2 * planes : ceil_div(a.tokens * 8, Small::BN);
-  if (!s->w_here) per_row = std::max(per_row, round_up(a.hidden, 8) * 2 * planes);
+  if (!w_here) per_row = std::max(per_row, round_up(a.hidden, 8) * 2 * planes);
   int64_t piece = std::max<int64_t>(1, kPieceBytes / per_row / Big::BN) * Big::BN;
   if (piece >= a.vocab) piece = a.vocab;
   else piece = round_up(ceil_div(a.vocab, ceil_div(a.vocab, piece)), Big::BN);  // pieces of about one size
   s->piece = piece;
-  s->x = s->x_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(a.tokens, a.hidden, a.dtype)));
-  s->w = s->w_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(piece, a.hidden, a.dtype)));
+  s->x = x_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(a.tokens, a.hidden, a.dtype)));
+  s->w = w_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(piece, a.hidden, a.dtype)));
   if (!backward) {
     s->part = static_cast<float2*>(c.take(ceil_div(piece, Small::BN) * a.tokens * 8));
     s->state = static_cast<float2*>(c.take(a.tokens * 8));
@@ -272,16 +270,14 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
   return c.used;
 }
 
-static int32_t ce_x(const p2p_linear_ce_t& a, const CeSpace& s, Mat* x, hipStream_t st) {
-  if (!s.x_here) return pack_matrix(a.x, a.ldx, a.tokens, a.hidden, a.dtype, s.x, x, st);
-  *x = Mat{{static_cast<const uint16_t*>(a.x), nullptr, nullptr}, a.ldx};
-  return P2P_OK;
-}
-static int32_t ce_w(const p2p_linear_ce_t& a, const CeSpace& s, int64_t v0, int64_t rows, Mat* w, hipStream_t st) {
+// x (with the first piece) and the rows [v0, v0 + rows) of W as the products read them.
+static int32_t ce_operands(const p2p_linear_ce_t& a, const CeSpace& s, int64_t v0, int64_t rows, Mat* x, Mat* w,
+                           hipStream_t st) {
   const char* p = static_cast<const char*>(a.w) + v0 * a.ldw * dtype_bytes(a.dtype);
-  if (!s.w_here) return pack_matrix(p, a.ldw, rows, a.hidden, a.dtype, s.w, w, st);
-  *w = Mat{{reinterpret_cast<const uint16_t*>(p), nullptr, nullptr}, a.ldw};
-  return P2P_OK;
+  const PackJob jobs[2] = {{p, a.ldw, rows, a.hidden, s.w}, {a.x, a.ldx, a.tokens, a.hidden, s.x}};
+  *w = mat_of(jobs[0], a.dtype);
+  *x = mat_of(jobs[1], a.dtype);
+  return pack_matrices(jobs, v0 ? 1 : 2, a.dtype, st);
 }
 
 }  // namespace p2p
@@ -310,10 +306,9 @@ extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, 
   if (ce_carve(*a, false, workspace, &s) > workspace_bytes || !workspace) return P2P_ERR_INVALID;
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   Mat x, w;
-  if ((rc = ce_x(*a, s, &x, st)) != P2P_OK) return rc;
   for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
     const int64_t rows = std::min(s.piece, a->vocab - v0);
-    if ((rc = ce_w(*a, s, v0, rows, &w, st)) != P2P_OK) return rc;
+    if ((rc = ce_operands(*a, s, v0, rows, &x, &w, st)) != P2P_OK) return rc;
     GemmArgs g{};
     add_pairs(&g, x, w, nullptr, a->dtype);
     g.lda = x.ld, g.ldb = w.ld;
@@ -346,10 +341,9 @@ extern "C" int32_t p2p_linear_ce_bwd(const p2p_linear_ce_t* a, void* workspace, 
   const bool f16_ = a->dtype == P2P_DTYPE_F16;
   const float alpha = f16_ ? 1.f / kHalfScale : 1.f;
   Mat x, w;
-  if ((rc = ce_x(*a, s, &x, st)) != P2P_OK) return rc;
   for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
     const int64_t rows = std::min(s.piece, a->vocab - v0), pitch = round_up(rows, 8), plane = a->tokens * pitch;
-    if ((rc = ce_w(*a, s, v0, rows, &w, st)) != P2P_OK) return rc;
+    if ((rc = ce_operands(*a, s, v0, rows, &x, &w, st)) != P2P_OK) return rc;
     {
       GemmArgs g{};
       add_pairs(&g, x, w, nullptr, a->dtype);

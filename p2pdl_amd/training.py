@@ -33,7 +33,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from .ops import _NO_CTX
 
 DTYPES = {torch.float32: N.P2P_DTYPE_F32, torch.float16: N.P2P_DTYPE_F16, torch.bfloat16: N.P2P_DTYPE_BF16}
 ACTIVATIONS = {"silu": N.P2P_ACT_SILU, "gelu": N.P2P_ACT_GELU, "relu": N.P2P_ACT_RELU}
@@ -41,38 +40,52 @@ MAX_NORM_COLS = 16384
 MAX_FEATURES = (1 << 22) - 8
 
 
-def _on(dev: torch.device):
-    """The device as the current one (no context where it is already)."""
-    return _NO_CTX if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _call(fn, what: str, dev: torch.device, *args) -> None:
+    """fn(*args, the current stream of dev) with dev as the current device."""
+    if dev.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, N.stream_handle(dev))
+    if rc:
+        N.check(rc, what)
 
 
 def _dtype(x: torch.Tensor, name: str) -> int:
-    N.require_device(x)
     dt = DTYPES.get(x.dtype)
-    if dt is None:
-        raise TypeError(f"{name}: expected float32, float16 or bfloat16, got {x.dtype}")
+    if dt is None or not x.is_cuda or not x.numel():
+        N.require_device(x)
+        if dt is None:
+            raise TypeError(f"{name}: expected float32, float16 or bfloat16, got {x.dtype}")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"{name}: needs a last dimension of at least one feature, got shape {tuple(x.shape)}")
     return dt
 
 
-def _like(t: torch.Tensor, x: torch.Tensor, name: str, shape=None) -> None:
+def _like(t: torch.Tensor, x: torch.Tensor, name: str, shape) -> None:
+    if t.shape == shape and t.dtype is x.dtype and t.device == x.device:
+        return
     if t.dtype != x.dtype:
         raise TypeError(f"{name}: expected {x.dtype}, got {t.dtype}")
     if t.device != x.device:
         raise RuntimeError(f"{name}: expected all tensors on {x.device}, got {t.device}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _new(x: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _stat(t: torch.Tensor, x: torch.Tensor, name: str, shape) -> None:
     """A dense float32 tensor that a forward pass left for its backward pass."""
+    if t.shape == shape and t.dtype is torch.float32 and t.device == x.device and t.is_contiguous():
+        return
     if t.dtype != torch.float32:
         raise TypeError(f"{name}: expected float32, got {t.dtype}")
     if t.device != x.device:
         raise RuntimeError(f"{name}: expected all tensors on {x.device}, got {t.device}")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _rows(t: torch.Tensor):
@@ -129,17 +142,14 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias
     dt = _norm_inputs(x, weight, bias)
     dev, cols = x.device, x.shape[-1]
     rows = x.numel() // cols
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=dev)
-    mean, rstd = stats[0], stats[1]
+    y = _new(x)
+    mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=dev).unbind(0)
     if rows:
         xr, ld = _rows(x)
         w = None if weight is None else weight.contiguous()
         b = None if bias is None else bias.contiguous()
-        with _on(dev):
-            N.check(N.lib().p2p_layernorm_fwd(xr.data_ptr(), ld, _ptr(w), _ptr(b), rows, cols, eps, y.data_ptr(),
-                                              mean.data_ptr(), rstd.data_ptr(), dt, N.stream_handle(dev)),
-                    "p2p_layernorm_fwd")
+        _call(N.lib().p2p_layernorm_fwd, "p2p_layernorm_fwd", dev, xr.data_ptr(), ld, _ptr(w), _ptr(b), rows, cols, eps,
+              y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dt)
     return y, mean, rstd
 
 
@@ -152,7 +162,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     _stat(rstd, x, "rstd", x.shape[:-1])
     dev, cols = x.device, x.shape[-1]
     rows = x.numel() // cols
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dx = _new(x)
     dw = db = None
     if weight is not None:
         dw, db = (torch.empty if rows else torch.zeros)((2, cols), dtype=x.dtype, device=dev).unbind(0)
@@ -166,10 +176,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
             w = weight.contiguous()
             nbytes = L.p2p_layernorm_bwd_workspace(rows, cols, dt)
             ws = _workspace(nbytes, dev, "p2p_layernorm_bwd_workspace")
-        with _on(dev):
-            N.check(L.p2p_layernorm_bwd(dyr.data_ptr(), lddy, xr.data_ptr(), ldx, _ptr(w), mean.data_ptr(),
-                                        rstd.data_ptr(), rows, cols, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nbytes,
-                                        dt, N.stream_handle(dev)), "p2p_layernorm_bwd")
+        _call(L.p2p_layernorm_bwd, "p2p_layernorm_bwd", dev, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, _ptr(w),
+              mean.data_ptr(), rstd.data_ptr(), rows, cols, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nbytes, dt)
     return dx, dw, db
 
 
@@ -215,13 +223,12 @@ def _dropout(x, p, seed, offset, residual):
     if residual is not None:
         _like(residual, x, "residual", x.shape)
         residual = residual.contiguous()
-    dev, n = x.device, x.numel()
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    n = x.numel()
+    y = _new(x)
     if n:
         xc = x.contiguous()
-        with _on(dev):
-            N.check(N.lib().p2p_dropout(xc.data_ptr(), _ptr(residual), n, p, seed, offset, _ptr(offset_dev), y.data_ptr(),
-                                        dt, N.stream_handle(dev)), "p2p_dropout")
+        _call(N.lib().p2p_dropout, "p2p_dropout", x.device, xc.data_ptr(), _ptr(residual), n, p, seed, offset,
+              _ptr(offset_dev), y.data_ptr(), dt)
     return y
 
 
@@ -316,8 +323,7 @@ def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
         a.h, a.gate, a.up = h.data_ptr(), _ptr(gate), _ptr(up)
         nbytes = L.p2p_gated_linear_workspace(a, 0)
         ws = _workspace(nbytes, dev, "p2p_gated_linear_workspace")
-        with _on(dev):
-            N.check(L.p2p_gated_linear_fwd(a, _ptr(ws), nbytes, N.stream_handle(dev)), "p2p_gated_linear_fwd")
+        _call(L.p2p_gated_linear_fwd, "p2p_gated_linear_fwd", dev, a, _ptr(ws), nbytes)
         del keep
     return h, gate, up
 
@@ -330,9 +336,7 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
     _like(dh, x, "dh", shape)
     _stat(gate, x, "gate", shape)
     _stat(up, x, "up", shape)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    make = torch.empty if x.numel() else torch.zeros
-    dwg, dwu = make(w_gate.shape, dtype=x.dtype, device=dev), make(w_gate.shape, dtype=x.dtype, device=dev)
+    dx, dwg, dwu = _new(x), _new(w_gate), _new(w_up)
     if x.numel():
         L = N.lib()
         a, keep = _gated_args(x, w_gate, w_up, dt, act)
@@ -341,9 +345,11 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tenso
         a.dx, a.dw_gate, a.dw_up = dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr()
         nbytes = L.p2p_gated_linear_workspace(a, 1)
         ws = _workspace(nbytes, dev, "p2p_gated_linear_workspace")
-        with _on(dev):
-            N.check(L.p2p_gated_linear_bwd(a, _ptr(ws), nbytes, N.stream_handle(dev)), "p2p_gated_linear_bwd")
+        _call(L.p2p_gated_linear_bwd, "p2p_gated_linear_bwd", dev, a, _ptr(ws), nbytes)
         del keep
+    else:
+        dwg.zero_()
+        dwu.zero_()
     return dx, dwg, dwu
 
 
@@ -414,8 +420,7 @@ def linear_cross_entropy_forward(x: torch.Tensor, weight: torch.Tensor, target: 
     L = N.lib()
     nbytes = L.p2p_linear_ce_workspace(a, 0)
     ws = _workspace(nbytes, dev, "p2p_linear_ce_workspace")
-    with _on(dev):
-        N.check(L.p2p_linear_ce_fwd(a, _ptr(ws), nbytes, N.stream_handle(dev)), "p2p_linear_ce_fwd")
+    _call(L.p2p_linear_ce_fwd, "p2p_linear_ce_fwd", dev, a, _ptr(ws), nbytes)
     del keep
     return loss, lse, norm
 
@@ -431,16 +436,16 @@ def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target:
     if dloss is not None and (dloss.dtype != torch.float32 or dloss.numel() != 1 or dloss.device != dev):
         raise ValueError(f"dloss: expected one float32 on {dev}, got {dloss.dtype} of {dloss.numel()} elements on "
                          f"{dloss.device}")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dw = (torch.empty if x.numel() else torch.zeros)(weight.shape, dtype=x.dtype, device=dev)
+    dx, dw = _new(x), _new(weight)
     if x.numel():
         a.lse, a.norm, a.dloss = lse.data_ptr(), norm.data_ptr(), _ptr(dloss)
         a.dx, a.dw = dx.data_ptr(), dw.data_ptr()
         L = N.lib()
         nbytes = L.p2p_linear_ce_workspace(a, 1)
         ws = _workspace(nbytes, dev, "p2p_linear_ce_workspace")
-        with _on(dev):
-            N.check(L.p2p_linear_ce_bwd(a, _ptr(ws), nbytes, N.stream_handle(dev)), "p2p_linear_ce_bwd")
+        _call(L.p2p_linear_ce_bwd, "p2p_linear_ce_bwd", dev, a, _ptr(ws), nbytes)
+    else:
+        dw.zero_()
     del keep
     return dx, dw
 
