@@ -17,6 +17,10 @@
 // once, as the operands of the matrix instructions (float32: not rounded,
 // three planes), lie side by side in one [T, 2F] buffer, and feed dx as two
 // segments of one sum and dWg, dWu as one product of 2F rows.
+//
+// Small float32 layers take the product of direct.h instead, forward into
+// sums of k-runs that a second kernel joins and activates: @@
+#include "direct.h"
 #include "gemm_tile.h"
 
 namespace p2p {
@@ -77,11 +81,12 @@ struct GatedEpi {
 
 // dg and du of 8 units per lane, into d [T, 2 * pitch]: dg, then du, zeros
 // in the columns past `units`; plane: elements from one plane to the next.
-template <typename T, int ACT>
+// DIRECT: as float, with no columns past `units` (pitch == units).
+template <typename T, int ACT, bool DIRECT>
 __global__ __launch_bounds__(kBlock) void gated_grad_kernel(const T* dh, int64_t lddh, const float* gate, const float* up,
                                                             int64_t rows, int64_t units, int64_t pitch, uint16_t* d,
                                                             int64_t plane) {
-  const int64_t per_row = pitch / 8, all = rows * per_row;
+  const int64_t per_row = (pitch + 7) / 8, all = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
        i += static_cast<int64_t>(gridDim.x) * kBlock) {
     const int64_t r = i / per_row, c = (i - r * per_row) * 8;
@@ -98,7 +103,11 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(const T* dh, int64_t
       u[e] = c + e < units ? du : 0.f;
     }
     uint16_t* to = d + r * 2 * pitch + c;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (DIRECT) {
+      float* row = reinterpret_cast<float*>(d) + r * 2 * pitch;
+      store_row<float, 8>(row, c, units, g);
+      store_row<float, 8>(row + pitch, c, units, u);
+    } else if constexpr (sizeof(T) == 4) {
       Pack<uint16_t, 8> og[3], ou[3];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -118,19 +127,45 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(const T* dh, int64_t
   }
 }
 
-template <typename T>
+template <typename T, bool DIRECT>
 static int32_t gated_grad(const p2p_gated_linear_t& a, int64_t pitch, uint16_t* d, hipStream_t st) {
-  const int64_t items = a.tokens * (pitch / 8), blocks = ceil_div(items, kBlock);
+  const int64_t items = a.tokens * ceil_div(pitch, 8), blocks = ceil_div(items, kBlock);
   const dim3 grid(static_cast<unsigned>(blocks < 256 * 32 ? blocks : 256 * 32)), block(kBlock);
-  const int64_t plane = a.tokens * 2 * pitch;
-  const T* dh = static_cast<const T*>(a.dh);
-  if (a.activation == P2P_ACT_SILU)
-    gated_grad_kernel<T, P2P_ACT_SILU><<<grid, block, 0, st>>>(dh, a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d, plane);
-  else if (a.activation == P2P_ACT_GELU)
-    gated_grad_kernel<T, P2P_ACT_GELU><<<grid, block, 0, st>>>(dh, a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d, plane);
-  else
-    gated_grad_kernel<T, P2P_ACT_RELU><<<grid, block, 0, st>>>(dh, a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d, plane);
+  const auto kernel = a.activation == P2P_ACT_SILU   ? gated_grad_kernel<T, P2P_ACT_SILU, DIRECT>
+                      : a.activation == P2P_ACT_GELU ? gated_grad_kernel<T, P2P_ACT_GELU, DIRECT>
+                                                     : gated_grad_kernel<T, P2P_ACT_RELU, DIRECT>;
+  kernel<<<grid, block, 0, st>>>(static_cast<const T*>(a.dh), a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d,
+                                 a.tokens * 2 * pitch);
   return launch_status();
+}
+
+// The direct product's runs [runs][T, 2 units] joined; gate, up and h.
+__global__ __launch_bounds__(kBlock) void gated_join_kernel(const float* parts, int runs, int64_t rows, int64_t units, int act,
+                                                            float* h, float* gate, float* up) {
+  const int64_t per_row = (units + 3) / 4, all = rows * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
+       i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 4;
+    float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
+#pragma unroll 4
+    for (int p = 0; p < runs; ++p) {
+      const float* row = parts + (p * rows + r) * 2 * units;
+      float x[4], y[4];
+      load_row<float, 4>(row, c, units, x);
+      load_row<float, 4>(row + units, c, units, y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[e] += x[e], u[e] += y[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float a, da;
+      activation(act, g[e], &a, &da);
+      o[e] = a * u[e];
+    }
+    store_row<float, 4>(h + r * units, c, units, o);
+    if (gate) store_row<float, 4>(gate + r * units, c, units, g);
+    if (up) store_row<float, 4>(up + r * units, c, units, u);
+  }
 }
 
 static int32_t gated_check(const p2p_gated_linear_t* a) {
@@ -157,8 +192,26 @@ static Plan gated_dx_plan(const p2p_gated_linear_t& a) {
 static Plan gated_dw_plan(const p2p_gated_linear_t& a) {
   return gemm_plan(2 * gated_pitch(a), a.hidden, ksteps(a.tokens, a.dtype == P2P_DTYPE_F32 ? 6 : 1), true);
 }
+static bool gated_direct(const p2p_gated_linear_t& a) {
+  return a.dtype == P2P_DTYPE_F32 && direct_pays(a.tokens, 2 * a.units, a.hidden);
+}
 static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* base, GatedSpace* s) {
   Carver c{static_cast<char*>(base)};
+  if (gated_direct(a)) {
+    const int64_t rows2 = 2 * a.units;
+    *s = GatedSpace{};
+    int64_t floats = 0;
+    if (backward) {
+      s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 4));
+      const int sx = direct_split(a.tokens, a.hidden, rows2), sw = direct_split(rows2, a.hidden, a.tokens);
+      if (sx > 1) floats = sx * a.tokens * a.hidden;
+      if (sw > 1) floats = std::max(floats, sw * rows2 * a.hidden);
+    } else {
+      floats = direct_split(a.tokens, 2 * a.units, a.hidden) * a.tokens * 2 * a.units;
+    }
+    if (floats) s->parts = static_cast<float*>(c.take(floats * 4));
+    return c.used;
+  }
   const auto operand = [&](const void* p, int64_t ld, int64_t rows) -> uint16_t* {
     return in_place(p, ld, a.hidden, a.dtype) ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(rows, a.hidden, a.dtype)));
   };
@@ -196,6 +249,45 @@ static int32_t gated_operands(const p2p_gated_linear_t& a, const GatedSpace& s, 
   return pack_matrices(jobs, 3, a.dtype, st);
 }
 
+static int32_t gated_direct_fwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
+  const int split = direct_split(a.tokens, 2 * a.units, a.hidden);
+  const DirectArgs g{static_cast<const float*>(a.x), static_cast<const float*>(a.w_gate), static_cast<const float*>(a.w_up),
+                     a.ldx, a.ldg, a.ldu, a.units, a.tokens, 2 * a.units, a.hidden, split, {nullptr, nullptr}, INT64_MAX,
+                     {nullptr, nullptr}, s.parts};
+  const int32_t rc = direct_product(false, false, g, st);
+  if (rc != P2P_OK) return rc;
+  const int64_t blocks = ceil_div(a.tokens * ceil_div(a.units, 4), kBlock);
+  gated_join_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
+      s.parts, split, a.tokens, a.units, a.activation, static_cast<float*>(a.h), a.gate, a.up);
+  return launch_status();
+}
+
+static int32_t gated_direct_bwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
+  const int64_t rows2 = 2 * a.units;
+  int32_t rc = gated_grad<float, true>(a, a.units, s.d, st);
+  if (rc != P2P_OK) return rc;
+  const float *d = reinterpret_cast<const float*>(s.d), *x = static_cast<const float*>(a.x);
+  {  // dx = [dg du] [Wg; Wu]
+    const int split = direct_split(a.tokens, a.hidden, rows2);
+    float* out = static_cast<float*>(a.dx);
+    const DirectArgs g{d, static_cast<const float*>(a.w_gate), static_cast<const float*>(a.w_up), rows2, a.ldg, a.ldu, a.units,
+                       a.tokens, a.hidden, rows2, split, {out, nullptr}, INT64_MAX, {nullptr, nullptr},
+                       split > 1 ? s.parts : nullptr};
+    if ((rc = direct_product(false, true, g, st)) != P2P_OK) return rc;
+    const int64_t n = a.tokens * a.hidden;
+    if (split > 1 && (rc = join_parts(s.parts, split, n, n, 0, nullptr, nullptr, 1.f, out, nullptr, a.dtype, st)) != P2P_OK)
+      return rc;
+  }
+  // [dWg; dWu] = [dg du]^T x
+  const int split = direct_split(rows2, a.hidden, a.tokens);
+  const DirectArgs g{d, x, x, rows2, a.ldx, a.ldx, INT64_MAX, rows2, a.hidden, a.tokens, split,
+                     {static_cast<float*>(a.dw_gate), static_cast<float*>(a.dw_up)}, a.units, {nullptr, nullptr},
+                     split > 1 ? s.parts : nullptr};
+  if ((rc = direct_product(true, true, g, st)) != P2P_OK || split == 1) return rc;
+  const int64_t n = a.units * a.hidden;
+  return join_parts(s.parts, split, 2 * n, n, n, nullptr, nullptr, 1.f, a.dw_gate, a.dw_up, a.dtype, st);
+}
+
 }  // namespace p2p
 
 using namespace p2p;
@@ -218,6 +310,7 @@ extern "C" int32_t p2p_gated_linear_fwd(const p2p_gated_linear_t* a, void* works
   if (need > workspace_bytes || (need && !workspace)) return P2P_ERR_INVALID;
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (gated_direct(*a)) return gated_direct_fwd(*a, s, st);
   Mat x, wg, wu;
   if ((rc = gated_operands(*a, s, &x, &wg, &wu, st)) != P2P_OK) return rc;
   GemmArgs g{};
@@ -244,13 +337,14 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
   if (need > workspace_bytes || !workspace) return P2P_ERR_INVALID;
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (gated_direct(*a)) return gated_direct_bwd(*a, s, st);
   const bool f16_ = a->dtype == P2P_DTYPE_F16;
   Mat x, wg, wu;
   if ((rc = gated_operands(*a, s, &x, &wg, &wu, st)) != P2P_OK) return rc;
   const int64_t pitch = gated_pitch(*a), plane = a->tokens * 2 * pitch;
-  rc = a->dtype == P2P_DTYPE_F32 ? gated_grad<float>(*a, pitch, s.d, st)
-       : f16_                    ? gated_grad<f16>(*a, pitch, s.d, st)
-                                 : gated_grad<bf16>(*a, pitch, s.d, st);
+  rc = a->dtype == P2P_DTYPE_F32 ? gated_grad<float, false>(*a, pitch, s.d, st)
+       : f16_                    ? gated_grad<f16, false>(*a, pitch, s.d, st)
+                                 : gated_grad<bf16, false>(*a, pitch, s.d, st);
   if (rc != P2P_OK) return rc;
   Mat dg{{s.d, s.d + plane, s.d + 2 * plane}, 2 * pitch};
   Mat du{{s.d + pitch, s.d + plane + pitch, s.d + 2 * plane + pitch}, 2 * pitch};
@@ -265,8 +359,8 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
     g.ksplit = plan.split;
     StoreEpi e{{a->dx, nullptr}, 0, 0, a->hidden, a->dtype, {nullptr, nullptr}, 1.f, plan.split > 1 ? s.parts : nullptr, 0};
     if ((rc = gemm_launch<false, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
-    if (plan.split > 1 && (rc = join_parts(s.parts, plan.split, g.M * g.N, g.M * g.N, nullptr, nullptr, 1.f, a->dx, a->dtype,
-                                           st)) != P2P_OK)
+    if (plan.split > 1 && (rc = join_parts(s.parts, plan.split, g.M * g.N, g.M * g.N, 0, nullptr, nullptr, 1.f, a->dx, nullptr,
+                                           a->dtype, st)) != P2P_OK)
       return rc;
   }
   {  // dWg = dg^T x, dWu = du^T x: one product of 2 pitch rows
@@ -279,14 +373,9 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
     StoreEpi e{{a->dw_gate, a->dw_up}, pitch, a->units, a->hidden, a->dtype, {nullptr, nullptr}, 1.f,
                plan.split > 1 ? s.parts : nullptr, 0};
     if ((rc = gemm_launch<true, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
-    if (plan.split > 1) {
-      const int64_t n = a->units * a->hidden, stride = g.M * g.N;
-      if ((rc = join_parts(s.parts, plan.split, stride, n, nullptr, nullptr, 1.f, a->dw_gate, a->dtype, st)) != P2P_OK)
-        return rc;
-      if ((rc = join_parts(s.parts + pitch * a->hidden, plan.split, stride, n, nullptr, nullptr, 1.f, a->dw_up, a->dtype,
-                           st)) != P2P_OK)
-        return rc;
-    }
+    if (plan.split > 1)
+      return join_parts(s.parts, plan.split, g.M * g.N, a->units * a->hidden, pitch * a->hidden, nullptr, nullptr, 1.f,
+                        a->dw_gate, a->dw_up, a->dtype, st);
   }
   return P2P_OK;
 }

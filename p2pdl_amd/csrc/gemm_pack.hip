@@ -66,10 +66,12 @@ int32_t pack_matrices(const PackJob* jobs, int n, int32_t dtype, hipStream_t st)
 }
 
 template <typename T>
-__global__ __launch_bounds__(kBlock) void join_kernel(const float* parts, int nparts, int64_t stride, int64_t n,
-                                                      const float* scale0, const float* scale1, float alpha, T* out) {
+__global__ __launch_bounds__(kBlock) void join_kernel(const float* parts, int nparts, int64_t stride, int64_t n, int64_t second,
+                                                      const float* scale0, const float* scale1, float alpha, T* out0, T* out1) {
   if (scale0) alpha *= ldc(scale0);
   if (scale1) alpha *= ldc(scale1);
+  parts += blockIdx.y * second;
+  T* out = blockIdx.y ? out1 : out0;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * 4; i < n;
        i += static_cast<int64_t>(gridDim.x) * kBlock * 4) {
     float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -86,13 +88,19 @@ __global__ __launch_bounds__(kBlock) void join_kernel(const float* parts, int np
   }
 }
 
-int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, const float* scale0, const float* scale1, float alpha,
-                   void* out, int32_t dtype, hipStream_t st) {
+int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, int64_t second, const float* scale0,
+                   const float* scale1, float alpha, void* out0, void* out1, int32_t dtype, hipStream_t st) {
   if (n == 0) return P2P_OK;
-  const dim3 grid(blocks_for(ceil_div(n, 4))), block(kBlock);
-  if (dtype == P2P_DTYPE_F32) join_kernel<float><<<grid, block, 0, st>>>(parts, nparts, stride, n, scale0, scale1, alpha, static_cast<float*>(out));
-  else if (dtype == P2P_DTYPE_F16) join_kernel<f16><<<grid, block, 0, st>>>(parts, nparts, stride, n, scale0, scale1, alpha, static_cast<f16*>(out));
-  else join_kernel<bf16><<<grid, block, 0, st>>>(parts, nparts, stride, n, scale0, scale1, alpha, static_cast<bf16*>(out));
+  const dim3 grid(blocks_for(ceil_div(n, 4)), out1 ? 2 : 1), block(kBlock);
+  if (dtype == P2P_DTYPE_F32)
+    join_kernel<float><<<grid, block, 0, st>>>(parts, nparts, stride, n, second, scale0, scale1, alpha,
+                                               static_cast<float*>(out0), static_cast<float*>(out1));
+  else if (dtype == P2P_DTYPE_F16)
+    join_kernel<f16><<<grid, block, 0, st>>>(parts, nparts, stride, n, second, scale0, scale1, alpha, static_cast<f16*>(out0),
+                                             static_cast<f16*>(out1));
+  else
+    join_kernel<bf16><<<grid, block, 0, st>>>(parts, nparts, stride, n, second, scale0, scale1, alpha,
+                                              static_cast<bf16*>(out0), static_cast<bf16*>(out1));
   return launch_status();
 }
 

@@ -543,9 +543,9 @@ static inline Mat mat_of(const PackJob& j, int32_t dtype) {
   const bool three = planes_of(dtype) == 3;
   return Mat{{j.dst, three ? j.dst + plane : nullptr, three ? j.dst + 2 * plane : nullptr}, pitch};
 }
-// out[i] = alpha * (parts[i] + parts[stride + i] + ...) in that order
-P2P_INTERNAL int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, const float* scale0,
-                                const float* scale1, float alpha, void* out, int32_t dtype, hipStream_t st);
+// out0[i] = alpha * (parts[i] + parts[stride + i] + ...) in that order, i < n; out1 (nullable) the same from parts + second.
+P2P_INTERNAL int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, int64_t second, const float* scale0,
+                                const float* scale1, float alpha, void* out0, void* out1, int32_t dtype, hipStream_t st);
 
 // The pairs of a product of two operands, appended to g (DUAL: b2 too).
 static inline void add_pairs(GemmArgs* g, const Mat& a, const Mat& b, const Mat* b2, int32_t dtype) {

@@ -22,6 +22,10 @@
 // large vocabulary would sit among float16's subnormal numbers; s and 2^-14
 // are applied to the 32-bit sums.  A target outside [0, V) that is not
 // ignore_index makes the loss and both gradients NaN and reads nothing.
+//
+// Small float32 heads take the product of direct.h, whose k-runs are joined by
+// the kernel that reduces a token's row (forward) or makes d of it: @@
+#include "direct.h"
 #include "gemm_tile.h"
 
 namespace p2p {
@@ -204,6 +208,79 @@ struct GradEpi {
   }
 };
 
+// The direct product's logits in k-runs [runs][T, V], one token per TEAM lanes: lse and the token's loss.
+template <int TEAM>
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void ce_row_kernel(const float* parts, int runs, int64_t T, int64_t V,
+                                                                         const int64_t* target, int64_t ignore, float* lse,
+                                                                         float* row_loss) {
+  constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+  __shared__ float2 stats[TEAM / 64 > 1 ? TEAM / 64 : 1];
+  __shared__ float found[TEAM / 64 > 1 ? TEAM / 64 : 1];
+  const int lane = threadIdx.x % TEAM;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * TEAMS + threadIdx.x / TEAM;
+  if (TEAMS > 1 && t >= T) return;  // a whole wave
+  const int64_t y = ldg(target + t);
+  float2 a = make_float2(-INFINITY, 0.f);
+  float at = 0.f;
+  for (int64_t n = lane * 4; n < V; n += TEAM * 4) {
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < runs; ++p) {
+      float v[4];
+      load_row<float, 4>(parts + (p * T + t) * V, n, V, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] += v[e];
+    }
+    float2 b = make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < V) {
+        b.x = fmaxf(b.x, z[e]);
+        if (n + e == y) at = z[e];
+      }
+    const float base = b.x == -INFINITY ? 0.f : b.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < V) b.y += expf(z[e] - base);
+    a = StatsEpi::join_stats(a, b);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a = StatsEpi::join_stats(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
+  at = wave_sum(at);
+  if constexpr (TEAM > 64) {
+    if ((threadIdx.x & 63) == 0) stats[threadIdx.x / 64] = a, found[threadIdx.x / 64] = at;
+    __syncthreads();
+    a = stats[0], at = found[0];
+    for (int w = 1; w < TEAM / 64; ++w) a = StatsEpi::join_stats(a, stats[w]), at += found[w];
+  }
+  if (lane) return;
+  lse[t] = a.x + logf(a.y);
+  row_loss[t] = y == ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at - a.x);
+}
+
+// d of the logits in k-runs, over the first run.
+__global__ __launch_bounds__(kBlock) void ce_grad_kernel(float* parts, int runs, int64_t T, int64_t V, const float* lse,
+                                                         const int64_t* target, int64_t ignore) {
+  const int64_t per_row = (V + 3) / 4, all = T * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
+       i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t t = i / per_row, n = (i - t * per_row) * 4;
+    const int64_t y = ldg(target + t);
+    const float l = y >= 0 && y < V ? ldg(lse + t) : NAN;
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < runs; ++p) {
+      float v[4];
+      load_row<float, 4>(parts + (p * T + t) * V, n, V, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = y == ignore ? 0.f : expf(z[e] - l) - (n + e == y ? 1.f : 0.f);
+    store_row<float, 4>(parts + t * V, n, V, z);
+  }
+}
+
 static int32_t ce_check(const p2p_linear_ce_t* a) {
   if (!a || !known_dtype(a->dtype) || a->tokens < 0 || a->hidden < 1 || a->vocab < 1 || a->ldx < a->hidden ||
       a->ldw < a->hidden)
@@ -236,8 +313,24 @@ static Plan ce_dw_plan(const p2p_linear_ce_t& a, int64_t rows) {
   return gemm_plan(rows, a.hidden, ksteps(a.tokens, a.dtype == P2P_DTYPE_F32 ? 6 : 1), true);
 }
 
+static bool ce_direct(const p2p_linear_ce_t& a) {
+  return a.dtype == P2P_DTYPE_F32 && direct_pays(a.tokens, a.vocab, a.hidden);
+}
 static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeSpace* s) {
   Carver c{static_cast<char*>(base)};
+  if (ce_direct(a)) {
+    *s = CeSpace{};
+    const int64_t runs = direct_split(a.tokens, a.vocab, a.hidden);
+    s->d = static_cast<uint16_t*>(c.take(runs * a.tokens * a.vocab * 4));
+    if (!backward) {
+      s->row_loss = static_cast<float*>(c.take(a.tokens * 4));
+      return c.used;
+    }
+    const int64_t sx = direct_split(a.tokens, a.hidden, a.vocab), sw = direct_split(a.vocab, a.hidden, a.tokens);
+    if (sx > 1) s->dx_parts = static_cast<float*>(c.take(sx * a.tokens * a.hidden * 4));
+    if (sw > 1) s->dw_parts = static_cast<float*>(c.take(sw * a.vocab * a.hidden * 4));
+    return c.used;
+  }
   const int planes = planes_of(a.dtype);
   const bool x_here = in_place(a.x, a.ldx, a.hidden, a.dtype), w_here = in_place(a.w, a.ldw, a.hidden, a.dtype);
   // pieces: the buffers that grow with one stay under kPieceBytes (one tile's columns at least)
@@ -280,6 +373,61 @@ static int32_t ce_operands(const p2p_linear_ce_t& a, const CeSpace& s, int64_t v
   return pack_matrices(jobs, v0 ? 1 : 2, a.dtype, st);
 }
 
+static int32_t ce_direct_logits(const p2p_linear_ce_t& a, const CeSpace& s, int* runs, hipStream_t st) {
+  *runs = direct_split(a.tokens, a.vocab, a.hidden);
+  const float *x = static_cast<const float*>(a.x), *w = static_cast<const float*>(a.w);
+  const DirectArgs g{x, w, w, a.ldx, a.ldw, a.ldw, INT64_MAX, a.tokens, a.vocab, a.hidden, *runs, {nullptr, nullptr}, INT64_MAX,
+                     {nullptr, nullptr}, reinterpret_cast<float*>(s.d)};
+  return direct_product(false, false, g, st);
+}
+
+static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStream_t st) {
+  int runs;
+  int32_t rc = ce_direct_logits(a, s, &runs, st);
+  if (rc != P2P_OK) return rc;
+  const float* z = reinterpret_cast<const float*>(s.d);
+  if (a.vocab <= 1024)
+    ce_row_kernel<64><<<dim3(static_cast<unsigned>(ceil_div(a.tokens, 4))), dim3(256), 0, st>>>(
+        z, runs, a.tokens, a.vocab, a.target, a.ignore_index, a.lse, s.row_loss);
+  else
+    ce_row_kernel<1024><<<dim3(static_cast<unsigned>(a.tokens)), dim3(1024), 0, st>>>(
+        z, runs, a.tokens, a.vocab, a.target, a.ignore_index, a.lse, s.row_loss);
+  if ((rc = launch_status()) != P2P_OK) return rc;
+  ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, a.target, a.tokens, a.ignore_index, a.mean, a.loss, a.norm);
+  return launch_status();
+}
+
+static int32_t ce_direct_bwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStream_t st) {
+  int runs;
+  int32_t rc = ce_direct_logits(a, s, &runs, st);
+  if (rc != P2P_OK) return rc;
+  float* d = reinterpret_cast<float*>(s.d);
+  const int64_t blocks = ceil_div(a.tokens * ceil_div(a.vocab, 4), kBlock);
+  ce_grad_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
+      d, runs, a.tokens, a.vocab, a.lse, a.target, a.ignore_index);
+  if ((rc = launch_status()) != P2P_OK) return rc;
+  const float *x = static_cast<const float*>(a.x), *w = static_cast<const float*>(a.w);
+  struct Side {
+    bool at;
+    const float* b;
+    int64_t ldb, M, K;
+    void* out;
+    float* parts;
+  };
+  // dx = d W, then dW = d^T x
+  for (const Side& e : {Side{false, w, a.ldw, a.tokens, a.vocab, a.dx, s.dx_parts},
+                        Side{true, x, a.ldx, a.vocab, a.tokens, a.dw, s.dw_parts}}) {
+    const int split = direct_split(e.M, a.hidden, e.K);
+    const DirectArgs g{d, e.b, e.b, a.vocab, e.ldb, e.ldb, INT64_MAX, e.M, a.hidden, e.K, split,
+                       {static_cast<float*>(e.out), nullptr}, INT64_MAX, {a.norm, a.dloss}, split > 1 ? e.parts : nullptr};
+    if ((rc = direct_product(e.at, true, g, st)) != P2P_OK) return rc;
+    const int64_t n = e.M * a.hidden;
+    if (split > 1 && (rc = join_parts(e.parts, split, n, n, 0, a.norm, a.dloss, 1.f, e.out, nullptr, a.dtype, st)) != P2P_OK)
+      return rc;
+  }
+  return P2P_OK;
+}
+
 }  // namespace p2p
 
 using namespace p2p;
@@ -305,6 +453,7 @@ extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, 
   CeSpace s;
   if (ce_carve(*a, false, workspace, &s) > workspace_bytes || !workspace) return P2P_ERR_INVALID;
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
+  if (ce_direct(*a)) return ce_direct_fwd(*a, s, st);
   Mat x, w;
   for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
     const int64_t rows = std::min(s.piece, a->vocab - v0);
@@ -338,6 +487,7 @@ extern "C" int32_t p2p_linear_ce_bwd(const p2p_linear_ce_t* a, void* workspace, 
   if (ce_carve(*a, true, workspace, &s) > workspace_bytes || !workspace) return P2P_ERR_INVALID;
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (ce_direct(*a)) return ce_direct_bwd(*a, s, st);
   const bool f16_ = a->dtype == P2P_DTYPE_F16;
   const float alpha = f16_ ? 1.f / kHalfScale : 1.f;
   Mat x, w;
@@ -375,14 +525,14 @@ extern "C" int32_t p2p_linear_ce_bwd(const p2p_linear_ce_t* a, void* workspace, 
       const StoreEpi e{{out, nullptr}, 0, 0, a->hidden, a->dtype, {a->norm, a->dloss}, alpha,
                        plan.split > 1 ? s.dw_parts : nullptr, 0};
       if ((rc = gemm_launch<true, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
-      if (plan.split > 1 && (rc = join_parts(s.dw_parts, plan.split, g.M * g.N, g.M * g.N, a->norm, a->dloss, alpha, out,
-                                             a->dtype, st)) != P2P_OK)
+      if (plan.split > 1 && (rc = join_parts(s.dw_parts, plan.split, g.M * g.N, g.M * g.N, 0, a->norm, a->dloss, alpha,
+                                             out, nullptr, a->dtype, st)) != P2P_OK)
         return rc;
     }
   }
   if (s.dx_parts) {
     const int64_t n = a->tokens * a->hidden;
-    return join_parts(s.dx_parts, s.dx_plan.split, n, n, a->norm, a->dloss, alpha, a->dx, a->dtype, st);
+    return join_parts(s.dx_parts, s.dx_plan.split, n, n, 0, a->norm, a->dloss, alpha, a->dx, nullptr, a->dtype, st);
   }
   return P2P_OK;
 }
