@@ -314,7 +314,7 @@ static Plan ce_dw_plan(const p2p_linear_ce_t& a, int64_t rows) {
 }
 
 static bool ce_direct(const p2p_linear_ce_t& a) {
-  return a.dtype == P2P_DTYPE_F32 && direct_pays(a.tokens, a.vocab, a.hidden);
+  return a.dtype == P2P_DTYPE_F32 && direct_pays(a.tokens, a.vocab, a.hidden) && a.tokens * a.vocab * 4 <= kPieceBytes;
 }
 static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeSpace* s) {
   Carver c{static_cast<char*>(base)};
