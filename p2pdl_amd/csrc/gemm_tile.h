@@ -89,17 +89,22 @@ using Small = GemmCfg<128, 128, 2, 2>;
 
 constexpr uint32_t kOutside = 0x80000000u;
 using i4 = int __attribute__((ext_vector_type(4)));
-// 16 bytes per lane from base + voff to dst + 16 * lane (dst wave-uniform).  In
-// assembly: for the builtin the compiler waits for all requests before any
-// LDS read (970 against 1216 TFLOP/s at 8192 x 4096 x 32768).  The kernel
-// counts and waits itself; no register is written.  (Four idle cycles: the
-// compiler does not look into the block for an address that a vector
-// instruction has just made scalar.)
-__device__ __forceinline__ void lds_dma(const void* base, uint32_t voff, char* dst) {
+// Twice 16 bytes per lane, from base + v0 to dst + 16 * lane and from base + v1
+// to dst + 1024 + 16 * lane (base, dst wave-uniform).  In assembly: for the
+// builtin the compiler waits for all requests before any LDS read (970 against
+// 1216 TFLOP/s at 8192 x 4096 x 32768).  The kernel counts and waits itself; no
+// register is written.  (Idle cycles: the compiler does not look into the block
+// for an address that a vector instruction has just made scalar, nor for the
+// use of m0.)
+__device__ __forceinline__ void lds_dma2(const void* base, uint32_t v0, uint32_t v1, char* dst) {
   const uint64_t b = uniform_u64(reinterpret_cast<uint64_t>(base));
   const i4 rs = {static_cast<int>(b), static_cast<int>(b >> 32), static_cast<int>(kOutside), 0x00020000};
   const uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((P2P_LDS void*)(dst))));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(voff), "s"(rs) : "memory");
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"s"(to),
+      "s"(to + 1024), "v"(v0), "v"(v1), "s"(rs)
+      : "memory");
 }
 
 template <int EXT>
@@ -108,19 +113,17 @@ __device__ __forceinline__ int line_swizzle(int k) {
   else return ((k >> 3) + (k & 2)) & 3;
 }
 
-// One operand's part of a stage.  EXT: rows of the tile, INSTS: 1-KiB
-// instructions per wave.
-template <bool ROWMAJOR, int EXT, int INSTS>
+// One half of an operand's part of a stage.  EXT: its rows; two 1-KiB instructions per wave.
+template <bool ROWMAJOR, int EXT>
 struct TileLoader {
-  uint32_t voff[INSTS];
-  int kpos[INSTS];
-  uint32_t kstep;  // bytes from one k-step to the next
+  uint32_t voff[2];
+  int kpos[2];
 
-  // Lane addresses relative to the tile's origin; `rows` left from it.
+  // Lane addresses relative to the half's origin; `rows` left from it.
   __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int64_t rows) {
 #pragma unroll
-    for (int j = 0; j < INSTS; ++j) {
-      const int q = wave * INSTS + j;
+    for (int j = 0; j < 2; ++j) {
+      const int q = wave * 2 + j;
       if constexpr (!ROWMAJOR) {
         const int r = q * 8 + lane / 8;
         const int c = (lane & 7) ^ ((r >> 1) & 7);
@@ -130,8 +133,7 @@ struct TileLoader {
         constexpr int CPL = EXT / 8;  // 16-byte chunks of a line
         const int k = q * (64 / CPL) + lane / CPL;
         const int pos = lane % CPL;
-        const int f = line_swizzle<EXT>(k);
-        const int m = ((pos >> 1) ^ f) * 16 + (pos & 1) * 8;
+        const int m = ((pos >> 1) ^ line_swizzle<EXT>(k)) * 16 + (pos & 1) * 8;
         kpos[j] = k;
         voff[j] = m < rows ? static_cast<uint32_t>(k * ld * 2 + m * 2) : kOutside;
       }
@@ -139,12 +141,8 @@ struct TileLoader {
   }
 
   // The k-step at `base` into the image at dst; `left`: k still in the segment.
-  __device__ __forceinline__ void issue(const uint16_t* base, int64_t left, char* dst, int wave) const {
-#pragma unroll
-    for (int j = 0; j < INSTS; ++j) {
-      const uint32_t v = kpos[j] < left ? voff[j] : kOutside;
-      lds_dma(base, v, dst + (wave * INSTS + j) * 1024);
-    }
+  __device__ __forceinline__ void issue(const uint16_t* base, int left, char* dst, int wave) const {
+    lds_dma2(base, kpos[0] < left ? voff[0] : kOutside, kpos[1] < left ? voff[1] : kOutside, dst + wave * 2048);
   }
 };
 
@@ -184,19 +182,42 @@ struct FragReader {
   }
 };
 
-// Blocks go to the eight XCDs in turn; give each XCD a contiguous run of
-// tiles, and order the tiles in groups of 8 rows so that a run shares its
-// operands in that XCD's L2.
-__device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int* tm, int* tn) {
-  const int total = tiles_m * tiles_n;
-  const int pid = blockIdx.x, per = total / 8, extra = total % 8, xcd = pid % 8;
+// Blocks go to the eight XCDs in turn, each with an L2 of its own.  Large
+// tiles: super-blocks of 16 x 16 tiles, as many as run at once, in which an
+// XCD has 4 x 8: it reads 12 panels of the operands for 32 tiles, and the chip 32
+// for 256.  What is left of the matrix at the right and below, and small tiles:
+// a contiguous run of tiles per XCD, ordered in groups of 4 rows.  8192 x 4096
+// x 32768, 32768 x 4096 x 8192 (A^T B): runs in groups of 8 rows 1786, 1951 us, of
+// 4 rows 1776, 1875 us, super-blocks 1752, 1824 us.
+__device__ __forceinline__ void tile_of_run(int pid, int total, int rows, int cols, int* m, int* n) {
+  const int per = total / 8, extra = total % 8, xcd = pid % 8;
   const int t = xcd * per + (xcd < extra ? xcd : extra) + pid / 8;
-  constexpr int G = 8;
-  const int group = t / (G * tiles_n), first = group * G;
-  const int rows = tiles_m - first < G ? tiles_m - first : G;
-  const int in = t - group * G * tiles_n;
-  *tm = first + in % rows;
-  *tn = in / rows;
+  constexpr int G = 4;
+  const int group = t / (G * cols), first = group * G;
+  const int height = rows - first < G ? rows - first : G;
+  const int in = t - first * cols;
+  *n = in / height;
+  *m = first + (in - *n * height);
+}
+template <bool SUPER>
+__device__ __forceinline__ void tile_of_block(int tiles_m, int tiles_n, int* tm, int* tn) {
+  const int pid = blockIdx.x;
+  const int sm = SUPER ? tiles_m / 16 : 0, sn = sm ? tiles_n / 16 : 0, whole = sm * sn * 256;
+  if (SUPER && pid < whole) {
+    const int sup = pid / 256, xcd = pid % 8, slot = pid % 256 / 8;
+    *tn = sup / sm * 16 + xcd % 2 * 8 + slot / 4;
+    *tm = sup % sm * 16 + xcd / 2 * 4 + slot % 4;
+    return;
+  }
+  // the columns past the super-blocks over all rows, then the rows below them
+  const int right = tiles_n - sn * 16, below = whole + tiles_m * right;
+  if (pid < below) {
+    tile_of_run(pid - whole, below - whole, tiles_m, right, tm, tn);
+    *tn += sn * 16;
+  } else {
+    tile_of_run(pid - below, tiles_m * tiles_n - below, tiles_m - sm * 16, sn * 16, tm, tn);
+    *tm += sm * 16;
+  }
 }
 
 // Where an accumulator element lies: acc[mi][nj][i] is C[m][n] of
@@ -216,17 +237,16 @@ struct Place {
 template <bool F16, bool AT, bool BT, bool DUAL, class Cfg, class Epi>
 __global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) void gemm_kernel(GemmArgs g, Epi epi) {
   __shared__ __attribute__((aligned(1024))) char lds[2 * Cfg::STAGE];
-  constexpr int A_INSTS = Cfg::HM / 8 / Cfg::WAVES, B_INSTS = Cfg::HN / 8 / Cfg::WAVES;  // per half and wave
-  static_assert(A_INSTS == B_INSTS, "the counts of the waits below");
+  static_assert(Cfg::HM / 8 / Cfg::WAVES == 2 && Cfg::HN / 8 / Cfg::WAVES == 2, "the counts of the waits below");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_m = static_cast<int>(ceil_div(g.M, Cfg::BM)), tiles_n = static_cast<int>(ceil_div(g.N, Cfg::BN));
   int tm, tn;
-  tile_of_block(tiles_m, tiles_n, &tm, &tn);
+  tile_of_block<Cfg::BLOCKS_PER_CU == 1>(tiles_m, tiles_n, &tm, &tn);
   const int64_t m0 = static_cast<int64_t>(tm) * Cfg::BM, n0 = static_cast<int64_t>(tn) * Cfg::BN;
 
-  TileLoader<AT, Cfg::HM, A_INSTS> la[2];
-  TileLoader<BT, Cfg::HN, B_INSTS> lb[2];
+  TileLoader<AT, Cfg::HM> la[2];
+  TileLoader<BT, Cfg::HN> lb[2];
   int64_t a_org[2], b_org[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -237,8 +257,8 @@ __global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) 
       static_assert(!BT, "two weights: k-contiguous");
       const int64_t units = g.N / 2 - n / 2;
 #pragma unroll
-      for (int j = 0; j < B_INSTS; ++j) {
-        const int r = (wave * B_INSTS + j) * 8 + lane / 8, u = (r >> 5) * 16 + (r & 15);
+      for (int j = 0; j < 2; ++j) {
+        const int r = (wave * 2 + j) * 8 + lane / 8, u = (r >> 5) * 16 + (r & 15);
         const int c = (lane & 7) ^ ((r >> 1) & 7);
         lb[h].kpos[j] = c * 8;
         lb[h].voff[j] = u < units ? static_cast<uint32_t>(u * g.ldb * 2 + c * 16) : kOutside;
@@ -279,12 +299,8 @@ __global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) 
   const auto issue_b = [&](int h, char* stage) {
     char* dst = stage + 2 * Cfg::A_HALF + h * Cfg::B_HALF;
     if constexpr (DUAL) {
-#pragma unroll
-      for (int j = 0; j < B_INSTS; ++j) {
-        const int q = wave * B_INSTS + j;
-        const uint32_t v = lb[h].kpos[j] < left ? lb[h].voff[j] : kOutside;
-        lds_dma(((q >> 1) & 1 ? pb2 : pb) + b_org[h], v, dst + q * 1024);
-      }
+      // a wave's two instructions are rows 16 wave .. + 15 of the half, all of one weight
+      lb[h].issue((wave % 2 ? pb2 : pb) + b_org[h], left, dst, wave);
     } else {
       lb[h].issue(pb + b_org[h], left, dst, wave);
     }
@@ -321,14 +337,16 @@ __global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) 
 #pragma unroll
       for (int i = 0; i < AI; ++i)
 #pragma unroll
-        for (int j = 0; j < BJ; ++j)
+        for (int t = 0; t < BJ; ++t) {
+          const int j = i % 2 ? BJ - 1 - t : t;  // each instruction shares an operand with the last
           acc[ha * AI + i][hb * BJ + j] = mfma16<F16>(fb[hb][j][half], fa[ha][i][half], acc[ha * AI + i][hb * BJ + j]);
+        }
     
   };
   // this wave's reads are done, its oldest half has landed; then everyone's
   const auto phase = [&] {
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(6 * (Cfg::HM / 8 / Cfg::WAVES)) : "memory");
+    asm volatile("s_waitcnt vmcnt(12) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
 
