@@ -185,7 +185,7 @@ struct GatedSpace {
   uint16_t *x, *wg, *wu, *d;
   float* parts;
 };
-static int64_t gated_pitch(const p2p_gated_linear_t& a) { return round_up(a.units, 8); }
+static int64_t gated_pitch(const p2p_gated_linear_t& a) { return line_pitch(a.units); }
 static Plan gated_dx_plan(const p2p_gated_linear_t& a) {
   return gemm_plan(a.tokens, a.hidden, ksteps(a.units, a.dtype == P2P_DTYPE_F32 ? 12 : 2), true);
 }
@@ -240,9 +240,9 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
 
 // x, w_gate and w_up as the products read them, copied (in one launch) where the workspace has a place for it.
 static int32_t gated_operands(const p2p_gated_linear_t& a, const GatedSpace& s, Mat* x, Mat* wg, Mat* wu, hipStream_t st) {
-  const PackJob jobs[3] = {{a.x, a.ldx, a.tokens, a.hidden, s.x},
-                           {a.w_gate, a.ldg, a.units, a.hidden, s.wg},
-                           {a.w_up, a.ldu, a.units, a.hidden, s.wu}};
+  const PackJob jobs[3] = {{a.x, a.ldx, a.tokens, a.hidden, s.x, 0},
+                           {a.w_gate, a.ldg, a.units, a.hidden, s.wg, 0},
+                           {a.w_up, a.ldu, a.units, a.hidden, s.wu, 0}};
   *x = mat_of(jobs[0], a.dtype);
   *wg = mat_of(jobs[1], a.dtype);
   *wu = mat_of(jobs[2], a.dtype);

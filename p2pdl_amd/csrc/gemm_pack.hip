@@ -13,7 +13,7 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(PackJobs jobs) {
   const PackJob& job = jobs.job[blockIdx.y];
   const T* src = static_cast<const T*>(job.src);
   uint16_t* dst = job.dst;
-  const int64_t ld = job.ld, cols = job.cols, pitch = (cols + 7) / 8 * 8, plane = job.rows * pitch;
+  const int64_t ld = job.ld, cols = job.cols, pitch = job.pitch, plane = job.rows * pitch;
   const int64_t per_row = pitch / 8, all = job.rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
        i += static_cast<int64_t>(gridDim.x) * kBlock) {
@@ -55,8 +55,9 @@ int32_t pack_matrices(const PackJob* jobs, int n, int32_t dtype, hipStream_t st)
   int used = 0;
   for (int i = 0; i < n; ++i) {
     if (!jobs[i].dst || jobs[i].rows == 0) continue;
-    all.job[used++] = jobs[i];
-    most = std::max(most, jobs[i].rows * (round_up(jobs[i].cols, 8) / 8));
+    all.job[used] = jobs[i];
+    all.job[used++].pitch = line_pitch(jobs[i].cols);
+    most = std::max(most, jobs[i].rows * (line_pitch(jobs[i].cols) / 8));
   }
   if (!used) return P2P_OK;
   const dim3 grid(blocks_for(most), used);

@@ -539,25 +539,29 @@ static inline bool in_place(const void* p, int64_t ld, int64_t cols, int32_t dty
   return dtype != P2P_DTYPE_F32 && aligned_to(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld <= kMaxPitch;
 }
 static inline int64_t round_up(int64_t n, int64_t to) { return ceil_div(n, to) * to; }
+// The pitch of a copy or of d: whole 128-byte lines, on which a tile's rows begin (1023 x 1001 x 32003
+// float16 with pitches of 16 bytes: @@).
+static inline int64_t line_pitch(int64_t cols) { return round_up(cols, cols > 32 ? 64 : 8); }
 static inline int planes_of(int32_t dtype) { return dtype == P2P_DTYPE_F32 ? 3 : 1; }
 static inline int64_t packed_bytes(int64_t rows, int64_t cols, int32_t dtype) {
-  return round_up(rows * round_up(cols, 8) * 2 * planes_of(dtype), 256);
+  return round_up(rows * line_pitch(cols) * 2 * planes_of(dtype), 256);
 }
 
-// src [rows, cols], pitch ld, as 16-bit planes of pitch round_up(cols, 8) at dst, zeros in the
+// src [rows, cols], pitch ld, as 16-bit planes of pitch line_pitch(cols) at dst, zeros in the
 // added columns.  Up to kMaxPack of them in one launch; those without a dst are left out.
 constexpr int kMaxPack = 3;
 struct PackJob {
   const void* src;
   int64_t ld, rows, cols;
   uint16_t* dst;
+  int64_t pitch;  // set by pack_matrices
 };
 P2P_INTERNAL int32_t pack_matrices(const PackJob* jobs, int n, int32_t dtype, hipStream_t st);
 
 // What the product reads of a job: its copy, or src in place where it has none.
 static inline Mat mat_of(const PackJob& j, int32_t dtype) {
   if (!j.dst) return Mat{{static_cast<const uint16_t*>(j.src), nullptr, nullptr}, j.ld};
-  const int64_t pitch = round_up(j.cols, 8), plane = j.rows * pitch;
+  const int64_t pitch = line_pitch(j.cols), plane = j.rows * pitch;
   const bool three = planes_of(dtype) == 3;
   return Mat{{j.dst, three ? j.dst + plane : nullptr, three ? j.dst + 2 * plane : nullptr}, pitch};
 }

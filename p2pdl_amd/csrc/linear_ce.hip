@@ -43,22 +43,35 @@ struct StatsEpi {
 
   template <class Cfg>
   __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
-    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+    const int i16 = p.lane & 15;
+    const int64_t n0 = p.n0 + (p.lane >> 4) * 4;  // this lane's columns: n0 + Cfg::col(j) + e
+    const int cols = static_cast<int>(std::min<int64_t>(g.N - n0, Cfg::BN));  // left from n0
+    const bool whole = p.n0 + Cfg::HN + 32 <= g.N;  // of the wave's columns none is past the end
     float2* rows = reinterpret_cast<float2*>(lds);  // [WN][BM]
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
       const int64_t m = p.m0 + Cfg::row(i) + i16;
-      const int64_t t = m < g.M ? ldg(target + m) - first - p.n0 : -1;
+      const int64_t y = m < g.M ? ldg(target + m) - first - n0 : -1;
+      const int t = y >= 0 && y < Cfg::BN ? static_cast<int>(y) : -1;
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < Cfg::NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (Cfg::col(j) + e >= cols) acc[i][j][e] = -INFINITY;
+      }
+      if (__any(t >= 0)) {  // few tiles hold a token's target
+#pragma unroll
+        for (int j = 0; j < Cfg::NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (Cfg::col(j) + e == t && t < cols) stg(at_target + m, acc[i][j][e]);
+      }
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < Cfg::NJ; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = Cfg::col(j) + q4 + e;
-          if (p.n0 + n >= g.N) acc[i][j][e] = -INFINITY;
-          else if (n == t) stg(at_target + m, acc[i][j][e]);
-          top = fmaxf(top, acc[i][j][e]);  // passes over a NaN, which the sum below takes up
-        }
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);  // passes over a NaN, which the sum below takes up
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float base = top == -INFINITY ? 0.f : top;  // -inf throughout: a sum of zeros
@@ -67,8 +80,8 @@ struct StatsEpi {
       for (int j = 0; j < Cfg::NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = acc[i][j][e] - base;
-          s += p.n0 + Cfg::col(j) + q4 + e < g.N ? (precise ? expf(x) : __expf(x)) : 0.f;
+          const float x = acc[i][j][e] - base;  // a column past the end: exp(-inf)
+          s += precise ? expf(x) : __expf(x);
         }
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
@@ -80,10 +93,7 @@ struct StatsEpi {
       if (m >= g.M) continue;
       float2 a = rows[r];
 #pragma unroll
-      for (int w = 1; w < Cfg::WN; ++w) {
-        const float2 b = rows[w * Cfg::BM + r];
-        a = join_stats(a, b);
-      }
+      for (int w = 1; w < Cfg::WN; ++w) a = join_stats(a, rows[w * Cfg::BM + r]);
       part[p.tn * g.M + m] = a;
     }
   }
@@ -99,31 +109,30 @@ struct StatsEpi {
 
 // Joins the column tiles of a piece, and with what earlier pieces left in
 // `state`; after the last piece, lse and the token's loss.  64 tokens per
-// block, 4 lanes of column tiles each.
-__global__ __launch_bounds__(kBlock) void ce_join_kernel(const float2* part, int tiles, int64_t T, float2* state, int first,
-                                                         int last, const int64_t* target, int64_t V, int64_t ignore,
-                                                         const float* at_target, float* lse, float* row_loss) {
-  __shared__ float2 groups[4][64];
+// block, a wave for every sixteenth of the tiles.
+__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int tiles, int64_t T, float2* state, int first,
+                                                       int last, const int64_t* target, int64_t V, int64_t ignore,
+                                                       const float* at_target, float* lse, float* row_loss) {
+  __shared__ float2 groups[16][64];
   const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 64 + lane;
   float2 a = make_float2(-INFINITY, 0.f);
   if (t < T) {
-    const int from = tiles * group / 4, to = tiles * (group + 1) / 4;
-#pragma unroll 4
+    const int from = tiles * group / 16, to = tiles * (group + 1) / 16;
+#pragma unroll 8
     for (int i = from; i < to; ++i) a = StatsEpi::join_stats(a, part[i * T + t]);
   }
   groups[group][lane] = a;
   __syncthreads();
   if (group || t >= T) return;
 #pragma unroll
-  for (int q = 1; q < 4; ++q) a = StatsEpi::join_stats(a, groups[q][lane]);
+  for (int q = 1; q < 16; ++q) a = StatsEpi::join_stats(a, groups[q][lane]);
   if (!first) a = StatsEpi::join_stats(state[t], a);
   if (!last) {
     state[t] = a;
     return;
   }
-  const float l = a.x + logf(a.y);
-  lse[t] = l;
+  lse[t] = a.x + logf(a.y);
   const int64_t y = target[t];
   // z - max and log(sum) apart: lse - z would lose the digits of a large maximum
   row_loss[t] = y == ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at_target[t] - a.x);
@@ -167,41 +176,54 @@ struct GradEpi {
 
   template <class Cfg>
   __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char*) const {
-    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+    const int64_t n0 = p.n0 + (p.lane >> 4) * 4;
+    const int cols = static_cast<int>(std::min<int64_t>(g.N - n0, Cfg::BN));
+    const int width = static_cast<int>(std::min<int64_t>(pitch - n0, Cfg::BN));  // with the padding
+    const bool whole = p.n0 + Cfg::HN + 32 <= g.N;
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + Cfg::row(i) + i16;
-      if (m >= g.M) continue;
-      const int64_t y = ldg(target + m);
+      const int64_t m = p.m0 + Cfg::row(i) + (p.lane & 15);
+      const int64_t y = m < g.M ? ldg(target + m) : ignore, at = y - first - n0;
       const bool counts = y != ignore;
-      const float l = y >= 0 && y < vocab ? ldg(lse + m) : NAN;
-      const int64_t t = y - first;
+      const float l = !counts ? 0.f : y >= 0 && y < vocab ? ldg(lse + m) : NAN;
+      const int t = counts && at >= 0 && at < Cfg::BN ? static_cast<int>(at) : -1;
 #pragma unroll
-      for (int j = 0; j < Cfg::NJ; ++j) {
-        const int64_t n = p.n0 + Cfg::col(j) + q4;
-        if (n >= pitch) continue;
-        f4 v;
+      for (int j = 0; j < Cfg::NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = acc[i][j][e] - l;
-          const float pr = dtype == P2P_DTYPE_F32 ? expf(x) : __expf(x);
-          v[e] = counts && n + e < g.N ? (n + e == t ? pr - 1.f : pr) : 0.f;
+          acc[i][j][e] = counts ? (dtype == P2P_DTYPE_F32 ? expf(x) : __expf(x)) : 0.f;
         }
-        uint16_t* to = d + m * pitch + n;
+      if (__any(t >= 0)) {  // few tiles hold a token's target
+#pragma unroll
+        for (int j = 0; j < Cfg::NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] -= Cfg::col(j) + e == t ? 1.f : 0.f;
+      }
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j) {
+        if (!whole) {
+          if (Cfg::col(j) >= width) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (Cfg::col(j) + e >= cols) acc[i][j][e] = 0.f;
+        }
+        uint16_t* to = d + m * pitch + n0 + Cfg::col(j);
         if (dtype == P2P_DTYPE_F32) {
           Pack<uint16_t, 4> o[3];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const Planes s = split3(v[e]);
+            const Planes s = split3(acc[i][j][e]);
 #pragma unroll
             for (int q = 0; q < 3; ++q) o[q].v[e] = s.p[q];
           }
 #pragma unroll
           for (int q = 0; q < 3; ++q) store_pack<uint16_t, 4>(to + q * plane, o[q]);
         } else if (dtype == P2P_DTYPE_F16) {
-          store4(reinterpret_cast<f16*>(to), 0, 4, v * kHalfScale);
+          store4(reinterpret_cast<f16*>(to), 0, 4, acc[i][j] * kHalfScale);
         } else {
-          store4(reinterpret_cast<bf16*>(to), 0, 4, v);
+          store4(reinterpret_cast<bf16*>(to), 0, 4, acc[i][j]);
         }
       }
     }
@@ -335,7 +357,7 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
   const bool x_here = in_place(a.x, a.ldx, a.hidden, a.dtype), w_here = in_place(a.w, a.ldw, a.hidden, a.dtype);
   // pieces: the buffers that grow with one stay under kPieceBytes (one tile's columns at least)
   int64_t per_row = backward ? a.tokens * 2 * planes : ceil_div(a.tokens * 8, Small::BN);
-  if (!w_here) per_row = std::max(per_row, round_up(a.hidden, 8) * 2 * planes);
+  if (!w_here) per_row = std::max(per_row, line_pitch(a.hidden) * 2 * planes);
   int64_t piece = std::max<int64_t>(1, kPieceBytes / per_row / Big::BN) * Big::BN;
   if (piece >= a.vocab) piece = a.vocab;
   else piece = round_up(ceil_div(a.vocab, ceil_div(a.vocab, piece)), Big::BN);  // pieces of about one size
@@ -350,7 +372,7 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
     return c.used;
   }
   const int nseg = a.dtype == P2P_DTYPE_F32 ? 6 : 1;
-  s->d = static_cast<uint16_t*>(c.take(a.tokens * round_up(piece, 8) * 2 * planes));
+  s->d = static_cast<uint16_t*>(c.take(a.tokens * line_pitch(piece) * 2 * planes));
   s->dx_plan = gemm_plan(a.tokens, a.hidden, ksteps(piece, nseg), true);
   const bool parts = s->dx_plan.split > 1 || piece < a.vocab;
   s->dx_parts = parts ? static_cast<float*>(c.take(s->dx_plan.split * a.tokens * a.hidden * 4)) : nullptr;
@@ -367,7 +389,7 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
 static int32_t ce_operands(const p2p_linear_ce_t& a, const CeSpace& s, int64_t v0, int64_t rows, Mat* x, Mat* w,
                            hipStream_t st) {
   const char* p = static_cast<const char*>(a.w) + v0 * a.ldw * dtype_bytes(a.dtype);
-  const PackJob jobs[2] = {{p, a.ldw, rows, a.hidden, s.w}, {a.x, a.ldx, a.tokens, a.hidden, s.x}};
+  const PackJob jobs[2] = {{p, a.ldw, rows, a.hidden, s.w, 0}, {a.x, a.ldx, a.tokens, a.hidden, s.x, 0}};
   *w = mat_of(jobs[0], a.dtype);
   *x = mat_of(jobs[1], a.dtype);
   return pack_matrices(jobs, v0 ? 1 : 2, a.dtype, st);
@@ -467,7 +489,7 @@ extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, 
     const bool big = gemm_plan(g.M, g.N, ksteps(g.K, g.nseg), false).big;
     if ((rc = gemm_launch<false, false, false>(g, a->dtype == P2P_DTYPE_F16, big, e, st)) != P2P_OK) return rc;
     const int tiles = static_cast<int>(ceil_div(rows, big ? Big::BN : Small::BN));
-    ce_join_kernel<<<dim3(static_cast<unsigned>(ceil_div(a->tokens, 64))), dim3(kBlock), 0, st>>>(
+    ce_join_kernel<<<dim3(static_cast<unsigned>(ceil_div(a->tokens, 64))), dim3(1024), 0, st>>>(
         s.part, tiles, a->tokens, s.state, v0 == 0, v0 + rows == a->vocab, a->target, a->vocab, a->ignore_index, s.at_target,
         a->lse, s.row_loss);
     if ((rc = launch_status()) != P2P_OK) return rc;
@@ -492,7 +514,7 @@ extern "C" int32_t p2p_linear_ce_bwd(const p2p_linear_ce_t* a, void* workspace, 
   const float alpha = f16_ ? 1.f / kHalfScale : 1.f;
   Mat x, w;
   for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
-    const int64_t rows = std::min(s.piece, a->vocab - v0), pitch = round_up(rows, 8), plane = a->tokens * pitch;
+    const int64_t rows = std::min(s.piece, a->vocab - v0), pitch = line_pitch(rows), plane = a->tokens * pitch;
     if ((rc = ce_operands(*a, s, v0, rows, &x, &w, st)) != P2P_OK) return rc;
     {
       GemmArgs g{};
