@@ -29,10 +29,17 @@ the ``*_forward`` / ``*_backward`` pairs.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
+
+# The calls of a step on dense tensors, checked and launched in C++ (csrc/train_host.cpp); its functions
+# return None for what the Python below has to copy, widen or refuse.
+_host = N.host_extension("_train_host")
+_bound = False
 
 DTYPES = {torch.float32: N.P2P_DTYPE_F32, torch.float16: N.P2P_DTYPE_F16, torch.bfloat16: N.P2P_DTYPE_BF16}
 ACTIVATIONS = {"silu": N.P2P_ACT_SILU, "gelu": N.P2P_ACT_GELU, "relu": N.P2P_ACT_RELU}
@@ -40,8 +47,21 @@ MAX_NORM_COLS = 16384
 MAX_FEATURES = (1 << 22) - 8
 
 
+def _bind() -> None:
+    """Gives csrc/train_host.cpp the library's functions (those of struct Abi there, in that order)."""
+    global _bound
+    L = N.lib()
+    names = ("layernorm_fwd", "layernorm_bwd_workspace", "layernorm_bwd", "dropout", "gated_linear_workspace",
+             "gated_linear_fwd", "gated_linear_bwd", "linear_ce_workspace", "linear_ce_fwd", "linear_ce_bwd")
+    _host.bind(tuple(ctypes.cast(getattr(L, "p2p_" + n), ctypes.c_void_p).value for n in names), N.check,
+               torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    _bound = True
+
+
 def _call(fn, what: str, dev: torch.device, *args) -> None:
     """fn(*args, the current stream of dev) with dev as the current device."""
+    if not _bound:
+        _bind()
     if dev.index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
@@ -139,6 +159,9 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension
     (at most 16384 features).  Returns (y, mean, rstd), the latter two float32
     of x's leading shape, for layer_norm_backward."""
+    done = _host.layer_norm_forward(x, weight, bias, eps)
+    if done is not None:
+        return done
     dt = _norm_inputs(x, weight, bias)
     dev, cols = x.device, x.shape[-1]
     rows = x.numel() // cols
@@ -156,6 +179,9 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
                         weight: torch.Tensor | None = None):
     """(dx, dweight, dbias) of layer_norm_forward; the latter two are None without a weight."""
+    done = _host.layer_norm_backward(dy, x, mean, rstd, weight)
+    if done is not None:
+        return done
     dt = _norm_inputs(x, weight, None)
     _like(dy, x, "dy", x.shape)
     _stat(mean, x, "mean", x.shape[:-1])
@@ -206,6 +232,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
 # ------------------------------------------------------------------ dropout
 def _dropout(x, p, seed, offset, residual):
+    done = _host.dropout(x, p, seed, offset, residual)
+    if done is not None:
+        return done
     dt = _dtype(x, "x")
     p = float(p)
     if not 0.0 <= p <= 1.0:
@@ -311,6 +340,9 @@ def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
     features], act "silu", "gelu" (exact) or "relu".  Returns (h, gate, up): the
     two products in float32, which gated_linear_backward reads (None with ``save``
     false, for inference)."""
+    done = _host.gated_linear_forward(x, w_gate, w_up, ACTIVATIONS.get(activation), save)
+    if done is not None:
+        return done
     dt, act = _gated_inputs(x, w_gate, w_up, activation)
     dev, shape = x.device, x.shape[:-1] + w_gate.shape[:1]
     h = torch.empty(shape, dtype=x.dtype, device=dev)
@@ -331,6 +363,9 @@ def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
 def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                           gate: torch.Tensor, up: torch.Tensor, activation: str = "silu"):
     """(dx, dw_gate, dw_up) of gated_linear_forward."""
+    done = _host.gated_linear_backward(dh, x, w_gate, w_up, gate, up, ACTIVATIONS.get(activation))
+    if done is not None:
+        return done
     dt, act = _gated_inputs(x, w_gate, w_up, activation)
     dev, shape = x.device, x.shape[:-1] + w_gate.shape[:1]
     _like(dh, x, "dh", shape)
@@ -411,6 +446,9 @@ def linear_cross_entropy_forward(x: torch.Tensor, weight: torch.Tensor, target: 
     of exponentials and the factor of the mean, which the backward pass reads."""
     if reduction not in ("mean", "sum"):
         raise ValueError(f"unknown reduction {reduction!r}; expected 'mean' or 'sum'")
+    done = _host.linear_cross_entropy_forward(x, weight, target, ignore_index, reduction == "mean")
+    if done is not None:
+        return done
     a, keep = _ce_args(x, weight, target, ignore_index)
     dev = x.device
     loss, norm = torch.empty(2, dtype=torch.float32, device=dev).unbind(0)
@@ -429,6 +467,9 @@ def linear_cross_entropy_backward(x: torch.Tensor, weight: torch.Tensor, target:
                                   norm: torch.Tensor, dloss: torch.Tensor | None = None, ignore_index: int = -100):
     """(dx, dweight) of linear_cross_entropy_forward's loss, times ``dloss`` (one
     float32 on the device; a loss scale, say) if given."""
+    done = _host.linear_cross_entropy_backward(x, weight, target, lse, norm, dloss, ignore_index)
+    if done is not None:
+        return done
     a, keep = _ce_args(x, weight, target, ignore_index)
     _stat(lse, x, "lse", target.shape)
     _stat(norm, x, "norm", torch.Size(()))
