@@ -27,7 +27,7 @@ struct DirectArgs {
 static inline bool direct_pays(int64_t M, int64_t N, int64_t K) {
   return M <= 128 || static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K) <= 4.0e9;
 }
-// Its k-runs: enough blocks for every CU twice, at least four k-steps each.
+// Its k-runs: enough blocks for every CU twice, at least two k-steps each.
 P2P_INTERNAL int direct_split(int64_t M, int64_t N, int64_t K);
 
 // AT / BT: the operand's lines are k (row-contiguous), else rows (k-contiguous).

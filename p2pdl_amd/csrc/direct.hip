@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void direct_kernel(DirectArgs g) {
 
 int direct_split(int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = ceil_div(M, M <= 32 ? 32 : 64) * ceil_div(N, kDirectN), steps = ceil_div(K, kDirectK);
-  return static_cast<int>(std::max<int64_t>(1, std::min({512 / tiles, steps / 4, int64_t(16)})));
+  return static_cast<int>(std::max<int64_t>(1, std::min({512 / tiles, steps / 2, int64_t(16)})));
 }
 
 template <bool AT, bool BT>

@@ -146,16 +146,10 @@ __global__ __launch_bounds__(kBlock) void gated_join_kernel(const float* parts, 
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
        i += static_cast<int64_t>(gridDim.x) * kBlock) {
     const int64_t r = i / per_row, c = (i - r * per_row) * 4;
-    float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f}, o[4];
-#pragma unroll 4
-    for (int p = 0; p < runs; ++p) {
-      const float* row = parts + (p * rows + r) * 2 * units;
-      float x[4], y[4];
-      load_row<float, 4>(row, c, units, x);
-      load_row<float, 4>(row + units, c, units, y);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) g[e] += x[e], u[e] += y[e];
-    }
+    float g[4], u[4], o[4];
+    const float* row = parts + r * 2 * units;
+    sum_runs<4>(row, rows * 2 * units, runs, c, units, g);
+    sum_runs<4>(row + units, rows * 2 * units, runs, c, units, u);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float a, da;

@@ -75,14 +75,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(const float* parts, int np
   T* out = blockIdx.y ? out1 : out0;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * 4; i < n;
        i += static_cast<int64_t>(gridDim.x) * kBlock * 4) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = 0; p < nparts; ++p) {
-      float v[4];
-      load_row<float, 4>(parts + p * stride, i, n, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] += v[e];
-    }
+    float s[4];
+    sum_runs<4>(parts, stride, nparts, i, n, s);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] *= alpha;
     store_row<T, 4>(out, i, n, s);

@@ -22,6 +22,7 @@ namespace p2p {
 constexpr int kLnMaxCols = 16384;
 constexpr int kLnFwdBlock = 256;
 constexpr int kLnBwdBlock = 512;
+constexpr int kLnAlone = 8;  // passes over its rows that one block makes alone
 constexpr int kLnMaxParts = 512;  // partial rows of dw / db: two blocks of 512 lanes per CU
 
 // Sum over a team of TEAM lanes (one wave, or several through LDS: then every
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layer
 template <typename T, int TEAM, int NV, bool DENSE>
 __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void layernorm_bwd_kernel(
     const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, const float* mean_in, const float* rstd_in, int64_t rows,
-    int cols, T* dx, float* parts) {
+    int cols, T* dx, float* parts, T* dw, T* db) {
   constexpr int V = Vec16<T>::N;
   constexpr int TEAMS = kLnBwdBlock / TEAM, WAVES = TEAM / 64;
   __shared__ float2 sums[2][kLnBwdBlock / 64];
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
       }
     }
   }
-  if (!parts) return;
+  if (!parts && !dw && !db) return;
   float* out = parts + static_cast<int64_t>(blockIdx.x) * 2 * cols;
   // the teams' sums of each column, added in team order by the first team
 #pragma unroll
@@ -210,7 +211,11 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
         }
       }
       const int c = (i * TEAM + lane) * V;
-      if (team == 0 && c < cols) store_row<float, V>(out + which * cols, c, cols, v);
+      if (team == 0 && c < cols) {
+        T* const whole = which ? db : dw;  // a block alone has the whole sums
+        if (parts) store_row<float, V>(out + which * cols, c, cols, v);
+        else if (whole) store_row<T, V>(whole, c, cols, v);
+      }
     }
 }
 
@@ -279,7 +284,9 @@ template <typename T>
 static int ln_parts_of(int64_t rows, int cols) {
   int teams = 1;
   ln_team<T>(cols, [&](auto team, auto) { teams = kLnBwdBlock / decltype(team)::value; });
-  return static_cast<int>(std::min<int64_t>(ceil_div(rows, teams), kLnMaxParts));
+  // few rows: one block, which needs no second launch
+  const int64_t blocks = ceil_div(rows, teams);
+  return static_cast<int>(blocks <= kLnAlone ? 1 : std::min<int64_t>(blocks, kLnMaxParts));
 }
 static int ln_parts(int64_t rows, int cols, int32_t dtype) {
   return dtype == P2P_DTYPE_F32 ? ln_parts_of<float>(rows, cols) : ln_parts_of<f16>(rows, cols);
@@ -302,11 +309,11 @@ static int32_t ln_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const 
                       const float* rstd, int64_t rows, int cols, T* dx, T* dw, T* db, float* parts, int32_t dtype,
                       hipStream_t st) {
   const int n = ln_parts(rows, cols, dtype);
-  float* const to = dw || db ? parts : nullptr;
+  float* const to = (dw || db) && n > 1 ? parts : nullptr;
   ln_team<T>(cols, [&](auto team, auto nv) {
     constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
     const auto kernel = cols % Vec16<T>::N == 0 ? layernorm_bwd_kernel<T, TEAM, NV, true> : layernorm_bwd_kernel<T, TEAM, NV, false>;
-    kernel<<<dim3(n), dim3(kLnBwdBlock), 0, st>>>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, to);
+    kernel<<<dim3(n), dim3(kLnBwdBlock), 0, st>>>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, to, dw, db);
   });
   const int32_t rc = launch_status();
   if (rc != P2P_OK || !to) return rc;

@@ -107,12 +107,52 @@ struct StatsEpi {
   }
 };
 
+// loss and norm, by one block of 1024 in a fixed order, in 64 bits.
+struct LossOut {
+  const int64_t* target;
+  int64_t T, ignore;
+  int mean;
+  float *loss, *norm;
+};
+__device__ void ce_loss_of(const float* row_loss, const LossOut& o) {
+  __shared__ double sums[16];
+  __shared__ int64_t counts[16];
+  double s = 0.0;
+  int64_t n = 0;
+  for (int64_t t = threadIdx.x; t < o.T; t += 1024) {
+    s += static_cast<double>(row_loss[t]);
+    n += o.target[t] != o.ignore;
+  }
+#pragma unroll
+  for (int h = 32; h > 0; h >>= 1) {
+    s += __shfl_xor(s, h, 64);
+    n += __shfl_xor(n, h, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sums[threadIdx.x / 64] = s;
+    counts[threadIdx.x / 64] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < 16; ++w) {
+      sums[0] += sums[w];
+      counts[0] += counts[w];
+    }
+  if (threadIdx.x == 0) {
+    const double f = !o.mean ? 1.0 : counts[0] ? 1.0 / static_cast<double>(counts[0]) : 0.0;
+    *o.loss = static_cast<float>(o.mean && counts[0] ? sums[0] / static_cast<double>(counts[0]) : sums[0]);
+    *o.norm = static_cast<float>(f);
+  }
+}
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* row_loss, LossOut o) { ce_loss_of(row_loss, o); }
+
 // Joins the column tiles of a piece, and with what earlier pieces left in
 // `state`; after the last piece, lse and the token's loss.  64 tokens per
-// block, a wave for every sixteenth of the tiles.
-__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int tiles, int64_t T, float2* state, int first,
-                                                       int last, const int64_t* target, int64_t V, int64_t ignore,
-                                                       const float* at_target, float* lse, float* row_loss) {
+// block, a wave for every sixteenth of the tiles; one block sums the losses itself.
+__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int tiles, float2* state, int first, int last,
+                                                       int64_t V, const float* at_target, float* lse, float* row_loss,
+                                                       LossOut o) {
+  const int64_t T = o.T;
   __shared__ float2 groups[16][64];
   const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 64 + lane;
@@ -124,44 +164,22 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int t
   }
   groups[group][lane] = a;
   __syncthreads();
-  if (group || t >= T) return;
+  if (group == 0 && t < T) {
 #pragma unroll
-  for (int q = 1; q < 16; ++q) a = StatsEpi::join_stats(a, groups[q][lane]);
-  if (!first) a = StatsEpi::join_stats(state[t], a);
-  if (!last) {
-    state[t] = a;
-    return;
-  }
-  lse[t] = a.x + logf(a.y);
-  const int64_t y = target[t];
-  // z - max and log(sum) apart: lse - z would lose the digits of a large maximum
-  row_loss[t] = y == ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at_target[t] - a.x);
-}
-
-// loss and norm, by one block in a fixed order, in 64 bits.
-__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* row_loss, const int64_t* target, int64_t T, int64_t ignore,
-                                                       int mean, float* loss, float* norm) {
-  __shared__ double sums[1024];
-  __shared__ int64_t counts[1024];
-  double s = 0.0;
-  int64_t n = 0;
-  for (int64_t t = threadIdx.x; t < T; t += 1024) {
-    s += static_cast<double>(row_loss[t]);
-    n += target[t] != ignore;
-  }
-  sums[threadIdx.x] = s;
-  counts[threadIdx.x] = n;
-  for (int o = 512; o > 0; o >>= 1) {
-    __syncthreads();
-    if (threadIdx.x < o) {
-      sums[threadIdx.x] += sums[threadIdx.x + o];
-      counts[threadIdx.x] += counts[threadIdx.x + o];
+    for (int q = 1; q < 16; ++q) a = StatsEpi::join_stats(a, groups[q][lane]);
+    if (!first) a = StatsEpi::join_stats(state[t], a);
+    if (!last) {
+      state[t] = a;
+    } else {
+      lse[t] = a.x + logf(a.y);
+      const int64_t y = o.target[t];
+      // z - max and log(sum) apart: lse - z would lose the digits of a large maximum
+      row_loss[t] = y == o.ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at_target[t] - a.x);
     }
   }
-  if (threadIdx.x == 0) {
-    const double f = !mean ? 1.0 : counts[0] ? 1.0 / static_cast<double>(counts[0]) : 0.0;
-    *loss = static_cast<float>(mean && counts[0] ? sums[0] / static_cast<double>(counts[0]) : sums[0]);
-    *norm = static_cast<float>(f);
+  if (last && gridDim.x == 1) {
+    __syncthreads();
+    ce_loss_of(row_loss, o);
   }
 }
 
@@ -230,54 +248,61 @@ struct GradEpi {
   }
 };
 
-// The direct product's logits in k-runs [runs][T, V], one token per TEAM lanes: lse and the token's loss.
+// The direct product's logits in k-runs [runs][T, V], a token per TEAM of a block's 1024 lanes: lse and the
+// token's loss.  A block alone with up to 64 tokens sums their losses itself.
 template <int TEAM>
-__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void ce_row_kernel(const float* parts, int runs, int64_t T, int64_t V,
-                                                                         const int64_t* target, int64_t ignore, float* lse,
-                                                                         float* row_loss) {
-  constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
-  __shared__ float2 stats[TEAM / 64 > 1 ? TEAM / 64 : 1];
-  __shared__ float found[TEAM / 64 > 1 ? TEAM / 64 : 1];
+__global__ __launch_bounds__(1024) void ce_row_kernel(const float* parts, int runs, int64_t V, float* lse, float* row_loss,
+                                                      LossOut o) {
+  constexpr int TEAMS = 1024 / TEAM;
+  __shared__ float2 stats[16];
+  __shared__ float found[16], losses[64];
+  const int64_t T = o.T;
+  const bool alone = gridDim.x == 1 && T <= 64;
   const int lane = threadIdx.x % TEAM;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * TEAMS + threadIdx.x / TEAM;
-  if (TEAMS > 1 && t >= T) return;  // a whole wave
-  const int64_t y = ldg(target + t);
-  float2 a = make_float2(-INFINITY, 0.f);
-  float at = 0.f;
-  for (int64_t n = lane * 4; n < V; n += TEAM * 4) {
-    float z[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = 0; p < runs; ++p) {
-      float v[4];
-      load_row<float, 4>(parts + (p * T + t) * V, n, V, v);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * TEAMS + threadIdx.x / TEAM; t < T;
+       t += static_cast<int64_t>(gridDim.x) * TEAMS) {
+    const int64_t y = ldg(o.target + t);
+    float2 a = make_float2(-INFINITY, 0.f);
+    float at = 0.f;
+    for (int64_t n = lane * 4; n < V; n += TEAM * 4) {
+      float z[4];
+      sum_runs<4>(parts + t * V, T * V, runs, n, V, z);
+      float2 b = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] += v[e];
+      for (int e = 0; e < 4; ++e)
+        if (n + e < V) {
+          b.x = fmaxf(b.x, z[e]);
+          if (n + e == y) at = z[e];
+        }
+      const float base = b.x == -INFINITY ? 0.f : b.x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < V) b.y += expf(z[e] - base);
+      a = StatsEpi::join_stats(a, b);
     }
-    float2 b = make_float2(-INFINITY, 0.f);
+    float top = a.x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < V) {
-        b.x = fmaxf(b.x, z[e]);
-        if (n + e == y) at = z[e];
-      }
-    const float base = b.x == -INFINITY ? 0.f : b.x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < V) b.y += expf(z[e] - base);
-    a = StatsEpi::join_stats(a, b);
+    for (int h = 32; h > 0; h >>= 1) top = fmaxf(top, __shfl_xor(top, h, 64));
+    a = make_float2(top, wave_sum(a.y * expf(a.x - (top == -INFINITY ? 0.f : top))));
+    at = wave_sum(at);
+    if constexpr (TEAM > 64) {  // the whole block is on this token
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) stats[threadIdx.x / 64] = a, found[threadIdx.x / 64] = at;
+      __syncthreads();
+      a = stats[0], at = found[0];
+      for (int w = 1; w < TEAM / 64; ++w) a = StatsEpi::join_stats(a, stats[w]), at += found[w];
+    }
+    if (lane == 0) {
+      lse[t] = a.x + logf(a.y);
+      const float l = y == o.ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at - a.x);
+      if (alone) losses[t] = l;
+      else row_loss[t] = l;
+    }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) a = StatsEpi::join_stats(a, make_float2(__shfl_xor(a.x, o, 64), __shfl_xor(a.y, o, 64)));
-  at = wave_sum(at);
-  if constexpr (TEAM > 64) {
-    if ((threadIdx.x & 63) == 0) stats[threadIdx.x / 64] = a, found[threadIdx.x / 64] = at;
+  if (alone) {
     __syncthreads();
-    a = stats[0], at = found[0];
-    for (int w = 1; w < TEAM / 64; ++w) a = StatsEpi::join_stats(a, stats[w]), at += found[w];
+    ce_loss_of(losses, o);
   }
-  if (lane) return;
-  lse[t] = a.x + logf(a.y);
-  row_loss[t] = y == ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at - a.x);
 }
 
 // d of the logits in k-runs, over the first run.
@@ -289,14 +314,8 @@ __global__ __launch_bounds__(kBlock) void ce_grad_kernel(float* parts, int runs,
     const int64_t t = i / per_row, n = (i - t * per_row) * 4;
     const int64_t y = ldg(target + t);
     const float l = y >= 0 && y < V ? ldg(lse + t) : NAN;
-    float z[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int p = 0; p < runs; ++p) {
-      float v[4];
-      load_row<float, 4>(parts + (p * T + t) * V, n, V, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] += v[e];
-    }
+    float z[4];
+    sum_runs<4>(parts + t * V, T * V, runs, n, V, z);
 #pragma unroll
     for (int e = 0; e < 4; ++e) z[e] = y == ignore ? 0.f : expf(z[e] - l) - (n + e == y ? 1.f : 0.f);
     store_row<float, 4>(parts + t * V, n, V, z);
@@ -395,6 +414,10 @@ static int32_t ce_operands(const p2p_linear_ce_t& a, const CeSpace& s, int64_t v
   return pack_matrices(jobs, v0 ? 1 : 2, a.dtype, st);
 }
 
+static LossOut ce_out(const p2p_linear_ce_t& a) {
+  return LossOut{a.target, a.tokens, a.ignore_index, a.mean, a.loss, a.norm};
+}
+
 static int32_t ce_direct_logits(const p2p_linear_ce_t& a, const CeSpace& s, int* runs, hipStream_t st) {
   *runs = direct_split(a.tokens, a.vocab, a.hidden);
   const float *x = static_cast<const float*>(a.x), *w = static_cast<const float*>(a.w);
@@ -408,14 +431,13 @@ static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStre
   int32_t rc = ce_direct_logits(a, s, &runs, st);
   if (rc != P2P_OK) return rc;
   const float* z = reinterpret_cast<const float*>(s.d);
-  if (a.vocab <= 1024)
-    ce_row_kernel<64><<<dim3(static_cast<unsigned>(ceil_div(a.tokens, 4))), dim3(256), 0, st>>>(
-        z, runs, a.tokens, a.vocab, a.target, a.ignore_index, a.lse, s.row_loss);
-  else
-    ce_row_kernel<1024><<<dim3(static_cast<unsigned>(a.tokens)), dim3(1024), 0, st>>>(
-        z, runs, a.tokens, a.vocab, a.target, a.ignore_index, a.lse, s.row_loss);
-  if ((rc = launch_status()) != P2P_OK) return rc;
-  ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, a.target, a.tokens, a.ignore_index, a.mean, a.loss, a.norm);
+  // a token per wave, up to 64 tokens in one block (which saves the launch of the sum); long rows a block each
+  const bool waves = a.vocab <= 1024;
+  const int64_t blocks = waves ? (a.tokens <= 64 ? 1 : ceil_div(a.tokens, 16)) : a.tokens;
+  const auto kernel = waves ? ce_row_kernel<64> : ce_row_kernel<1024>;
+  kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, st>>>(z, runs, a.vocab, a.lse, s.row_loss, ce_out(a));
+  if ((rc = launch_status()) != P2P_OK || (blocks == 1 && a.tokens <= 64)) return rc;
+  ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, ce_out(a));
   return launch_status();
 }
 
@@ -469,7 +491,7 @@ extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, 
   if (!aligned_to(a->loss, 4)) return P2P_ERR_ALIGN;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->tokens == 0) {  // the empty sum
-    ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(nullptr, nullptr, 0, a->ignore_index, a->mean, a->loss, a->norm);
+    ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(nullptr, ce_out(*a));
     return launch_status();
   }
   CeSpace s;
@@ -490,11 +512,11 @@ extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, 
     if ((rc = gemm_launch<false, false, false>(g, a->dtype == P2P_DTYPE_F16, big, e, st)) != P2P_OK) return rc;
     const int tiles = static_cast<int>(ceil_div(rows, big ? Big::BN : Small::BN));
     ce_join_kernel<<<dim3(static_cast<unsigned>(ceil_div(a->tokens, 64))), dim3(1024), 0, st>>>(
-        s.part, tiles, a->tokens, s.state, v0 == 0, v0 + rows == a->vocab, a->target, a->vocab, a->ignore_index, s.at_target,
-        a->lse, s.row_loss);
+        s.part, tiles, s.state, v0 == 0, v0 + rows == a->vocab, a->vocab, s.at_target, a->lse, s.row_loss, ce_out(*a));
     if ((rc = launch_status()) != P2P_OK) return rc;
   }
-  ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, a->target, a->tokens, a->ignore_index, a->mean, a->loss, a->norm);
+  if (a->tokens <= 64) return P2P_OK;  // the join's one block has summed the losses
+  ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, ce_out(*a));
   return launch_status();
 }
 

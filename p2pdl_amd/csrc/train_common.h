@@ -116,6 +116,37 @@ __device__ __forceinline__ void store_row(T* row, int64_t c, int64_t cols, const
   }
 }
 
+// s[e] = p[c + e] + p[stride + c + e] + ... over `runs`, in that order; elements at and past `cols` are 0.  Loads
+// go out eight runs at a time, the last ones again in place of what is past them: a loop over a
+// remainder would wait for each.
+template <int N>
+__device__ __forceinline__ void sum_runs(const float* p, int64_t stride, int runs, int64_t c, int64_t cols, float (&s)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) s[e] = 0.f;
+  const bool whole = c + N <= cols;
+  for (int r0 = 0; r0 < runs; r0 += 8) {
+    float v[8][N];
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const Pack<float, N> q = load_pack<float, N>(p + (r0 + u < runs ? r0 + u : runs - 1) * stride + c);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[u][e] = q.v[e];
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          v[u][e] = ldg(p + (r0 + u < runs ? r0 + u : runs - 1) * stride + (c + e < cols ? c + e : cols - 1));
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] += r0 + u < runs && c + e < cols ? v[u][e] : 0.f;
+  }
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
