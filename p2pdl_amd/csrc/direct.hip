@@ -1,4 +1,4 @@
-// The float32 product of direct.h.
+// The product of direct.h.
 //
 // Tile 64 x 64 (32 x 64 for few rows) x 32 in two LDS images of pitch 36
 // floats, on which a fragment's 16 rows of four floats fall on all 64 banks
@@ -18,14 +18,14 @@ using f4 = float __attribute__((ext_vector_type(4)));
 constexpr int kDirectN = 64, kDirectK = 32, kDirectPitch = kDirectK + 4;
 
 // EXT rows of an operand for one k-step: EXT / 8 floats per lane.
-template <bool T, int EXT>
+template <typename E, bool T, int EXT>
 struct DirectLoader {
-  static constexpr int VECS = EXT / 32;  // 4-float vectors per lane
-  const float *p, *p2;
+  static constexpr int VECS = EXT / 32;  // vectors of four elements per lane
+  const E *p, *p2;
   int64_t ld, ld2, lines, rows, K;
   float v[VECS][4];
 
-  __device__ __forceinline__ const float* line(int64_t i) const { return i < lines ? p + i * ld : p2 + (i - lines) * ld2; }
+  __device__ __forceinline__ const E* line(int64_t i) const { return i < lines ? p + i * ld : p2 + (i - lines) * ld2; }
 
   __device__ __forceinline__ void load(int64_t row0, int64_t k0) {
 #pragma unroll
@@ -33,11 +33,11 @@ struct DirectLoader {
       const int q = i * 256 + threadIdx.x;
       if constexpr (!T) {
         const int64_t r = row0 + q / 8;
-        if (r < rows) load_row<float, 4>(line(r), k0 + q % 8 * 4, K, v[i]);
+        if (r < rows) load_row<E, 4>(line(r), k0 + q % 8 * 4, K, v[i]);
         else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
       } else {
         const int64_t k = k0 + q / (EXT / 4);
-        if (k < K) load_row<float, 4>(line(k), row0 + q % (EXT / 4) * 4, rows, v[i]);
+        if (k < K) load_row<E, 4>(line(k), row0 + q % (EXT / 4) * 4, rows, v[i]);
         else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
       }
     }
@@ -57,7 +57,7 @@ struct DirectLoader {
   }
 };
 
-template <bool AT, bool BT, int BM>
+template <typename TA, typename TB, bool AT, bool BT, int BM>
 __global__ __launch_bounds__(256) void direct_kernel(DirectArgs g) {
   constexpr int WM = BM / 32, WN = 4 / WM;                    // waves over the tile
   constexpr int MI = BM / WM / 16, NJ = kDirectN / WN / 16;   // 16 x 16 blocks of a wave
@@ -68,10 +68,10 @@ __global__ __launch_bounds__(256) void direct_kernel(DirectArgs g) {
   const int64_t steps = ceil_div(g.K, kDirectK);
   const int64_t first = steps * blockIdx.y / g.split, last = steps * (blockIdx.y + 1) / g.split;
 
-  DirectLoader<AT, BM> a;
-  DirectLoader<BT, kDirectN> b;
-  a.p = a.p2 = g.a, a.ld = a.ld2 = g.lda, a.lines = INT64_MAX, a.rows = g.M, a.K = g.K;
-  b.p = g.b, b.p2 = g.b2, b.ld = g.ldb, b.ld2 = g.ldb2, b.lines = g.b_rows, b.rows = g.N, b.K = g.K;
+  DirectLoader<TA, AT, BM> a;
+  DirectLoader<TB, BT, kDirectN> b;
+  a.p = a.p2 = static_cast<const TA*>(g.a), a.ld = a.ld2 = g.lda, a.lines = INT64_MAX, a.rows = g.M, a.K = g.K;
+  b.p = static_cast<const TB*>(g.b), b.p2 = static_cast<const TB*>(g.b2), b.ld = g.ldb, b.ld2 = g.ldb2, b.lines = g.b_rows, b.rows = g.N, b.K = g.K;
   f4 acc[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -116,37 +116,46 @@ __global__ __launch_bounds__(256) void direct_kernel(DirectArgs g) {
   for (int i = 0; i < MI; ++i) {
     const int64_t m = m0 + (wm * MI + i) * 16 + (lane & 15);
     if (m >= g.M) continue;
-    float* row = g.partial  ? g.partial + (blockIdx.y * g.M + m) * g.N
-                 : m < g.half ? g.out[0] + m * g.N
-                              : g.out[1] + (m - g.half) * g.N;
+    float* sums = g.partial ? g.partial + (blockIdx.y * g.M + m) * g.N : nullptr;
+    TB* row = m < g.half ? static_cast<TB*>(g.out[0]) + m * g.N : static_cast<TB*>(g.out[1]) + (m - g.half) * g.N;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int64_t n = n0 + (wn * NJ + j) * 16 + (lane >> 4) * 4;
       const float v[4] = {acc[i][j][0] * alpha, acc[i][j][1] * alpha, acc[i][j][2] * alpha, acc[i][j][3] * alpha};
-      if (n < g.N) store_row<float, 4>(row, n, g.N, v);
+      if (n >= g.N) continue;
+      if (sums) store_row<float, 4>(sums, n, g.N, v);
+      else store_row<TB, 4>(row, n, g.N, v);
     }
   }
 }
 
 int direct_split(int64_t M, int64_t N, int64_t K) {
   const int64_t tiles = ceil_div(M, M <= 32 ? 32 : 64) * ceil_div(N, kDirectN), steps = ceil_div(K, kDirectK);
-  return static_cast<int>(std::max<int64_t>(1, std::min({512 / tiles, steps / 2, int64_t(16)})));
+  return static_cast<int>(std::max<int64_t>(1, std::min({512 / tiles, steps / 2, int64_t(32)})));
 }
 
-template <bool AT, bool BT>
+template <typename TA, typename TB, bool AT, bool BT>
 static int32_t direct_run(const DirectArgs& g, hipStream_t st) {
   const bool low = g.M <= 32;
   const int64_t tiles = ceil_div(g.M, low ? 32 : 64) * ceil_div(g.N, kDirectN);
   if (tiles >= (int64_t(1) << 23)) return P2P_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(tiles), g.split);
-  if (low) direct_kernel<AT, BT, 32><<<grid, dim3(256), 0, st>>>(g);
-  else direct_kernel<AT, BT, 64><<<grid, dim3(256), 0, st>>>(g);
+  if (low) direct_kernel<TA, TB, AT, BT, 32><<<grid, dim3(256), 0, st>>>(g);
+  else direct_kernel<TA, TB, AT, BT, 64><<<grid, dim3(256), 0, st>>>(g);
   return launch_status();
 }
 
+// The products used: x W^T, and d (always float) with W or, both row-contiguous, with x.
+template <typename T>
+static int32_t direct_typed(bool at, bool bt, const DirectArgs& g, hipStream_t st) {
+  if (at) return direct_run<float, T, true, true>(g, st);
+  return bt ? direct_run<float, T, false, true>(g, st) : direct_run<T, T, false, false>(g, st);
+}
+
 int32_t direct_product(bool at, bool bt, const DirectArgs& g, hipStream_t st) {
-  if (at) return direct_run<true, true>(g, st);  // the products used: A k-contiguous with either B, both row-contiguous
-  return bt ? direct_run<false, true>(g, st) : direct_run<false, false>(g, st);
+  if (g.a_type != (bt ? P2P_DTYPE_F32 : g.b_type) || (at && !bt)) return P2P_ERR_INVALID;
+  if (g.b_type == P2P_DTYPE_F32) return direct_typed<float>(at, bt, g, st);
+  return g.b_type == P2P_DTYPE_F16 ? direct_typed<f16>(at, bt, g, st) : direct_typed<bf16>(at, bt, g, st);
 }
 
 }  // namespace p2p

@@ -18,7 +18,7 @@
 // three planes), lie side by side in one [T, 2F] buffer, and feed dx as two
 // segments of one sum and dWg, dWu as one product of 2F rows.
 //
-// Small float32 layers take the product of direct.h instead, forward into
+// Small layers take the product of direct.h instead, forward into
 // sums of k-runs that a second kernel joins and activates: @@
 #include "direct.h"
 #include "gemm_tile.h"
@@ -141,7 +141,7 @@ static int32_t gated_grad(const p2p_gated_linear_t& a, int64_t pitch, uint16_t* 
 
 // The direct product's runs [runs][T, 2 units] joined; gate, up and h.
 __global__ __launch_bounds__(kBlock) void gated_join_kernel(const float* parts, int runs, int64_t rows, int64_t units, int act,
-                                                            float* h, float* gate, float* up) {
+                                                            void* h, int32_t dtype, float* gate, float* up) {
   const int64_t per_row = (units + 3) / 4, all = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
        i += static_cast<int64_t>(gridDim.x) * kBlock) {
@@ -156,7 +156,9 @@ __global__ __launch_bounds__(kBlock) void gated_join_kernel(const float* parts, 
       activation(act, g[e], &a, &da);
       o[e] = a * u[e];
     }
-    store_row<float, 4>(h + r * units, c, units, o);
+    if (dtype == P2P_DTYPE_F32) store_row<float, 4>(static_cast<float*>(h) + r * units, c, units, o);
+    else if (dtype == P2P_DTYPE_F16) store_row<f16, 4>(static_cast<f16*>(h) + r * units, c, units, o);
+    else store_row<bf16, 4>(static_cast<bf16*>(h) + r * units, c, units, o);
     if (gate) store_row<float, 4>(gate + r * units, c, units, g);
     if (up) store_row<float, 4>(up + r * units, c, units, u);
   }
@@ -187,7 +189,7 @@ static Plan gated_dw_plan(const p2p_gated_linear_t& a) {
   return gemm_plan(2 * gated_pitch(a), a.hidden, ksteps(a.tokens, a.dtype == P2P_DTYPE_F32 ? 6 : 1), true);
 }
 static bool gated_direct(const p2p_gated_linear_t& a) {
-  return a.dtype == P2P_DTYPE_F32 && direct_pays(a.tokens, 2 * a.units, a.hidden);
+  return direct_pays(a.tokens, 2 * a.units, a.hidden, a.dtype);
 }
 static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* base, GatedSpace* s) {
   Carver c{static_cast<char*>(base)};
@@ -245,38 +247,35 @@ static int32_t gated_operands(const p2p_gated_linear_t& a, const GatedSpace& s, 
 
 static int32_t gated_direct_fwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
   const int split = direct_split(a.tokens, 2 * a.units, a.hidden);
-  const DirectArgs g{static_cast<const float*>(a.x), static_cast<const float*>(a.w_gate), static_cast<const float*>(a.w_up),
-                     a.ldx, a.ldg, a.ldu, a.units, a.tokens, 2 * a.units, a.hidden, split, {nullptr, nullptr}, INT64_MAX,
-                     {nullptr, nullptr}, s.parts};
+  const DirectArgs g{a.x, a.w_gate, a.w_up, a.dtype, a.dtype, a.ldx, a.ldg, a.ldu, a.units, a.tokens, 2 * a.units, a.hidden,
+                     split, {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, s.parts};
   const int32_t rc = direct_product(false, false, g, st);
   if (rc != P2P_OK) return rc;
   const int64_t blocks = ceil_div(a.tokens * ceil_div(a.units, 4), kBlock);
   gated_join_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
-      s.parts, split, a.tokens, a.units, a.activation, static_cast<float*>(a.h), a.gate, a.up);
+      s.parts, split, a.tokens, a.units, a.activation, a.h, a.dtype, a.gate, a.up);
   return launch_status();
 }
 
 static int32_t gated_direct_bwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
   const int64_t rows2 = 2 * a.units;
-  int32_t rc = gated_grad<float, true>(a, a.units, s.d, st);
+  int32_t rc = a.dtype == P2P_DTYPE_F32   ? gated_grad<float, true>(a, a.units, s.d, st)
+               : a.dtype == P2P_DTYPE_F16 ? gated_grad<f16, true>(a, a.units, s.d, st)
+                                          : gated_grad<bf16, true>(a, a.units, s.d, st);
   if (rc != P2P_OK) return rc;
-  const float *d = reinterpret_cast<const float*>(s.d), *x = static_cast<const float*>(a.x);
   {  // dx = [dg du] [Wg; Wu]
     const int split = direct_split(a.tokens, a.hidden, rows2);
-    float* out = static_cast<float*>(a.dx);
-    const DirectArgs g{d, static_cast<const float*>(a.w_gate), static_cast<const float*>(a.w_up), rows2, a.ldg, a.ldu, a.units,
-                       a.tokens, a.hidden, rows2, split, {out, nullptr}, INT64_MAX, {nullptr, nullptr},
-                       split > 1 ? s.parts : nullptr};
+    const DirectArgs g{s.d, a.w_gate, a.w_up, P2P_DTYPE_F32, a.dtype, rows2, a.ldg, a.ldu, a.units, a.tokens, a.hidden, rows2,
+                       split, {a.dx, nullptr}, INT64_MAX, {nullptr, nullptr}, split > 1 ? s.parts : nullptr};
     if ((rc = direct_product(false, true, g, st)) != P2P_OK) return rc;
     const int64_t n = a.tokens * a.hidden;
-    if (split > 1 && (rc = join_parts(s.parts, split, n, n, 0, nullptr, nullptr, 1.f, out, nullptr, a.dtype, st)) != P2P_OK)
+    if (split > 1 && (rc = join_parts(s.parts, split, n, n, 0, nullptr, nullptr, 1.f, a.dx, nullptr, a.dtype, st)) != P2P_OK)
       return rc;
   }
   // [dWg; dWu] = [dg du]^T x
   const int split = direct_split(rows2, a.hidden, a.tokens);
-  const DirectArgs g{d, x, x, rows2, a.ldx, a.ldx, INT64_MAX, rows2, a.hidden, a.tokens, split,
-                     {static_cast<float*>(a.dw_gate), static_cast<float*>(a.dw_up)}, a.units, {nullptr, nullptr},
-                     split > 1 ? s.parts : nullptr};
+  const DirectArgs g{s.d, a.x, a.x, P2P_DTYPE_F32, a.dtype, rows2, a.ldx, a.ldx, INT64_MAX, rows2, a.hidden, a.tokens, split,
+                     {a.dw_gate, a.dw_up}, a.units, {nullptr, nullptr}, split > 1 ? s.parts : nullptr};
   if ((rc = direct_product(true, true, g, st)) != P2P_OK || split == 1) return rc;
   const int64_t n = a.units * a.hidden;
   return join_parts(s.parts, split, 2 * n, n, n, nullptr, nullptr, 1.f, a.dw_gate, a.dw_up, a.dtype, st);

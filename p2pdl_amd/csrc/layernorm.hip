@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
   constexpr int V = Vec16<T>::N;
   constexpr int TEAMS = kLnBwdBlock / TEAM, WAVES = TEAM / 64;
   __shared__ float2 sums[2][kLnBwdBlock / 64];
-  __shared__ float joined[TEAMS > 1 ? TEAM * V : 1];
+  __shared__ float joined[TEAMS > 1 ? kLnBwdBlock * V : 1];
   const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, wave = threadIdx.x / 64;
   float dwv[NV][V], dbv[NV][V];
   Raw wv[NV], xv[NV], gv[NV];
@@ -199,16 +199,15 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
     for (int i = 0; i < NV; ++i) {
       float (&v)[V] = which ? dbv[i] : dwv[i];
       if constexpr (TEAMS > 1) {
-        for (int t = 1; t < TEAMS; ++t) {
-          __syncthreads();
-          if (team == t)
+        __syncthreads();
 #pragma unroll
-            for (int e = 0; e < V; ++e) joined[e * TEAM + lane] = v[e];
-          __syncthreads();
-          if (team == 0)
+        for (int e = 0; e < V; ++e) joined[e * kLnBwdBlock + threadIdx.x] = v[e];
+        __syncthreads();
+        if (team == 0)
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] += joined[e * TEAM + lane];
-        }
+          for (int e = 0; e < V; ++e)
+#pragma unroll
+            for (int t = 1; t < TEAMS; ++t) v[e] += joined[e * kLnBwdBlock + t * TEAM + lane];
       }
       const int c = (i * TEAM + lane) * V;
       if (team == 0 && c < cols) {

@@ -23,7 +23,7 @@
 // are applied to the 32-bit sums.  A target outside [0, V) that is not
 // ignore_index makes the loss and both gradients NaN and reads nothing.
 //
-// Small float32 heads take the product of direct.h, whose k-runs are joined by
+// Small heads take the product of direct.h, whose k-runs are joined by
 // the kernel that reduces a token's row (forward) or makes d of it: @@
 #include "direct.h"
 #include "gemm_tile.h"
@@ -355,7 +355,7 @@ static Plan ce_dw_plan(const p2p_linear_ce_t& a, int64_t rows) {
 }
 
 static bool ce_direct(const p2p_linear_ce_t& a) {
-  return a.dtype == P2P_DTYPE_F32 && direct_pays(a.tokens, a.vocab, a.hidden) && a.tokens * a.vocab * 4 <= kPieceBytes;
+  return direct_pays(a.tokens, a.vocab, a.hidden, a.dtype) && a.tokens * a.vocab * 4 <= kPieceBytes;
 }
 static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeSpace* s) {
   Carver c{static_cast<char*>(base)};
@@ -420,9 +420,8 @@ static LossOut ce_out(const p2p_linear_ce_t& a) {
 
 static int32_t ce_direct_logits(const p2p_linear_ce_t& a, const CeSpace& s, int* runs, hipStream_t st) {
   *runs = direct_split(a.tokens, a.vocab, a.hidden);
-  const float *x = static_cast<const float*>(a.x), *w = static_cast<const float*>(a.w);
-  const DirectArgs g{x, w, w, a.ldx, a.ldw, a.ldw, INT64_MAX, a.tokens, a.vocab, a.hidden, *runs, {nullptr, nullptr}, INT64_MAX,
-                     {nullptr, nullptr}, reinterpret_cast<float*>(s.d)};
+  const DirectArgs g{a.x, a.w, a.w, a.dtype, a.dtype, a.ldx, a.ldw, a.ldw, INT64_MAX, a.tokens, a.vocab, a.hidden, *runs,
+                     {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, reinterpret_cast<float*>(s.d)};
   return direct_product(false, false, g, st);
 }
 
@@ -450,20 +449,19 @@ static int32_t ce_direct_bwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStre
   ce_grad_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
       d, runs, a.tokens, a.vocab, a.lse, a.target, a.ignore_index);
   if ((rc = launch_status()) != P2P_OK) return rc;
-  const float *x = static_cast<const float*>(a.x), *w = static_cast<const float*>(a.w);
   struct Side {
     bool at;
-    const float* b;
+    const void* b;
     int64_t ldb, M, K;
     void* out;
     float* parts;
   };
   // dx = d W, then dW = d^T x
-  for (const Side& e : {Side{false, w, a.ldw, a.tokens, a.vocab, a.dx, s.dx_parts},
-                        Side{true, x, a.ldx, a.vocab, a.tokens, a.dw, s.dw_parts}}) {
+  for (const Side& e : {Side{false, a.w, a.ldw, a.tokens, a.vocab, a.dx, s.dx_parts},
+                        Side{true, a.x, a.ldx, a.vocab, a.tokens, a.dw, s.dw_parts}}) {
     const int split = direct_split(e.M, a.hidden, e.K);
-    const DirectArgs g{d, e.b, e.b, a.vocab, e.ldb, e.ldb, INT64_MAX, e.M, a.hidden, e.K, split,
-                       {static_cast<float*>(e.out), nullptr}, INT64_MAX, {a.norm, a.dloss}, split > 1 ? e.parts : nullptr};
+    const DirectArgs g{d, e.b, e.b, P2P_DTYPE_F32, a.dtype, a.vocab, e.ldb, e.ldb, INT64_MAX, e.M, a.hidden, e.K, split,
+                       {e.out, nullptr}, INT64_MAX, {a.norm, a.dloss}, split > 1 ? e.parts : nullptr};
     if ((rc = direct_product(e.at, true, g, st)) != P2P_OK) return rc;
     const int64_t n = e.M * a.hidden;
     if (split > 1 && (rc = join_parts(e.parts, split, n, n, 0, a.norm, a.dloss, 1.f, e.out, nullptr, a.dtype, st)) != P2P_OK)

@@ -133,11 +133,12 @@ def test_gated_linear_arguments_without_gpu():
     assert L.p2p_gated_linear_bwd(gated_args(gate=None), ok, big, None) == -1
     assert L.p2p_gated_linear_bwd(gated_args(lddh=31), ok, big, None) == -1
     assert L.p2p_gated_linear_bwd(gated_args(dw_up=None), ok, big, None) == -1
-    # aligned 16-bit operands are read in place; float32 and odd ones need their copies
-    assert L.p2p_gated_linear_workspace(gated_args(), 0) == 0
-    assert L.p2p_gated_linear_workspace(gated_args(dtype=0, tokens=1 << 20), 0) >= 3 * 2 * 64 * ((1 << 20) + 32 + 32)
-    assert 0 < L.p2p_gated_linear_workspace(gated_args(dtype=0), 0) < 1 << 20  # few float32 tokens: no copies
-    assert L.p2p_gated_linear_workspace(gated_args(x=ok + 2), 0) >= 2 * 64 * 4
+    # many tokens: aligned 16-bit operands are read in place; float32 and odd ones need their copies
+    many = 1 << 20
+    assert L.p2p_gated_linear_workspace(gated_args(tokens=many), 0) == 0
+    assert L.p2p_gated_linear_workspace(gated_args(dtype=0, tokens=many), 0) >= 3 * 2 * 64 * (many + 32 + 32)
+    assert L.p2p_gated_linear_workspace(gated_args(x=ok + 2, tokens=many), 0) >= 2 * 64 * many
+    assert 0 < L.p2p_gated_linear_workspace(gated_args(dtype=0), 0) < 1 << 20  # few tokens: no copies
     need = L.p2p_gated_linear_workspace(gated_args(), 1)
     assert need >= 4 * 64 * 2
     assert L.p2p_gated_linear_bwd(gated_args(), ok, need - 1, None) == -1
