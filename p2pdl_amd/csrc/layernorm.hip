@@ -25,6 +25,28 @@ constexpr int kLnBwdBlock = 512;
 constexpr int kLnAlone = 8;  // passes over its rows that one block makes alone
 constexpr int kLnMaxParts = 512;  // partial rows of dw / db: two blocks of 512 lanes per CU
 
+// How a row's 16-byte vectors fit it.  DENSE: its length is a multiple of them.
+// SHIFTED: the last one is moved back to the row's end, over elements of the
+// one before, which count once in the sums and are computed and stored
+// twice, alike (a tail of single elements costs its wave a load and a store
+// each: 4099 x 1001 float16 takes 23.3 us a pass with it, 21.1 us so).  SHORT: rows of less
+// than one vector, element by element.
+enum Fit { SHORT, DENSE, SHIFTED };
+template <typename T, Fit FIT>
+struct Span {
+  int c, at;  // first element that counts, first element
+  bool in;
+  __device__ __forceinline__ Span(int vec, int cols) {
+    constexpr int V = Vec16<T>::N;
+    c = vec * V;
+    in = c < cols;
+    at = FIT == SHIFTED && c + V > cols ? cols - V : c;
+  }
+  __device__ __forceinline__ bool counts(int e, int cols) const {
+    return FIT == DENSE ? in : FIT == SHIFTED ? in && at + e >= c : c + e < cols;
+  }
+};
+
 // Sum over a team of TEAM lanes (one wave, or several through LDS: then every
 // lane of the block must call it).
 template <int TEAM, int BLOCK>
@@ -43,7 +65,7 @@ __device__ __forceinline__ float team_sum(float v, float* scratch) {
   return v;
 }
 
-template <typename T, int TEAM, int NV>
+template <typename T, int TEAM, int NV, Fit FIT>
 __global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layernorm_fwd_kernel(
     const T* x, int64_t ldx, const T* w, const T* b, int64_t rows, int cols, float eps, T* y, float* mean_out,
     float* rstd_out) {
@@ -58,34 +80,39 @@ __global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layer
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_row<T, V>(xr, (i * TEAM + lane) * V, have, v[i]);
+    const Span<T, FIT> p(i * TEAM + lane, have);
+    const Raw r = p.in ? load_raw<T, FIT != SHORT>(xr, p.at, have) : Raw{{0u, 0u, 0u, 0u}};
 #pragma unroll
-    for (int e = 0; e < V; ++e) s += v[i][e];
+    for (int e = 0; e < V; ++e) {
+      v[i][e] = raw_at<T>(r, e);
+      s += p.counts(e, have) ? v[i][e] : 0.f;
+    }
   }
   const float mean = team_sum<TEAM, BLOCK>(s, scratch) / static_cast<float>(cols);
   s = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const Span<T, FIT> p(i * TEAM + lane, have);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float d = (i * TEAM + lane) * V + e < have ? v[i][e] - mean : 0.f;
-      v[i][e] = d;
-      s += d * d;
+      v[i][e] -= mean;
+      s += p.counts(e, have) ? v[i][e] * v[i][e] : 0.f;
     }
+  }
   const float rstd = 1.f / sqrtf(team_sum<TEAM, BLOCK>(s, scratch) / static_cast<float>(cols) + eps);
   if (row >= rows) return;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * TEAM + lane) * V;
-    if (c >= cols) continue;
+    const Span<T, FIT> p(i * TEAM + lane, cols);
+    if (!p.in) continue;
     float wv[V], bv[V], o[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) wv[e] = 1.f, bv[e] = 0.f;
-    if (w) load_row<T, V>(w, c, cols, wv);
-    if (b) load_row<T, V>(b, c, cols, bv);
+    if (w) load_row<T, V>(w, p.at, cols, wv);
+    if (b) load_row<T, V>(b, p.at, cols, bv);
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = v[i][e] * rstd * wv[e] + bv[e];
-    store_row<T, V>(y + row * cols, c, cols, o);
+    store_row<T, V, FIT != SHORT>(y + row * cols, p.at, cols, o);
   }
   if (lane == 0) {
     mean_out[row] = mean;
@@ -98,7 +125,7 @@ __global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layer
 // before this one is worked on (rows of up to 4096) and rows are held as they
 // lie, two registers per four 16-bit elements, so that two blocks fit a CU:
 // 16384 x 4096 bf16 in 143.6 us without either, 91 us (4.4 TB/s) with.
-template <typename T, int TEAM, int NV, bool DENSE>
+template <typename T, int TEAM, int NV, Fit FIT>
 __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void layernorm_bwd_kernel(
     const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, const float* mean_in, const float* rstd_in, int64_t rows,
     int cols, T* dx, float* parts, T* dw, T* db) {
@@ -113,7 +140,9 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
   for (int i = 0; i < NV; ++i) {
 #pragma unroll
     for (int e = 0; e < V; ++e) dwv[i][e] = 0.f, dbv[i][e] = 0.f;
-    if (w) wv[i] = load_raw<T, DENSE>(w, (i * TEAM + lane) * V, cols);
+    const Span<T, FIT> p(i * TEAM + lane, cols);
+    if (w && p.in) wv[i] = load_raw<T, FIT != SHORT>(w, p.at, cols);
+    else wv[i] = Raw{{0u, 0u, 0u, 0u}};
   }
   const float inv = 1.f / static_cast<float>(cols);
   const int64_t step = static_cast<int64_t>(gridDim.x) * TEAMS;
@@ -125,9 +154,12 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
     rstd = have ? ldg(rstd_in + r) : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TEAM + lane) * V;
-      xv[i] = load_raw<T, DENSE>(x + r * ldx, c, have);
-      gv[i] = load_raw<T, DENSE>(dy + r * lddy, c, have);
+      const Span<T, FIT> p(i * TEAM + lane, have);
+      xv[i] = gv[i] = Raw{{0u, 0u, 0u, 0u}};
+      if (p.in) {
+        xv[i] = load_raw<T, FIT != SHORT>(x + r * ldx, p.at, have);
+        gv[i] = load_raw<T, FIT != SHORT>(dy + r * lddy, p.at, have);
+      }
     }
   };
   constexpr bool AHEAD = NV * V <= 8;
@@ -144,14 +176,17 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const Span<T, FIT> p(i * TEAM + lane, have);
       forget(wv[i]);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float h = (DENSE ? (i * TEAM + lane) * V : (i * TEAM + lane) * V + e) < have ? (raw_at<T>(xc[i], e) - mu) * rs : 0.f;
+        // past the row dy is 0, and what it adds to sums with it
+        const float h = (raw_at<T>(xc[i], e) - mu) * rs;
         const float d = raw_at<T>(gc[i], e);
-        const float g = w ? d * raw_at<T>(wv[i], e) : d;
+        float g = w ? d * raw_at<T>(wv[i], e) : d;
         dwv[i][e] += d * h;
         dbv[i][e] += d;
+        if (FIT == SHIFTED) g = p.counts(e, have) ? g : 0.f;
         s1 += g;
         s2 += g * h;
       }
@@ -178,7 +213,7 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
     if (have) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * TEAM + lane) * V;
+        const Span<T, FIT> p(i * TEAM + lane, cols);
         float o[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -186,7 +221,7 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
           const float d = raw_at<T>(gc[i], e);
           o[e] = rs * ((w ? d * raw_at<T>(wv[i], e) : d) - s1 - h * s2);
         }
-        if (c < cols) store_row<T, V, DENSE>(dx + row * cols, c, cols, o);
+        if (p.in) store_row<T, V, FIT != SHORT>(dx + row * cols, p.at, cols, o);
       }
     }
   }
@@ -209,11 +244,11 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
 #pragma unroll
             for (int t = 1; t < TEAMS; ++t) v[e] += joined[e * kLnBwdBlock + t * TEAM + lane];
       }
-      const int c = (i * TEAM + lane) * V;
-      if (team == 0 && c < cols) {
+      const Span<T, FIT> p(i * TEAM + lane, cols);
+      if (team == 0 && p.in) {
         T* const whole = which ? db : dw;  // a block alone has the whole sums
-        if (parts) store_row<float, V>(out + which * cols, c, cols, v);
-        else if (whole) store_row<T, V>(whole, c, cols, v);
+        if (parts) store_row<float, V, FIT != SHORT>(out + which * cols, p.at, cols, v);
+        else if (whole) store_row<T, V, FIT != SHORT>(whole, p.at, cols, v);
       }
     }
 }
@@ -296,9 +331,12 @@ static int32_t ln_fwd(const T* x, int64_t ldx, const T* w, const T* b, int64_t r
                       float* mean, float* rstd, hipStream_t st) {
   ln_fwd_team<T>(cols, [&](auto team, auto nv) {
     constexpr int TEAM = decltype(team)::value, BLOCK = kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock;
-    layernorm_fwd_kernel<T, TEAM, decltype(nv)::value>
-        <<<dim3(static_cast<unsigned>(ceil_div(rows, BLOCK / TEAM))), dim3(BLOCK), 0, st>>>(x, ldx, w, b, rows, cols, eps,
-                                                                                           y, mean, rstd);
+    constexpr int NV = decltype(nv)::value, V = Vec16<T>::N;
+    auto kernel = cols % V == 0 ? layernorm_fwd_kernel<T, TEAM, NV, DENSE> : layernorm_fwd_kernel<T, TEAM, NV, SHIFTED>;
+    if constexpr (TEAM == 64)
+      if (cols < V) kernel = layernorm_fwd_kernel<T, TEAM, NV, SHORT>;
+    kernel<<<dim3(static_cast<unsigned>(ceil_div(rows, BLOCK / TEAM))), dim3(BLOCK), 0, st>>>(x, ldx, w, b, rows, cols, eps, y,
+                                                                                            mean, rstd);
   });
   return launch_status();
 }
@@ -311,7 +349,10 @@ static int32_t ln_bwd(const T* dy, int64_t lddy, const T* x, int64_t ldx, const 
   float* const to = (dw || db) && n > 1 ? parts : nullptr;
   ln_team<T>(cols, [&](auto team, auto nv) {
     constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
-    const auto kernel = cols % Vec16<T>::N == 0 ? layernorm_bwd_kernel<T, TEAM, NV, true> : layernorm_bwd_kernel<T, TEAM, NV, false>;
+    constexpr int V = Vec16<T>::N;
+    auto kernel = cols % V == 0 ? layernorm_bwd_kernel<T, TEAM, NV, DENSE> : layernorm_bwd_kernel<T, TEAM, NV, SHIFTED>;
+    if constexpr (TEAM == 64)
+      if (cols < V) kernel = layernorm_bwd_kernel<T, TEAM, NV, SHORT>;
     kernel<<<dim3(n), dim3(kLnBwdBlock), 0, st>>>(dy, lddy, x, ldx, w, mean, rstd, rows, cols, dx, to, dw, db);
   });
   const int32_t rc = launch_status();

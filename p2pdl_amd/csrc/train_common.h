@@ -60,7 +60,7 @@ struct Vec16 {
 struct Raw {
   uint32_t w[4];
 };
-// DENSE: cols is a multiple of the vector.
+// DENSE: the vector lies within the row, or past it whole.
 template <typename T, bool DENSE>
 __device__ __forceinline__ Raw load_raw(const T* row, int64_t c, int64_t cols) {
   constexpr int N = 16 / sizeof(T);
