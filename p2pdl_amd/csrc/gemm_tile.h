@@ -330,18 +330,34 @@ __global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) 
 #pragma unroll
       for (int j = 0; j < BJ; ++j) fb[h][j][half] = rb.read(stage + 2 * Cfg::A_HALF + h * Cfg::B_HALF, wn * Cfg::QN + j * 16, half);
   };
-  const auto mma = [&](int ha, int hb) {
-    
+  const auto mma = [&](int ha, int hb, int half) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int i = 0; i < AI; ++i)
 #pragma unroll
-      for (int i = 0; i < AI; ++i)
-#pragma unroll
-        for (int t = 0; t < BJ; ++t) {
-          const int j = i % 2 ? BJ - 1 - t : t;  // each instruction shares an operand with the last
-          acc[ha * AI + i][hb * BJ + j] = mfma16<F16>(fb[hb][j][half], fa[ha][i][half], acc[ha * AI + i][hb * BJ + j]);
-        }
-    
+      for (int t = 0; t < BJ; ++t) {
+        const int j = i % 2 ? BJ - 1 - t : t;  // each instruction shares an operand with the last
+        acc[ha * AI + i][hb * BJ + j] = mfma16<F16>(fb[hb][j][half], fa[ha][i][half], acc[ha * AI + i][hb * BJ + j]);
+      }
+  };
+  // One phase's work.  A request holds its wave's issue for some hundred
+  // cycles.  Where B is read transposed out of LDS the phase's reads go first
+  // and the request between the products (KM 8192 x 4096 x 32768 1740 -> 1697
+  // us, MM 32768 x 4096 x 8192 1800 -> 1769); where B's k is contiguous the
+  // request goes first (KK 8192 x 32768 x 4096 1883 us, between them 1969).
+  const auto work = [&](auto request, auto read, int ha, int hb) {
+    if constexpr (BT) {
+      read();
+      __builtin_amdgcn_sched_barrier(0);
+      mma(ha, hb, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      request();
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      request();
+      read();
+      mma(ha, hb, 0);
+    }
+    mma(ha, hb, 1);
   };
   // this wave's reads are done, its oldest half has landed; then everyone's
   const auto phase = [&] {
@@ -370,22 +386,14 @@ __global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) 
   issue_a(0, cur);
   for (int s = first; s < last; ++s) {
     phase();
-    issue_b(0, cur);
-    read_b(1, cur);
-    mma(0, 0);
+    work([&] { issue_b(0, cur); }, [&] { read_b(1, cur); }, 0, 0);
     phase();
-    issue_b(1, cur);
-    read_a(1, cur);
-    mma(0, 1);
+    work([&] { issue_b(1, cur); }, [&] { read_a(1, cur); }, 0, 1);
     phase();
-    issue_a(1, cur);
-    read_a(0, nxt);
-    mma(1, 0);
+    work([&] { issue_a(1, cur); }, [&] { read_a(0, nxt); }, 1, 0);
     phase();
     next();
-    issue_a(0, nxt);
-    read_b(0, nxt);
-    mma(1, 1);
+    work([&] { issue_a(0, nxt); }, [&] { read_b(0, nxt); }, 1, 1);
     char* const t = cur;
     cur = nxt;
     nxt = t;
@@ -539,8 +547,9 @@ static inline bool in_place(const void* p, int64_t ld, int64_t cols, int32_t dty
   return dtype != P2P_DTYPE_F32 && aligned_to(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld <= kMaxPitch;
 }
 static inline int64_t round_up(int64_t n, int64_t to) { return ceil_div(n, to) * to; }
-// The pitch of a copy or of d: whole 128-byte lines, on which a tile's rows begin (1023 x 1001 x 32003
-// float16 with pitches of 16 bytes: @@).
+// The pitch of a copy or of d: whole 128-byte lines, on which a tile's rows
+// begin (1023 x 1001 x 32003 float16, forward and backward: 457 us with pitches
+// of 16 bytes, 442 so).
 static inline int64_t line_pitch(int64_t cols) { return round_up(cols, cols > 32 ? 64 : 8); }
 static inline int planes_of(int32_t dtype) { return dtype == P2P_DTYPE_F32 ? 3 : 1; }
 static inline int64_t packed_bytes(int64_t rows, int64_t cols, int32_t dtype) {

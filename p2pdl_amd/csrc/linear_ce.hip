@@ -23,8 +23,9 @@
 // are applied to the 32-bit sums.  A target outside [0, V) that is not
 // ignore_index makes the loss and both gradients NaN and reads nothing.
 //
-// Small heads take the product of direct.h, whose k-runs are joined by
-// the kernel that reduces a token's row (forward) or makes d of it: @@
+// Small heads take the product of direct.h, whose k-runs are joined by the
+// kernel that reduces a token's row (forward) or makes d of it (forward and
+// backward of 32 x 256 x 10 float32 75 -> 41 us, 1 x 512 x 1000 bfloat16 51 -> 31).
 #include "direct.h"
 #include "gemm_tile.h"
 
