@@ -68,12 +68,12 @@ __device__ __forceinline__ float team_sum(float v, float* scratch) {
 template <typename T, int TEAM, int NV, Fit FIT>
 __global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layernorm_fwd_kernel(
     const T* x, int64_t ldx, const T* w, const T* b, int64_t rows, int cols, float eps, T* y, float* mean_out,
-    float* rstd_out) {
+    float* rstd_out, unsigned gx) {
   constexpr int BLOCK = kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock;
   constexpr int V = Vec16<T>::N;
   __shared__ float scratch[BLOCK / 64];
   const int lane = threadIdx.x % TEAM;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (BLOCK / TEAM) + threadIdx.x / TEAM;
+  const int64_t row = tile_id(gx) * (BLOCK / TEAM) + threadIdx.x / TEAM;
   const int have = row < rows ? cols : 0;  // surplus teams of the last block hold an empty row
   const T* xr = x + row * ldx;
   float v[NV][V];
@@ -335,8 +335,8 @@ static int32_t ln_fwd(const T* x, int64_t ldx, const T* w, const T* b, int64_t r
     auto kernel = cols % V == 0 ? layernorm_fwd_kernel<T, TEAM, NV, DENSE> : layernorm_fwd_kernel<T, TEAM, NV, SHIFTED>;
     if constexpr (TEAM == 64)
       if (cols < V) kernel = layernorm_fwd_kernel<T, TEAM, NV, SHORT>;
-    kernel<<<dim3(static_cast<unsigned>(ceil_div(rows, BLOCK / TEAM))), dim3(BLOCK), 0, st>>>(x, ldx, w, b, rows, cols, eps, y,
-                                                                                            mean, rstd);
+    const TileGrid grid = tile_grid(ceil_div(rows, BLOCK / TEAM), BLOCK);
+    kernel<<<dim3(grid.gx, grid.gy), dim3(BLOCK), 0, st>>>(x, ldx, w, b, rows, cols, eps, y, mean, rstd, grid.gx);
   });
   return launch_status();
 }

@@ -311,6 +311,21 @@ def test_layer_norm_many_rows(cuda):
         check(g, v, rounded(v, e, torch.bfloat16), name)
 
 
+@gpu
+def test_layer_norm_rows_past_one_grid_dimension(cuda):
+    """2^26 rows: more work-items than a launch counts in one dimension."""
+    rows, cols = (1 << 26) + 9, 2
+    x = torch.zeros((rows, cols), dtype=torch.float16, device="cuda")
+    tail = randn((700, cols), torch.float16, 15)
+    x[-700:] = tail
+    y, mean, rstd = T.layer_norm_forward(x)
+    want = T.layer_norm_forward(tail)
+    assert all(same_bits(a[-700:], b) for a, b in zip((y, mean, rstd), want))
+    assert not y[:-700].any() and not mean[:-700].any()
+    dx = T.layer_norm_backward(x, x, mean, rstd)[0]
+    assert same_bits(dx[-700:], T.layer_norm_backward(tail, tail, *want[1:])[0]) and not dx[:-700].any()
+
+
 # ------------------------------------------------------------------ dropout
 def philox_words(seed, blocks):
     """Philox4x32-10 in Python integers: the four words of each block."""
