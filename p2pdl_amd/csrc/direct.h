@@ -26,9 +26,11 @@ struct DirectArgs {
 // 2048 x 1024 328 / 327, 2048 x 2048 x 2048 1153 / 673; few rows leave the tiles
 // empty and pay for copies of all of B: 16 x 4096 x 8192 232 / 794.  bfloat16:
 // 1 x 512 x 1000 28 / 35, 256 x 256 x 512 38 / 41, 90 x 512 x 1000 42 / 43, 512 x 256 x
-// 1024 65 / 47 (the loss: 31 / 51, 44 / 55, 49 / 61, 65 / 61).
+// 1024 65 / 47 (the loss: 31 / 51, 44 / 55, 49 / 61, 65 / 61).  Up to 2^24 rows and
+// columns: its 64 x 64 tiles and the rows of its epilogues then fit one dimension of a grid.
 static inline bool direct_pays(int64_t M, int64_t N, int64_t K, int32_t dtype) {
   const double size = static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+  if (M > 1 << 24 || N > 1 << 24) return false;
   return dtype == P2P_DTYPE_F32 ? M <= 128 || size <= 4.0e9 : size <= 6.0e7;
 }
 // Its k-runs: enough blocks for every CU twice, at least two k-steps each.

@@ -152,11 +152,11 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const float* row_loss, Lo
 // block, a wave for every sixteenth of the tiles; one block sums the losses itself.
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int tiles, float2* state, int first, int last,
                                                        int64_t V, const float* at_target, float* lse, float* row_loss,
-                                                       LossOut o) {
+                                                       LossOut o, unsigned gx) {
   const int64_t T = o.T;
   __shared__ float2 groups[16][64];
   const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  const int64_t t = tile_id(gx) * 64 + lane;
   float2 a = make_float2(-INFINITY, 0.f);
   if (t < T) {
     const int from = tiles * group / 16, to = tiles * (group + 1) / 16;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int t
       row_loss[t] = y == o.ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at_target[t] - a.x);
     }
   }
-  if (last && gridDim.x == 1) {
+  if (last && T <= 64) {
     __syncthreads();
     ce_loss_of(row_loss, o);
   }
@@ -510,8 +510,10 @@ extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, 
     const bool big = gemm_plan(g.M, g.N, ksteps(g.K, g.nseg), false).big;
     if ((rc = gemm_launch<false, false, false>(g, a->dtype == P2P_DTYPE_F16, big, e, st)) != P2P_OK) return rc;
     const int tiles = static_cast<int>(ceil_div(rows, big ? Big::BN : Small::BN));
-    ce_join_kernel<<<dim3(static_cast<unsigned>(ceil_div(a->tokens, 64))), dim3(1024), 0, st>>>(
-        s.part, tiles, s.state, v0 == 0, v0 + rows == a->vocab, a->vocab, s.at_target, a->lse, s.row_loss, ce_out(*a));
+    const TileGrid grid = tile_grid(ceil_div(a->tokens, 64), 1024);
+    ce_join_kernel<<<dim3(grid.gx, grid.gy), dim3(1024), 0, st>>>(s.part, tiles, s.state, v0 == 0, v0 + rows == a->vocab,
+                                                                  a->vocab, s.at_target, a->lse, s.row_loss, ce_out(*a),
+                                                                  grid.gx);
     if ((rc = launch_status()) != P2P_OK) return rc;
   }
   if (a->tokens <= 64) return P2P_OK;  // the join's one block has summed the losses

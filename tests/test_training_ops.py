@@ -667,6 +667,23 @@ def test_linear_cross_entropy_pieces(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,rows", [(torch.bfloat16, (1 << 28) + 70), (torch.float32, (1 << 27) + 70)])
+def test_linear_cross_entropy_tokens_past_one_grid_dimension(cuda, dtype, rows):
+    """One feature, two classes: more tokens than a launch has work-items for in one dimension.  With
+    logits 0 and c every token's lse is log(1 + e^c) and its loss lse or lse - c."""
+    c, ones = 0.5, 70
+    x = torch.ones((rows, 1), dtype=dtype, device="cuda")
+    w = torch.tensor([[0.0], [c]], dtype=dtype, device="cuda")
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    t[-ones:] = 1
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t, reduction="sum")
+    want = math.log(1 + math.exp(c))
+    # expf, logf and the sums of two: a few roundings each
+    assert (lse - want).abs().max().item() <= 16 * U * (1 + want)
+    assert abs(loss.item() - (rows * want - ones * c)) <= 16 * U * (1 + want) * rows
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_cross_entropy_targets(cuda, dtype):
     x, w, t = ce_inputs(40, 32, 50, dtype, 60)
