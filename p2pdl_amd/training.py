@@ -423,6 +423,8 @@ def _ce_args(x, weight, target, ignore_index):
         raise ValueError(f"target: expected shape {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
     if x.shape[-1] > MAX_FEATURES:
         raise ValueError(f"at most {MAX_FEATURES} features, got {x.shape[-1]}")
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"ignore_index: expected a 64-bit integer, got {ignore_index}")
     a = N.LinearCeArgs()
     xr, a.ldx = _rows(x)
     wr, a.ldw = _rows(weight)

@@ -801,6 +801,16 @@ def test_refusals(cuda):
             call()
 
 
+@gpu
+def test_linear_cross_entropy_refuses_wide_ignore_index(cuda):
+    """2^64 is not class 0."""
+    x, w, t = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    for index in (1 << 64, 1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="ignore_index"):
+            T.linear_cross_entropy_forward(x, w, t, ignore_index=index)
+    assert T.linear_cross_entropy_forward(x, w, t, ignore_index=-(1 << 63))[0].item() > 1
+
+
 # ------------------------------------------------------------------ graphs, streams, autograd
 def step_calls(dtype, rows=150, cols=264, units=136, vocab=1000):
     x, w, b, dy = randn((rows, cols), dtype, 70), randn((cols,), dtype, 71), randn((cols,), dtype, 72), randn((rows, cols), dtype, 73)
