@@ -284,6 +284,11 @@ int32_t p2p_digest_accept(const uint8_t *digests, const uint8_t *expected,
  * are dense.  A workspace is 16-byte aligned device memory of at least the
  * bytes its query returns for the same arguments (< 0: P2P_ERR_*); it holds
  * nothing between calls, and two calls that may run at once need one each.
+ * K9 and K10 take at most 2^22 - 8 features, 2^21 - 8 units and, as far as
+ * their tiles fit one launch, 2^31 - 256 tokens or classes
+ * (P2P_ERR_UNSUPPORTED past that).  An infinity in a float32 operand of
+ * theirs may come out as NaN: larger float32 products are sums of products of
+ * three 16-bit parts of each operand.
  *
  * K7, layer norm.  y = (x - mean) * rstd * w + b per row, w / b nullable;
  * mean and rstd (float, one per row) feed the backward pass, which writes dx

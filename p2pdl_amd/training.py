@@ -14,7 +14,8 @@ gradient:
 Every operator has a differentiable form (above) and a pair ``*_forward`` /
 ``*_backward`` that a hand-written or captured step calls directly.  Types:
 float32, float16, bfloat16, one per call; sums and statistics are held in 32
-bits, float32 products are float32 products.  No result depends on the order
+bits, float32 products are float32 products (an infinity among their operands
+may come out as NaN: larger ones are sums over 16-bit parts).  No result depends on the order
 of atomics and a dropout mask depends on (seed, offset) alone, so a step run
 again on the same inputs gives the same bits, and a local update the same
 digest.
@@ -22,8 +23,8 @@ digest.
 Tensors are [..., features]; rows may have a pitch (a slice of a wider
 tensor is read in place), other layouts are copied.  Work is launched on the
 current stream of the tensors' device; workspaces come from torch's
-allocator, per call.  A differentiable form refuses to be captured into a
-graph: torch accumulates the gradients of its leaves on the streams of
+allocator, per call.  A differentiable form, and its backward pass, refuses to
+be captured into a graph: torch accumulates the gradients of its leaves on the streams of
 earlier backward passes, which a capture cannot join; a captured step calls
 the ``*_forward`` / ``*_backward`` pairs.
 """
@@ -134,11 +135,15 @@ def _workspace(nbytes: int, dev: torch.device, what: str):
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _no_capture(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing() \
-            and any(t is not None and t.requires_grad for t in tensors):
+def _refuse_capture(what: str) -> None:
+    if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what}: the differentiable form cannot be captured into a graph; "
                            f"call {what}_forward and {what}_backward")
+
+
+def _no_capture(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _refuse_capture(what)
 
 
 # ------------------------------------------------------------------ layer norm
@@ -218,6 +223,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture("layer_norm")
         x, weight, mean, rstd = ctx.saved_tensors
         dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight)
         return dx, dw, db if ctx.has_bias else None, None
@@ -295,6 +301,7 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _refuse_capture("dropout")
         dx = dropout_backward(dy, *ctx.at) if ctx.needs_input_grad[0] else None
         return dx, None, None, None, dy if ctx.needs_input_grad[4] else None
 
@@ -399,6 +406,7 @@ class _GatedLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
+        _refuse_capture("gated_linear")
         x, w_gate, w_up, gate, up = ctx.saved_tensors
         return gated_linear_backward(dh, x, w_gate, w_up, gate, up, ctx.activation) + (None,)
 
@@ -504,6 +512,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
+        _refuse_capture("linear_cross_entropy")
         x, weight, target, lse, norm = ctx.saved_tensors
         return linear_cross_entropy_backward(x, weight, target, lse, norm, dloss, ctx.ignore_index) + (None, None, None)
 

@@ -811,6 +811,97 @@ def test_linear_cross_entropy_refuses_wide_ignore_index(cuda):
     assert T.linear_cross_entropy_forward(x, w, t, ignore_index=-(1 << 63))[0].item() > 1
 
 
+# ------------------------------------------------------------------ offsets past 32 bits
+def device_randn(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, dtype=dtype, device="cuda") * scale).to(dtype)
+
+
+@gpu
+def test_rows_past_32_bits(cuda):
+    """Layer norm and dropout over 2^32 + 2^15 elements: the last rows are those of a call on them alone."""
+    rows, cols, last = (1 << 18) + 2, 1 << 14, 3
+    x = device_randn((rows, cols), torch.bfloat16, 90)
+    w = device_randn((cols,), torch.bfloat16, 91)
+    y, mean, rstd = T.layer_norm_forward(x, w)
+    tail = T.layer_norm_forward(x[-last:], w)
+    assert all(same_bits(a[-last:], b) for a, b in zip((y, mean, rstd), tail))
+    dx = T.layer_norm_backward(y, x, mean, rstd, w)[0]
+    assert same_bits(dx[-last:], T.layer_norm_backward(y[-last:], x[-last:], *tail[1:], w)[0])
+    del dx, y
+    d = T.dropout_forward(x, 0.3, 7, 11)
+    assert same_bits(d[-last:], T.dropout_forward(x[-last:], 0.3, 7, 11 + (rows - last) * cols // 4))
+    assert same_bits(d[:last], T.dropout_forward(x[:last], 0.3, 7, 11))
+
+
+@gpu
+def test_gated_linear_units_past_32_bits(cuda):
+    """tokens x units past 2^31: the last tokens against a call on them alone, the last units' gradients
+    against the sum over all tokens."""
+    rows, cols, units, last = (1 << 17) + 5, 64, 1 << 14, 40
+    x, wg, wu = (device_randn(s, torch.bfloat16, 92 + i, k) for i, (s, k) in enumerate([((rows, cols), 1.0), ((units, cols), 0.12), ((units, cols), 0.12)]))
+    h, gate, up = T.gated_linear_forward(x, wg, wu)
+    g64 = x[-last:].double() @ wg.double().t()
+    u64 = x[-last:].double() @ wu.double().t()
+    mag_g, mag_u = x[-last:].double().abs() @ wg.double().abs().t(), x[-last:].double().abs() @ wu.double().abs().t()
+    # a sum of 64 products each, the additions within an instruction counted as such
+    check(gate[-last:], g64, 2 * cols * U * mag_g, "gate")
+    check(up[-last:], u64, 2 * cols * U * mag_u, "up")
+    dx, dwg, dwu = T.gated_linear_backward(h, x, wg, wu, gate, up)
+    few = slice(units - 2, units)
+    s = torch.sigmoid(gate[:, few].double())
+    act = gate[:, few].double() * s
+    dg = h[:, few].double() * up[:, few].double() * s * (1 + gate[:, few].double() * (1 - s))
+    du = h[:, few].double() * act
+    del gate, up, h
+    for got, d, name in ((dwg, dg, "dw_gate"), (dwu, du, "dw_up")):
+        want, mag = d.t() @ x.double(), d.t().abs() @ x.double().abs()
+        # d is rounded to bf16 once after a few 32-bit operations; the sum over the tokens
+        err = (u(torch.bfloat16) + 64 * U) * mag + rows * U * mag
+        check(got[few], want, rounded(want, err, torch.bfloat16), name)
+
+
+@gpu
+def test_linear_cross_entropy_weight_past_32_bits(cuda):
+    """vocabulary x features past 2^31: logits, loss and gradients of the last classes."""
+    rows, cols, vocab = 24, 1040, (1 << 21) + 3
+    x, w = device_randn((rows, cols), torch.bfloat16, 96), device_randn((vocab, cols), torch.bfloat16, 97, cols ** -0.5)
+    t = vocab - 1 - torch.arange(rows, device="cuda")
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    z = torch.cat([x.double() @ p.double().t() for p in w.split(1 << 18)], 1)
+    mag = torch.cat([x.double().abs() @ p.double().abs().t() for p in w.split(1 << 18)], 1).amax(1)
+    want = torch.logsumexp(z, 1)
+    e_z = 2 * cols * U * mag
+    spread = z.amax(1) - z.amin(1) + 1
+    # as in ce_reference: the logits' error, the sums of exponentials, their rounded arguments, the logarithm
+    err = e_z * 1.01 + (32 + vocab / 64) * U + 8 * U * spread + 4 * U * want.abs() + 8 * U
+    check(lse, want, err, "lse")
+    at = z.gather(1, t[:, None])[:, 0]
+    row = want - at
+    check(loss, row.mean(), (err + e_z + 4 * U * (row.abs() + spread)).mean() + 4 * U * row.mean().abs(), "loss")
+    dx, dw = T.linear_cross_entropy_backward(x, w, t, lse, norm)
+    few = slice(vocab - 8, vocab)
+    logp = z[:, few] - want[:, None]
+    d = logp.exp() - (torch.arange(vocab, device="cuda")[few] == t[:, None]).double()
+    e_d = logp.exp() * ((e_z + err)[:, None] + 4 * U * logp.abs() + 8 * U) * 1.01 + 2 * U * d.abs()
+    e_d = e_d + u(torch.bfloat16) * (d.abs() + e_d) + tiny(torch.bfloat16)  # rounded once as an operand
+    dw_want, m = d.t() @ x.double() / rows, d.t().abs() @ x.double().abs() / rows
+    e = e_d.t() @ x.double().abs() / rows * 1.001 + (2 * rows + 6) * U * m
+    check(dw[few], dw_want, rounded(dw_want, e, torch.bfloat16), "dw")
+    # dx: d of every class times w, in float64 a part of the classes at a time
+    dx_want, e = torch.zeros(rows, cols, dtype=torch.float64, device="cuda"), torch.zeros(rows, cols, dtype=torch.float64, device="cuda")
+    for v0 in range(0, vocab, 1 << 18):
+        part = slice(v0, min(v0 + (1 << 18), vocab))
+        logp = z[:, part] - want[:, None]
+        d = logp.exp() - (torch.arange(vocab, device="cuda")[part] == t[:, None]).double()
+        e_d = logp.exp() * ((e_z + err)[:, None] + 4 * U * logp.abs() + 8 * U) * 1.01 + 2 * U * d.abs()
+        e_d = e_d + u(torch.bfloat16) * (d.abs() + e_d) + tiny(torch.bfloat16)
+        dx_want += d @ w[part].double() / rows
+        # the sum over the classes: tiles of 64 in at most 16 runs and their pieces, no element twice
+        e += (e_d + 2 * vocab * U * d.abs()) @ w[part].double().abs() / rows
+    check(dx, dx_want, rounded(dx_want, e + 6 * U * dx_want.abs(), torch.bfloat16), "dx")
+
+
 # ------------------------------------------------------------------ graphs, streams, autograd
 def step_calls(dtype, rows=150, cols=264, units=136, vocab=1000):
     x, w, b, dy = randn((rows, cols), dtype, 70), randn((cols,), dtype, 71), randn((cols,), dtype, 72), randn((rows, cols), dtype, 73)
@@ -870,6 +961,38 @@ def test_differentiable_forms_refuse_capture(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert keep.item() == 1
+
+
+@gpu
+def test_backward_of_an_eager_forward_refuses_capture(cuda):
+    """A forward pass run eagerly on the capture's stream: its backward pass may not be captured either."""
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    w = torch.zeros(6, 8, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    forms = (lambda x: T.layer_norm(x), lambda x: T.dropout(x, 0.5, 1), lambda x: T.gated_linear(x, w, w),
+             lambda x: T.linear_cross_entropy(x, w, t))
+    with torch.cuda.stream(side):
+        keep = torch.zeros(1, device="cuda")
+        leaves = [torch.zeros(4, 8, device="cuda", requires_grad=True) for _ in forms]
+        outs = [form(x) for form, x in zip(forms, leaves)]
+        dys = [torch.ones_like(o) for o in outs]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        keep.add_(1)
+        for out, dy in zip(outs, dys):
+            with pytest.raises(RuntimeError, match="captured"):
+                out.backward(dy, retain_graph=True)
+    assert all(x.grad is None for x in leaves)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert keep.item() == 1
+    with torch.cuda.stream(side):  # outside the capture the same passes run
+        for out, dy in zip(outs, dys):
+            out.backward(dy)
+    torch.cuda.synchronize()
+    assert all(x.grad is not None for x in leaves)
 
 
 @gpu
