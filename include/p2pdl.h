@@ -282,7 +282,7 @@ int32_t p2p_digest_accept(const uint8_t *digests, const uint8_t *expected,
  * call gives the same bits.  Tensors need the alignment of their elements
  * only; an `ld` is a row pitch in elements (>= the row's length), outputs
  * are dense.  A workspace is 16-byte aligned device memory of at least the
- * bytes its query returns for the same arguments (< 0: P2P_ERR_*); it holds
+ * bytes its query returns for the same arguments (0: none, < 0: P2P_ERR_*); it holds
  * nothing between calls, and two calls that may run at once need one each.
  * K9 and K10 take at most 2^22 - 8 features, 2^21 - 8 units and, as far as
  * their tiles fit one launch, 2^31 - 256 tokens or classes

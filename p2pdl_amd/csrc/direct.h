@@ -9,7 +9,6 @@ namespace p2p {
 
 struct DirectArgs {
   const void *a, *b, *b2;
-  int32_t a_type, b_type;  // of the operands; b_type also of out
   int64_t lda, ldb, ldb2;
   int64_t b_rows;  // lines of b; the further ones are b2's (INT64_MAX: b alone)
   int64_t M, N, K;
@@ -20,23 +19,31 @@ struct DirectArgs {
   float* partial;
 };
 
-// Whether a product of this size goes this way.  Forward and backward of the
-// gated layer, direct / tiles, us.  Float32 (three planes in tiles): 32 x 512 x
-// 512 46 / 82, 512 x 1024 x 1024 118 / 171, 1024 x 1024 x 1024 198 / 204, 1024 x
-// 2048 x 1024 328 / 327, 2048 x 2048 x 2048 1153 / 673; few rows leave the tiles
-// empty and pay for copies of all of B: 16 x 4096 x 8192 232 / 794.  bfloat16:
-// 1 x 512 x 1000 28 / 35, 256 x 256 x 512 38 / 41, 90 x 512 x 1000 42 / 43, 512 x 256 x
-// 1024 65 / 47 (the loss: 31 / 51, 44 / 55, 49 / 61, 65 / 61).  Up to 2^24 rows and
-// columns: its 64 x 64 tiles and the rows of its epilogues then fit one dimension of a grid.
+// Whether a product of this size (N of the gated layer: 2 units) goes this
+// way.  Forward and backward together, direct / tiles, us.  Gated layer,
+// float32 (three planes in tiles): 1024 x 1024 x 512 103 / 168, 800 x 1024 x 1024
+// 160 / 186, 1024 x 1024 x 1024 174 / 200, 1024 x 1024 x 2048 341 / 244; bfloat16:
+// 256 x 256 x 512 32 / 41, 90 x 512 x 1000 36 / 42, 128 x 512 x 1000 46 / 43, 512 x
+// 256 x 1024 53 / 46.  Loss, float32: 1024 x 1024 x 1024 136 / 246, 1024 x 1024 x
+// 2048 239 / 271, 1500 x 1500 x 1500 448 / 349; bfloat16: 128 x 512 x 1000 49 / 61,
+// 200 x 512 x 1000 61 / 62, 512 x 256 x 1024 61 / 61.  Few rows leave the tiles empty
+// and float32 pays for copies of all of B: 16 x 4096 x 8192 232 / 794.  Up to 2^24
+// rows and columns: its tiles and the rows of its epilogues then fit one
+// dimension of a grid.
 static inline bool direct_pays(int64_t M, int64_t N, int64_t K, int32_t dtype) {
   const double size = static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
   if (M > 1 << 24 || N > 1 << 24) return false;
-  return dtype == P2P_DTYPE_F32 ? M <= 128 || size <= 4.0e9 : size <= 6.0e7;
+  return dtype == P2P_DTYPE_F32 ? M <= 128 || size <= 2.6e9 : size <= 1.0e8;
 }
-// Its k-runs: enough blocks for every CU twice, at least two k-steps each.
-P2P_INTERNAL int direct_split(int64_t M, int64_t N, int64_t K);
+// Its k-runs: enough blocks for every CU twice, at least two k-steps each, at
+// most `most`.  Forward as many as a lane's loads take at once (sum_runs):
+// 32 x 784 x 10 float32 19.1 us with up to 32 runs, 15.0 with 8, 16.9 with 4;
+// 8 x 2048 x 1000 23.2, 16.3, 20.5.  The gradients' long sums more: 64 x 512 x
+// 32000 backward 96 us with 32, 195 with 8.
+constexpr int kForwardRuns = 8, kGradRuns = 32;
+P2P_INTERNAL int direct_split(int64_t M, int64_t N, int64_t K, int most);
 
-// AT / BT: the operand's lines are k (row-contiguous), else rows (k-contiguous).
-P2P_INTERNAL int32_t direct_product(bool at, bool bt, const DirectArgs& g, hipStream_t st);
+// A B^T, both operands' lines their rows, of one type.
+P2P_INTERNAL int32_t direct_product(const DirectArgs& g, int32_t dtype, hipStream_t st);
 
 }  // namespace p2p

@@ -20,9 +20,9 @@
 //
 // Small layers take the product of direct.h instead, forward into
 // sums of k-runs that a second kernel joins and activates (forward and
-// backward of 32 x 512 x 512 float32 82 -> 46 us, 1 x 512 x 1000 bfloat16 35 ->
-// 28; direct.h has the sizes on both sides of the rule).
-#include "direct.h"
+// backward of 32 x 512 x 512 float32 82 us on tiles, 21 so; 1 x 512 x 1000
+// bfloat16 35, 22; direct.h has the sizes on both sides of the rule).
+#include "direct_tile.h"
 #include "gemm_tile.h"
 
 namespace p2p {
@@ -182,6 +182,7 @@ static int32_t gated_check(const p2p_gated_linear_t* a) {
 struct GatedSpace {
   uint16_t *x, *wg, *wu, *d;
   float* parts;
+  float* dx_parts;  // of direct.h's product, whose gradients are made side by side
 };
 static int64_t gated_pitch(const p2p_gated_linear_t& a) { return line_pitch(a.units); }
 static Plan gated_dx_plan(const p2p_gated_linear_t& a) {
@@ -193,6 +194,13 @@ static Plan gated_dw_plan(const p2p_gated_linear_t& a) {
 static bool gated_direct(const p2p_gated_linear_t& a) {
   return direct_pays(a.tokens, 2 * a.units, a.hidden, a.dtype);
 }
+// Whether the direct gradients make d where they read it instead of reading
+// it out of a buffer.  Backward, us, so / out of a buffer: 32 x 256 x 10 float32
+// 7.1 / 11.1, 32 x 784 x 512 11.6 / 14.1, 256 x 256 x 256 16.0 / 17.2, 128 x 256 x
+// 1000 23.0 / 23.2, 512 x 1024 x 1024 102 / 67.
+static bool gated_made_in_place(const p2p_gated_linear_t& a) {
+  return static_cast<double>(a.tokens) * static_cast<double>(2 * a.units) * static_cast<double>(a.hidden) <= 6.0e7;
+}
 static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* base, GatedSpace* s) {
   Carver c{static_cast<char*>(base)};
   if (gated_direct(a)) {
@@ -200,12 +208,12 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
     *s = GatedSpace{};
     int64_t floats = 0;
     if (backward) {
-      s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 4));
-      const int sx = direct_split(a.tokens, a.hidden, rows2), sw = direct_split(rows2, a.hidden, a.tokens);
-      if (sx > 1) floats = sx * a.tokens * a.hidden;
-      if (sw > 1) floats = std::max(floats, sw * rows2 * a.hidden);
+      if (!gated_made_in_place(a)) s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 4));
+      const int sx = direct_split(a.tokens, a.hidden, rows2, kGradRuns), sw = direct_split(rows2, a.hidden, a.tokens, kGradRuns);
+      if (sx > 1) s->dx_parts = static_cast<float*>(c.take(sx * a.tokens * a.hidden * 4));
+      if (sw > 1) floats = sw * rows2 * a.hidden;
     } else {
-      floats = direct_split(a.tokens, 2 * a.units, a.hidden) * a.tokens * 2 * a.units;
+      floats = direct_split(a.tokens, 2 * a.units, a.hidden, kForwardRuns) * a.tokens * 2 * a.units;
     }
     if (floats) s->parts = static_cast<float*>(c.take(floats * 4));
     return c.used;
@@ -223,7 +231,7 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
     s->wu = static_cast<uint16_t*>(c.take(packed_bytes(a.units, a.hidden, a.dtype)));
   }
   s->d = nullptr;
-  s->parts = nullptr;
+  s->parts = s->dx_parts = nullptr;
   if (backward) {
     const int64_t rows2 = 2 * gated_pitch(a);
     s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 2 * planes_of(a.dtype)));
@@ -248,10 +256,10 @@ static int32_t gated_operands(const p2p_gated_linear_t& a, const GatedSpace& s, 
 }
 
 static int32_t gated_direct_fwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
-  const int split = direct_split(a.tokens, 2 * a.units, a.hidden);
-  const DirectArgs g{a.x, a.w_gate, a.w_up, a.dtype, a.dtype, a.ldx, a.ldg, a.ldu, a.units, a.tokens, 2 * a.units, a.hidden,
-                     split, {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, s.parts};
-  const int32_t rc = direct_product(false, false, g, st);
+  const int split = direct_split(a.tokens, 2 * a.units, a.hidden, kForwardRuns);
+  const DirectArgs g{a.x, a.w_gate, a.w_up, a.ldx, a.ldg, a.ldu, a.units, a.tokens, 2 * a.units, a.hidden, split,
+                     {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, s.parts};
+  const int32_t rc = direct_product(g, a.dtype, st);
   if (rc != P2P_OK) return rc;
   const int64_t blocks = ceil_div(a.tokens * ceil_div(a.units, 4), kBlock);
   gated_join_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
@@ -259,28 +267,64 @@ static int32_t gated_direct_fwd(const p2p_gated_linear_t& a, const GatedSpace& s
   return launch_status();
 }
 
-static int32_t gated_direct_bwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
-  const int64_t rows2 = 2 * a.units;
-  int32_t rc = a.dtype == P2P_DTYPE_F32   ? gated_grad<float, true>(a, a.units, s.d, st)
-               : a.dtype == P2P_DTYPE_F16 ? gated_grad<f16, true>(a, a.units, s.d, st)
-                                          : gated_grad<bf16, true>(a, a.units, s.d, st);
-  if (rc != P2P_OK) return rc;
-  {  // dx = [dg du] [Wg; Wu]
-    const int split = direct_split(a.tokens, a.hidden, rows2);
-    const DirectArgs g{s.d, a.w_gate, a.w_up, P2P_DTYPE_F32, a.dtype, rows2, a.ldg, a.ldu, a.units, a.tokens, a.hidden, rows2,
-                       split, {a.dx, nullptr}, INT64_MAX, {nullptr, nullptr}, split > 1 ? s.parts : nullptr};
-    if ((rc = direct_product(false, true, g, st)) != P2P_OK) return rc;
-    const int64_t n = a.tokens * a.hidden;
-    if (split > 1 && (rc = join_parts(s.parts, split, n, n, 0, nullptr, nullptr, 1.f, a.dx, nullptr, a.dtype, st)) != P2P_OK)
-      return rc;
+// [dg du] of a token, made where the gradients' products read it (again for
+// every 64 columns of x, against a launch and a buffer).
+template <typename T>
+struct GatedGrad {
+  const T* dh;
+  int64_t lddh;
+  const float *gate, *up;
+  int64_t units;
+  int act;
+
+  __device__ __forceinline__ float one(float g, float u, float d, bool second) const {
+    float a, da;
+    activation(act, g, &a, &da);
+    return second ? d * a : d * u * da;
   }
-  // [dWg; dWu] = [dg du]^T x
-  const int split = direct_split(rows2, a.hidden, a.tokens);
-  const DirectArgs g{s.d, a.x, a.x, P2P_DTYPE_F32, a.dtype, rows2, a.ldx, a.ldx, INT64_MAX, rows2, a.hidden, a.tokens, split,
-                     {a.dw_gate, a.dw_up}, a.units, {nullptr, nullptr}, split > 1 ? s.parts : nullptr};
-  if ((rc = direct_product(true, true, g, st)) != P2P_OK || split == 1) return rc;
-  const int64_t n = a.units * a.hidden;
-  return join_parts(s.parts, split, 2 * n, n, n, nullptr, nullptr, 1.f, a.dw_gate, a.dw_up, a.dtype, st);
+  __device__ __forceinline__ void read(int64_t t, int64_t c, int64_t cols, float (&v)[4]) const {
+    const float *gr = gate + t * units, *ur = up + t * units;
+    const T* dr = dh + t * lddh;
+    const bool second = c >= units;
+    const int64_t n = second ? c - units : c;
+    if (n + 4 <= units) {
+      float g[4], u[4], d[4];
+      load_row<float, 4>(gr, n, units, g);
+      load_row<float, 4>(ur, n, units, u);
+      load_row<T, 4>(dr, n, units, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = one(g[e], u[e], d[e], second);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // from dg into du, or past both
+        const bool s = c + e >= units;
+        const int64_t m = s ? c + e - units : c + e;
+        v[e] = m < units ? one(ldg(gr + m), ldg(ur + m), static_cast<float>(ldg(dr + m)), s) : 0.f;
+      }
+    }
+  }
+};
+
+template <typename T>
+static int32_t gated_direct_bwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
+  const int64_t rows2 = 2 * a.units, nx = a.tokens * a.hidden, nw = a.units * a.hidden;
+  const int sx = direct_split(a.tokens, a.hidden, rows2, kGradRuns), sw = direct_split(rows2, a.hidden, a.tokens, kGradRuns);
+  // dx = [dg du] [Wg; Wu], [dWg; dWu] = [dg du]^T x
+  const DirectArgs x{nullptr, a.w_gate, a.w_up, 0, a.ldg, a.ldu, a.units, a.tokens, a.hidden, rows2, sx,
+                     {a.dx, nullptr}, INT64_MAX, {nullptr, nullptr}, sx > 1 ? s.dx_parts : nullptr};
+  const DirectArgs w{nullptr, a.x, a.x, 0, a.ldx, a.ldx, INT64_MAX, rows2, a.hidden, a.tokens, sw,
+                     {a.dw_gate, a.dw_up}, a.units, {nullptr, nullptr}, sw > 1 ? s.parts : nullptr};
+  int32_t rc;
+  if (s.d) {
+    if ((rc = gated_grad<T, true>(a, a.units, s.d, st)) != P2P_OK) return rc;
+    const float* d = reinterpret_cast<const float*>(s.d);
+    rc = direct_grads<DirectLines<float>, T>(x, w, {d, d, rows2, rows2, INT64_MAX}, st);
+  } else {
+    rc = direct_grads<GatedGrad<T>, T>(x, w, {static_cast<const T*>(a.dh), a.lddh, a.gate, a.up, a.units, a.activation}, st);
+  }
+  if (rc == P2P_OK && sx > 1) rc = join_parts(s.dx_parts, sx, nx, nx, 0, nullptr, nullptr, 1.f, a.dx, nullptr, a.dtype, st);
+  if (rc == P2P_OK && sw > 1) rc = join_parts(s.parts, sw, 2 * nw, nw, nw, nullptr, nullptr, 1.f, a.dw_gate, a.dw_up, a.dtype, st);
+  return rc;
 }
 
 }  // namespace p2p
@@ -329,11 +373,14 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
     return P2P_ERR_ALIGN;
   GatedSpace s;
   const int64_t need = gated_carve(*a, true, workspace, &s);
-  if (need > workspace_bytes || !workspace) return P2P_ERR_INVALID;
+  if (need > workspace_bytes || (need && !workspace)) return P2P_ERR_INVALID;
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (gated_direct(*a)) return gated_direct_bwd(*a, s, st);
   const bool f16_ = a->dtype == P2P_DTYPE_F16;
+  if (gated_direct(*a))
+    return a->dtype == P2P_DTYPE_F32 ? gated_direct_bwd<float>(*a, s, st)
+           : f16_                    ? gated_direct_bwd<f16>(*a, s, st)
+                                     : gated_direct_bwd<bf16>(*a, s, st);
   Mat x, wg, wu;
   if ((rc = gated_operands(*a, s, &x, &wg, &wu, st)) != P2P_OK) return rc;
   const int64_t pitch = gated_pitch(*a), plane = a->tokens * 2 * pitch;

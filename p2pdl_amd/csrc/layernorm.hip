@@ -397,7 +397,8 @@ extern "C" int32_t p2p_layernorm_fwd(const void* x, int64_t ldx, const void* w, 
 
 extern "C" int64_t p2p_layernorm_bwd_workspace(int64_t rows, int64_t cols, int32_t dtype) {
   if (!known_dtype(dtype) || rows < 0 || cols < 1 || cols > kLnMaxCols) return P2P_ERR_INVALID;
-  return static_cast<int64_t>(ln_parts(rows, static_cast<int>(cols), dtype)) * 2 * cols * 4;
+  const int n = ln_parts(rows, static_cast<int>(cols), dtype);
+  return n > 1 ? static_cast<int64_t>(n) * 2 * cols * 4 : 0;  // a block alone writes dw and db itself
 }
 
 extern "C" int32_t p2p_layernorm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
@@ -411,7 +412,8 @@ extern "C" int32_t p2p_layernorm_bwd(const void* dy, int64_t lddy, const void* x
   if (rows == 0) return P2P_OK;
   if (!mean || !rstd || !dx) return P2P_ERR_INVALID;
   if (dw || db) {
-    if (!workspace || workspace_bytes < p2p_layernorm_bwd_workspace(rows, cols, dtype)) return P2P_ERR_INVALID;
+    const int64_t need = p2p_layernorm_bwd_workspace(rows, cols, dtype);
+    if (workspace_bytes < need || (need && !workspace)) return P2P_ERR_INVALID;
     if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   }
   const int s = dtype_bytes(dtype);

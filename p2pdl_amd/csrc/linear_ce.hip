@@ -25,14 +25,18 @@
 //
 // Small heads take the product of direct.h, whose k-runs are joined by the
 // kernel that reduces a token's row (forward) or makes d of it (forward and
-// backward of 32 x 256 x 10 float32 75 -> 41 us, 1 x 512 x 1000 bfloat16 51 -> 31).
-#include "direct.h"
+// backward of 32 x 256 x 10 float32 75 us on tiles, 20 so; 1 x 512 x 1000
+// bfloat16 51, 26).
+#include <type_traits>
+
+#include "direct_tile.h"
 #include "gemm_tile.h"
 
 namespace p2p {
 
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
 constexpr float kHalfScale = 16384.f;
+constexpr int kAloneTokens = 32, kAloneLogits = 16384;  // tokens and partial logits of one block alone
 
 // Per token and tile of columns: (maximum, sum of exp(z - maximum)).
 struct StatsEpi {
@@ -115,14 +119,17 @@ struct LossOut {
   int mean;
   float *loss, *norm;
 };
-__device__ void ce_loss_of(const float* row_loss, const LossOut& o) {
+// at(t): the token's loss and whether it counts.
+template <typename At>
+__device__ __forceinline__ void ce_loss_of(const At& at, const LossOut& o) {
   __shared__ double sums[16];
   __shared__ int64_t counts[16];
   double s = 0.0;
   int64_t n = 0;
   for (int64_t t = threadIdx.x; t < o.T; t += 1024) {
-    s += static_cast<double>(row_loss[t]);
-    n += o.target[t] != o.ignore;
+    const float2 l = at(t);
+    s += static_cast<double>(l.x);
+    n += l.y != 0.f;
   }
 #pragma unroll
   for (int h = 32; h > 0; h >>= 1) {
@@ -145,7 +152,10 @@ __device__ void ce_loss_of(const float* row_loss, const LossOut& o) {
     *o.norm = static_cast<float>(f);
   }
 }
-__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* row_loss, LossOut o) { ce_loss_of(row_loss, o); }
+__device__ __forceinline__ void ce_loss_of_rows(const float* row_loss, const LossOut& o) {
+  ce_loss_of([&](int64_t t) { return make_float2(row_loss[t], o.target[t] != o.ignore ? 1.f : 0.f); }, o);
+}
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* row_loss, LossOut o) { ce_loss_of_rows(row_loss, o); }
 
 // Joins the column tiles of a piece, and with what earlier pieces left in
 // `state`; after the last piece, lse and the token's loss.  64 tokens per
@@ -180,7 +190,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int t
   }
   if (last && T <= 64) {
     __syncthreads();
-    ce_loss_of(row_loss, o);
+    ce_loss_of_rows(row_loss, o);
   }
 }
 
@@ -250,15 +260,15 @@ struct GradEpi {
 };
 
 // The direct product's logits in k-runs [runs][T, V], a token per TEAM of a block's 1024 lanes: lse and the
-// token's loss.  A block alone with up to 64 tokens sums their losses itself.
+// token's loss.  A block alone with few tokens sums their losses itself.
 template <int TEAM>
 __global__ __launch_bounds__(1024) void ce_row_kernel(const float* parts, int runs, int64_t V, float* lse, float* row_loss,
                                                       LossOut o) {
-  constexpr int TEAMS = 1024 / TEAM;
-  __shared__ float2 stats[16];
-  __shared__ float found[16], losses[64];
+  constexpr int TEAMS = 1024 / TEAM, LANES = TEAM < 64 ? TEAM : 64;
+  __shared__ float2 stats[16], losses[kAloneTokens];
+  __shared__ float found[16];
   const int64_t T = o.T;
-  const bool alone = gridDim.x == 1 && T <= 64;
+  const bool alone = gridDim.x == 1 && T <= kAloneTokens;
   const int lane = threadIdx.x % TEAM;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * TEAMS + threadIdx.x / TEAM; t < T;
        t += static_cast<int64_t>(gridDim.x) * TEAMS) {
@@ -283,9 +293,13 @@ __global__ __launch_bounds__(1024) void ce_row_kernel(const float* parts, int ru
     }
     float top = a.x;
 #pragma unroll
-    for (int h = 32; h > 0; h >>= 1) top = fmaxf(top, __shfl_xor(top, h, 64));
-    a = make_float2(top, wave_sum(a.y * expf(a.x - (top == -INFINITY ? 0.f : top))));
-    at = wave_sum(at);
+    for (int h = LANES / 2; h > 0; h >>= 1) top = fmaxf(top, __shfl_xor(top, h, 64));
+    a = make_float2(top, a.y * expf(a.x - (top == -INFINITY ? 0.f : top)));
+#pragma unroll
+    for (int h = LANES / 2; h > 0; h >>= 1) {
+      a.y += __shfl_xor(a.y, h, 64);
+      at += __shfl_xor(at, h, 64);
+    }
     if constexpr (TEAM > 64) {  // the whole block is on this token
       __syncthreads();
       if ((threadIdx.x & 63) == 0) stats[threadIdx.x / 64] = a, found[threadIdx.x / 64] = at;
@@ -296,13 +310,13 @@ __global__ __launch_bounds__(1024) void ce_row_kernel(const float* parts, int ru
     if (lane == 0) {
       lse[t] = a.x + logf(a.y);
       const float l = y == o.ignore ? 0.f : (y < 0 || y >= V) ? NAN : logf(a.y) - (at - a.x);
-      if (alone) losses[t] = l;
+      if (alone) losses[t] = make_float2(l, y != o.ignore ? 1.f : 0.f);
       else row_loss[t] = l;
     }
   }
   if (alone) {
     __syncthreads();
-    ce_loss_of(losses, o);
+    ce_loss_of([&](int64_t t) { return losses[t]; }, o);
   }
 }
 
@@ -322,6 +336,26 @@ __global__ __launch_bounds__(kBlock) void ce_grad_kernel(float* parts, int runs,
     store_row<float, 4>(parts + t * V, n, V, z);
   }
 }
+
+// The same, made where the gradients' products read it (again for every 64
+// columns of x, against a launch).
+struct CeGrad {
+  const float* parts;
+  int runs;
+  int64_t T, V;
+  const float* lse;
+  const int64_t* target;
+  int64_t ignore;
+
+  __device__ __forceinline__ void read(int64_t t, int64_t n, int64_t cols, float (&v)[4]) const {
+    const int64_t y = ldg(target + t);
+    const float l = y >= 0 && y < V ? ldg(lse + t) : NAN;
+    float z[4];
+    sum_runs<4>(parts + t * V, T * V, runs, n, V, z);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = y == ignore || n + e >= V ? 0.f : expf(z[e] - l) - (n + e == y ? 1.f : 0.f);
+  }
+};
 
 static int32_t ce_check(const p2p_linear_ce_t* a) {
   if (!a || !known_dtype(a->dtype) || a->tokens < 0 || a->hidden < 1 || a->vocab < 1 || a->ldx < a->hidden ||
@@ -358,17 +392,23 @@ static Plan ce_dw_plan(const p2p_linear_ce_t& a, int64_t rows) {
 static bool ce_direct(const p2p_linear_ce_t& a) {
   return direct_pays(a.tokens, a.vocab, a.hidden, a.dtype) && a.tokens * a.vocab * 4 <= kPieceBytes;
 }
+// Whether the direct gradients make d where they read it.  Backward, us, so /
+// out of the logits' buffer: 32 x 256 x 10 float32 9.4 / 12.5, 1 x 512 x 1000
+// bfloat16 13.8 / 14.8, 64 x 256 x 512 float32 17.7 / 17.2, 64 x 512 x 1000 22.0 / 19.7.
+static bool ce_made_in_place(const p2p_linear_ce_t& a) {
+  return static_cast<double>(a.tokens) * static_cast<double>(a.vocab) * static_cast<double>(a.hidden) <= 8.0e6;
+}
 static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeSpace* s) {
   Carver c{static_cast<char*>(base)};
   if (ce_direct(a)) {
     *s = CeSpace{};
-    const int64_t runs = direct_split(a.tokens, a.vocab, a.hidden);
+    const int64_t runs = direct_split(a.tokens, a.vocab, a.hidden, kForwardRuns);
     s->d = static_cast<uint16_t*>(c.take(runs * a.tokens * a.vocab * 4));
     if (!backward) {
       s->row_loss = static_cast<float*>(c.take(a.tokens * 4));
       return c.used;
     }
-    const int64_t sx = direct_split(a.tokens, a.hidden, a.vocab), sw = direct_split(a.vocab, a.hidden, a.tokens);
+    const int64_t sx = direct_split(a.tokens, a.hidden, a.vocab, kGradRuns), sw = direct_split(a.vocab, a.hidden, a.tokens, kGradRuns);
     if (sx > 1) s->dx_parts = static_cast<float*>(c.take(sx * a.tokens * a.hidden * 4));
     if (sw > 1) s->dw_parts = static_cast<float*>(c.take(sw * a.vocab * a.hidden * 4));
     return c.used;
@@ -420,10 +460,10 @@ static LossOut ce_out(const p2p_linear_ce_t& a) {
 }
 
 static int32_t ce_direct_logits(const p2p_linear_ce_t& a, const CeSpace& s, int* runs, hipStream_t st) {
-  *runs = direct_split(a.tokens, a.vocab, a.hidden);
-  const DirectArgs g{a.x, a.w, a.w, a.dtype, a.dtype, a.ldx, a.ldw, a.ldw, INT64_MAX, a.tokens, a.vocab, a.hidden, *runs,
+  *runs = direct_split(a.tokens, a.vocab, a.hidden, kForwardRuns);
+  const DirectArgs g{a.x, a.w, a.w, a.ldx, a.ldw, a.ldw, INT64_MAX, a.tokens, a.vocab, a.hidden, *runs,
                      {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, reinterpret_cast<float*>(s.d)};
-  return direct_product(false, false, g, st);
+  return direct_product(g, a.dtype, st);
 }
 
 static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStream_t st) {
@@ -431,12 +471,15 @@ static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStre
   int32_t rc = ce_direct_logits(a, s, &runs, st);
   if (rc != P2P_OK) return rc;
   const float* z = reinterpret_cast<const float*>(s.d);
-  // a token per wave, up to 64 tokens in one block (which saves the launch of the sum); long rows a block each
-  const bool waves = a.vocab <= 1024;
-  const int64_t blocks = waves ? (a.tokens <= 64 ? 1 : ceil_div(a.tokens, 16)) : a.tokens;
-  const auto kernel = waves ? ce_row_kernel<64> : ce_row_kernel<1024>;
+  // a token per 16 lanes, wave or block by the length of its row; few tokens in one block, which saves the launch
+  // of the sum.  Forward, us: 32 x 784 x 10 float32 15.1 with a wave per token, 10.8 so; 32 x 512 x 512, of 131072
+  // partial logits, 16.1 in one block, 13.3 in two; 64 x 128 x 100 17.5, 12.6.
+  const int team = a.vocab <= 64 ? 16 : a.vocab <= 1024 ? 64 : 1024;
+  const bool alone = a.tokens <= kAloneTokens && runs * a.tokens * a.vocab <= kAloneLogits;
+  const int64_t blocks = alone && team < 1024 ? 1 : ceil_div(a.tokens, 1024 / team);
+  const auto kernel = team == 16 ? ce_row_kernel<16> : team == 64 ? ce_row_kernel<64> : ce_row_kernel<1024>;
   kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, st>>>(z, runs, a.vocab, a.lse, s.row_loss, ce_out(a));
-  if ((rc = launch_status()) != P2P_OK || (blocks == 1 && a.tokens <= 64)) return rc;
+  if ((rc = launch_status()) != P2P_OK || (blocks == 1 && a.tokens <= kAloneTokens)) return rc;
   ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, ce_out(a));
   return launch_status();
 }
@@ -445,30 +488,32 @@ static int32_t ce_direct_bwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStre
   int runs;
   int32_t rc = ce_direct_logits(a, s, &runs, st);
   if (rc != P2P_OK) return rc;
-  float* d = reinterpret_cast<float*>(s.d);
-  const int64_t blocks = ceil_div(a.tokens * ceil_div(a.vocab, 4), kBlock);
-  ce_grad_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
-      d, runs, a.tokens, a.vocab, a.lse, a.target, a.ignore_index);
-  if ((rc = launch_status()) != P2P_OK) return rc;
-  struct Side {
-    bool at;
-    const void* b;
-    int64_t ldb, M, K;
-    void* out;
-    float* parts;
+  const int64_t nx = a.tokens * a.hidden, nw = a.vocab * a.hidden;
+  const int sx = direct_split(a.tokens, a.hidden, a.vocab, kGradRuns), sw = direct_split(a.vocab, a.hidden, a.tokens, kGradRuns);
+  // dx = d W, dW = d^T x
+  const DirectArgs x{nullptr, a.w, a.w, 0, a.ldw, a.ldw, INT64_MAX, a.tokens, a.hidden, a.vocab, sx,
+                     {a.dx, nullptr}, INT64_MAX, {a.norm, a.dloss}, sx > 1 ? s.dx_parts : nullptr};
+  const DirectArgs w{nullptr, a.x, a.x, 0, a.ldx, a.ldx, INT64_MAX, a.vocab, a.hidden, a.tokens, sw,
+                     {a.dw, nullptr}, INT64_MAX, {a.norm, a.dloss}, sw > 1 ? s.dw_parts : nullptr};
+  float* z = reinterpret_cast<float*>(s.d);
+  const auto grads = [&](const auto& d) {
+    using D = std::decay_t<decltype(d)>;
+    return a.dtype == P2P_DTYPE_F32   ? direct_grads<D, float>(x, w, d, st)
+           : a.dtype == P2P_DTYPE_F16 ? direct_grads<D, f16>(x, w, d, st)
+                                      : direct_grads<D, bf16>(x, w, d, st);
   };
-  // dx = d W, then dW = d^T x
-  for (const Side& e : {Side{false, a.w, a.ldw, a.tokens, a.vocab, a.dx, s.dx_parts},
-                        Side{true, a.x, a.ldx, a.vocab, a.tokens, a.dw, s.dw_parts}}) {
-    const int split = direct_split(e.M, a.hidden, e.K);
-    const DirectArgs g{d, e.b, e.b, P2P_DTYPE_F32, a.dtype, a.vocab, e.ldb, e.ldb, INT64_MAX, e.M, a.hidden, e.K, split,
-                       {e.out, nullptr}, INT64_MAX, {a.norm, a.dloss}, split > 1 ? e.parts : nullptr};
-    if ((rc = direct_product(e.at, true, g, st)) != P2P_OK) return rc;
-    const int64_t n = e.M * a.hidden;
-    if (split > 1 && (rc = join_parts(e.parts, split, n, n, 0, a.norm, a.dloss, 1.f, e.out, nullptr, a.dtype, st)) != P2P_OK)
-      return rc;
+  if (ce_made_in_place(a)) {
+    rc = grads(CeGrad{z, runs, a.tokens, a.vocab, a.lse, a.target, a.ignore_index});
+  } else {
+    const int64_t blocks = ceil_div(a.tokens * ceil_div(a.vocab, 4), kBlock);
+    ce_grad_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
+        z, runs, a.tokens, a.vocab, a.lse, a.target, a.ignore_index);
+    if ((rc = launch_status()) != P2P_OK) return rc;
+    rc = grads(DirectLines<float>{z, z, a.vocab, a.vocab, INT64_MAX});
   }
-  return P2P_OK;
+  if (rc == P2P_OK && sx > 1) rc = join_parts(s.dx_parts, sx, nx, nx, 0, a.norm, a.dloss, 1.f, a.dx, nullptr, a.dtype, st);
+  if (rc == P2P_OK && sw > 1) rc = join_parts(s.dw_parts, sw, nw, nw, 0, a.norm, a.dloss, 1.f, a.dw, nullptr, a.dtype, st);
+  return rc;
 }
 
 }  // namespace p2p
