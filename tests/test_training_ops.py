@@ -812,6 +812,116 @@ def test_linear_cross_entropy_refuses_wide_ignore_index(cuda):
     assert T.linear_cross_entropy_forward(x, w, t, ignore_index=-(1 << 63))[0].item() > 1
 
 
+# ------------------------------------------------------------------ each product's way
+# Small products go one way, large ones another, and their gradients' operands are made in place or
+# in a buffer: the cases above that are small have their likes here on the other side of each rule.
+TILED = (1100, 1032, 1208, 2608)  # rows, features, units, vocabulary: on tiles in every type
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,units", [(90, 500, 1001), (100, 250, 1003)])
+def test_gated_linear_gradients_out_of_a_buffer(cuda, dtype, rows, cols, units):
+    test_gated_linear(cuda, dtype, rows, cols, units, "gelu")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,vocab", [(100, 520, 1003), (40, 300, 1500), (33, 64, 61)])
+def test_linear_cross_entropy_gradients_out_of_a_buffer(cuda, dtype, rows, cols, vocab):
+    test_linear_cross_entropy(cuda, dtype, rows, cols, vocab, "mean")
+
+
+@gpu
+def test_long_sums_of_few_tiles(cuda):
+    """Float32 on small tiles, the sum cut into runs in both gradients."""
+    test_gated_linear_large_tiles(cuda, torch.float32, 200, 36000, 200)
+
+
+@gpu
+def test_linear_cross_entropy_copied_pieces(cuda):
+    """A weight whose copy is made in several pieces, forward and backward."""
+    rows, cols, vocab = 130, 1000, 90000
+    x, w, t = ce_inputs(rows, cols, vocab, torch.float32, 110)
+    a, keep = T._ce_args(x, w, t, -100)
+    a.lse = a.norm = x.data_ptr()
+    assert N.lib().p2p_linear_ce_workspace(a, 0) < 6 * vocab * cols  # fewer bytes than the copy of all of w
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    got = T.linear_cross_entropy_backward(x, w, t, lse, norm)
+    want, err = ce_reference(x, w, t, 1.0, -100, "mean")
+    check(loss, want[0], rounded(want[0], err[0], torch.float32), "loss")
+    for o, v, e, name in zip(got, want[1:], err[1:], ("dx", "dw")):
+        check(o, v, rounded(v, e, torch.float32), name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tiled_layouts(cuda, dtype):
+    """Pitches, bases at any element and strides on tiles: the bits of the dense call."""
+    rows, cols, units, vocab = TILED
+    wide = randn((rows, 2 * cols + 8), dtype, 111)
+    ww = randn((vocab, 2 * cols + 8), dtype, 112, cols ** -0.5)
+    dh = randn((rows, units + 3), dtype, 113)[:, 3:]
+    t = torch.arange(rows, device="cuda") % vocab
+    for x, w in ((wide[:, 8:8 + cols], ww[:, :cols]), (wide[:, 3:3 + cols], ww[:, 5:5 + cols]), (wide[:, :2 * cols:2], ww[:, :2 * cols:2]),
+                 (wide[:, 8:7 + cols], ww[:, 1:cols])):
+        dx, dw = (a.clone(memory_format=torch.contiguous_format) for a in (x, w))
+        a = T.gated_linear_forward(x, w[:units], w[units:2 * units], "gelu")
+        b = T.gated_linear_forward(dx, dw[:units], dw[units:2 * units], "gelu")
+        a += T.gated_linear_backward(dh, x, w[:units], w[units:2 * units], *a[1:], "gelu")
+        b += T.gated_linear_backward(dh.contiguous(), dx, dw[:units], dw[units:2 * units], *b[1:], "gelu")
+        assert all(same_bits(p, q) for p, q in zip(a, b))
+        a, b = T.linear_cross_entropy_forward(x, w, t), T.linear_cross_entropy_forward(dx, dw, t)
+        a += T.linear_cross_entropy_backward(x, w, t, *a[1:])
+        b += T.linear_cross_entropy_backward(dx, dw, t, *b[1:])
+        assert all(same_bits(p, q) for p, q in zip(a, b))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tiled_guards(cuda, dtype):
+    """NaN all round the operands of tiles, in the pitch and behind the last row, reaches no result."""
+    rows, cols, units, vocab = TILED
+    for cols_ in (cols, cols - 3):
+        xs = torch.full((rows + 3, cols + 24), float("nan"), dtype=dtype, device="cuda")
+        ws = torch.full((vocab + 2, cols + 24), float("nan"), dtype=dtype, device="cuda")
+        x, w = xs[1:1 + rows, 8:8 + cols_], ws[1:1 + vocab, 8:8 + cols_]
+        x.copy_(randn(x.shape, dtype, 114, 0.2))
+        w.copy_(randn(w.shape, dtype, 115, 0.2))
+        dh = torch.full((rows, units + 8), float("nan"), dtype=dtype, device="cuda")[:, 8:]
+        dh.copy_(randn(dh.shape, dtype, 116))
+        wg, wu = w[:units], w[units:2 * units]
+        h, gate, up = T.gated_linear_forward(x, wg, wu)
+        out = (h, gate, up) + T.gated_linear_backward(dh, x, wg, wu, gate, up)
+        t = torch.arange(rows, device="cuda") % vocab
+        loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+        out += (loss, lse) + T.linear_cross_entropy_backward(x, w, t, lse, norm)
+        assert all(torch.isfinite(o).all() for o in out)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("odd", [0, 1])
+def test_tiled_captured_step(cuda, dtype, odd):
+    rows, cols, units, vocab = TILED
+    replayed(step_calls(dtype, rows + odd, cols + odd, units + odd, vocab + odd), str(dtype))
+
+
+@gpu
+def test_tiled_side_streams(cuda):
+    """Two calls at once on tiles, each with its own workspace."""
+    step = step_calls(torch.float16, *(n + 1 for n in TILED))
+    want = [t.clone() for t in step()]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(step())
+    torch.cuda.synchronize()
+    for out in got:
+        assert all(same_bits(a, b) for a, b in zip(out, want))
+
+
 # ------------------------------------------------------------------ offsets past 32 bits
 def device_randn(shape, dtype, seed, scale=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
