@@ -517,22 +517,37 @@ static int32_t gemm_launch(const GemmArgs& g, bool is_f16, bool big, const Epi& 
              : gemm_launch_cfg<false, AT, BT, DUAL, Small>(g, epi, st);
 }
 
-// Tile and k-runs of a product.  The large tile where its tiles fill most of
-// the 256 CUs; where they do not and the sum is long, its k-steps are cut into
-// runs of at least kMinRun steps; what is still short of blocks takes the
-// small tile (two blocks per CU).
-constexpr int kMinRun = 8, kMaxSplit = 16;
+// Tile and k-runs of a product: what is least by the times of a k-step (us) of a
+// round of blocks, 256 large or 512 small ones (256 alone on their CUs take
+// less), and of writing and joining the runs' sums.  Kernel times, large / small
+// (runs): M x N x K = 2048 x 4096 x 2048 64.3 / 43.8; 4096 x 2048 x 2048 57.1 (2) /
+// 43.3 (1); 4096 x 512 x 4096 44.2 (8) / 33.0 (4); 1024 x 4096 x 8192 89.3 (4) /
+// 82.7 (2); 1024 x 1000 x 64000 144.8 (16) / 173.9 (8); 8192 x 4096 x 1024 82.3 /
+// 95.6; 1024 x 32000 x 1000 84.6 / 104.8.  Tiles of 256 x 128 were between the
+// two or behind them everywhere.
+constexpr int kMinRun = 8;
 struct Plan {
   bool big;
   int split;
 };
+static inline double gemm_time(bool big, int64_t tiles, int64_t steps, int split, int64_t out) {
+  const int64_t blocks = tiles * split, slots = big ? 256 : 512, rest = blocks % slots;
+  const double round = big ? 1.8 : 1.05, last = rest == 0 ? 0.0 : !big && rest <= 256 ? 0.74 : round;
+  const double product = (static_cast<double>(blocks / slots) * round + last) * static_cast<double>(ceil_div(steps, split));
+  return split == 1 ? product : product + 5.0 + 8.0 * split * static_cast<double>(out) / 6.0e6;
+}
 static inline Plan gemm_plan(int64_t M, int64_t N, int64_t steps, bool may_split) {
   const int64_t tb = ceil_div(M, Big::BM) * ceil_div(N, Big::BN), ts = ceil_div(M, Small::BM) * ceil_div(N, Small::BN);
-  if (tb >= 192) return Plan{true, 1};
-  const int64_t most = may_split ? std::min<int64_t>(kMaxSplit, std::max<int64_t>(1, steps / kMinRun)) : 1;
-  const int64_t sb = std::min(most, 256 / tb);
-  if (tb * sb >= 192) return Plan{true, static_cast<int>(sb)};
-  return Plan{false, static_cast<int>(std::max<int64_t>(1, std::min(most, 512 / ts)))};
+  const int64_t most = may_split ? std::max<int64_t>(1, steps / kMinRun) : 1;
+  Plan best{true, 1};
+  double least = gemm_time(true, tb, steps, 1, M * N);
+  for (const int split : {1, 2, 3, 4, 6, 8, 12, 16})
+    for (const bool big : {true, false}) {
+      if (split > most) return best;
+      const double t = gemm_time(big, big ? tb : ts, steps, split, M * N);
+      if (t < least) least = t, best = Plan{big, split};
+    }
+  return best;
 }
 static inline int64_t ksteps(int64_t K, int nseg) { return ceil_div(K, kGemmK) * nseg; }
 
