@@ -55,28 +55,40 @@ struct GatedEpi {
   int32_t dtype, act;
 
   template <class Cfg>
-  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char*) const {
-    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
+    const auto put = [&](int64_t m, int64_t n, f4 gv, f4 uv) {
+      if (m >= g.M || n >= units) return;
+      f4 hv;
 #pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + Cfg::row(i) + i16;
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int j = 0; j < Cfg::NJ; j += 2) {
-        const int64_t n = (p.n0 + Cfg::col(j)) / 2 + q4;
-        if (n >= units) continue;
-        const f4 gv = acc[i][j], uv = acc[i][j + 1];
-        f4 hv;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a, da;
-          activation(act, gv[e], &a, &da);
-          hv[e] = a * uv[e];
-        }
-        store4_as(h, dtype, m, units, n, units, hv);
-        if (gate) store4(gate + m * units, n, units, gv);
-        if (up) store4(up + m * units, n, units, uv);
+      for (int e = 0; e < 4; ++e) {
+        float a, da;
+        activation(act, gv[e], &a, &da);
+        hv[e] = a * uv[e];
       }
+      store4_as(h, dtype, m, units, n, units, hv);
+      if (gate) store4(gate + m * units, n, units, gv);
+      if (up) store4(up + m * units, n, units, uv);
+    };
+    if constexpr (RowImage<Cfg>::USED) {
+      constexpr int LANES = Cfg::BN / 8, PER = 64 / LANES, ROWS = RowImage<Cfg>::ROWS;
+      const RowImage<Cfg> image{lds, p};
+      const int k = p.lane % LANES, chunk = k / 4 * 8 + k % 4;  // four units: their g, and four chunks on their u
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        image.put(acc, half);
+#pragma unroll 4
+        for (int r = 0; r < ROWS; r += PER) {
+          const int row = image.template row<PER>(p.wave, r + p.lane / LANES);
+          put(static_cast<int64_t>(p.tm) * Cfg::BM + half * Cfg::HM + row, static_cast<int64_t>(p.tn) * (Cfg::BN / 2) + k * 4,
+              image.get(row, chunk), image.get(row, chunk + 4));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < Cfg::NJ; j += 2)
+          put(p.m0 + Cfg::row(i) + (p.lane & 15), (p.n0 + Cfg::col(j)) / 2 + (p.lane >> 4) * 4, acc[i][j], acc[i][j + 1]);
     }
   }
 };

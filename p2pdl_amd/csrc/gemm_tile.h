@@ -408,6 +408,82 @@ __global__ __launch_bounds__(Cfg::THREADS, Cfg::WAVES * Cfg::BLOCKS_PER_CU / 4) 
 }
 
 // ------------------------------------------------------------------ epilogues
+// A large tile's halves (rows) laid out by rows in LDS, floats, 16-byte chunk c
+// of row r at position c ^ r % 16: a wave then stores whole rows.  As the
+// accumulators lie, 16 rows of 32 bytes an instruction, the 33 MB of bf16 of a
+// round of tiles leave in 11 us, so in 8, the copy through LDS in it (1023 x 1001
+// x 32003 float16: d 108 -> 101 us, dW 100 -> 94).  Small tiles, two blocks to
+// a CU, are stored as they lie (1023 x 2731 x 1001: 27 us, by rows 29).
+template <class Cfg>
+struct RowImage {
+  static constexpr bool USED = Cfg::BLOCKS_PER_CU == 1;
+  static constexpr int PITCH = Cfg::BN * 4, ROWS = USED ? Cfg::HM / Cfg::WAVES : 0;  // a wave's rows of a half
+  char* lds;
+  const Place& p;
+
+  // Half h, whole for every wave of the block when it returns.
+  __device__ __forceinline__ void put(const f4 (&acc)[Cfg::MI][Cfg::NJ], int h) const {
+    const int i16 = p.lane & 15;
+    if (h) __syncthreads();  // the last half has been read
+#pragma unroll
+    for (int i = 0; i < Cfg::MI / 2; ++i)
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j) {
+        const int row = p.wm * Cfg::QM + i * 16 + i16, chunk = (p.wn * Cfg::QN + Cfg::col(j)) / 4 + (p.lane >> 4);
+        *(P2P_LDS f4*)((P2P_LDS char*)(lds) + row * PITCH + ((chunk ^ i16) << 4)) = acc[h * (Cfg::MI / 2) + i][j];
+      }
+    __syncthreads();
+  }
+  __device__ __forceinline__ f4 get(int row, int chunk) const {
+    return *(const P2P_LDS f4*)((const P2P_LDS char*)(lds) + row * PITCH + ((chunk ^ (row & 15)) << 4));
+  }
+  // Row r of a wave, PER of them an instruction: the waves' rows alternate, so that few rows are shared by all.
+  template <int PER>
+  static __device__ __forceinline__ int row(int wave, int r) {
+    return (r / PER * Cfg::WAVES + wave) * PER + r % PER;
+  }
+};
+// f(r, m, n, C[m][n .. n + 3]) over the wave's part of the tile, n in steps of 4; r: which of its rows m is.
+template <class Cfg, typename F>
+__device__ __forceinline__ void by_rows(const f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, char* lds, const F& f) {
+  if constexpr (RowImage<Cfg>::USED) {
+    static_assert(Cfg::BN == 256, "a row per instruction");
+    constexpr int ROWS = RowImage<Cfg>::ROWS;
+    const RowImage<Cfg> image{lds, p};
+    const int64_t n = static_cast<int64_t>(p.tn) * Cfg::BN + p.lane * 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      image.put(acc, h);
+      const int64_t m0 = static_cast<int64_t>(p.tm) * Cfg::BM + h * Cfg::HM;
+#pragma unroll 4
+      for (int r = 0; r < ROWS; ++r) {
+        const int row = image.template row<1>(p.wave, r);
+        f(h * ROWS + r, m0 + row, n, image.get(row, p.lane));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i)
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j)
+        f(i * 16 + (p.lane & 15), p.m0 + Cfg::row(i) + (p.lane & 15), p.n0 + Cfg::col(j) + (p.lane >> 4) * 4, acc[i][j]);
+  }
+}
+// The row m whose number r is the lane's own: the lane requests what the row needs from memory before the image is
+// made, and the others take it from there.
+template <class Cfg>
+__device__ __forceinline__ int64_t row_of_lane(const Place& p) {
+  if constexpr (RowImage<Cfg>::USED) {
+    constexpr int ROWS = RowImage<Cfg>::ROWS;
+    static_assert(2 * ROWS <= 64, "");
+    const int r = p.lane & (2 * ROWS - 1);
+    return static_cast<int64_t>(p.tm) * Cfg::BM + r / ROWS * Cfg::HM + RowImage<Cfg>::template row<1>(p.wave, r % ROWS);
+  } else {
+    static_assert(Cfg::MI == 4, "64 rows");
+    return p.m0 + (p.lane / 32) * Cfg::HM + p.lane % 32;  // Cfg::row(lane / 16) + lane % 16
+  }
+}
+
 // Four neighbours of one row, columns n .. n + 3 of `cols`, as T.
 template <typename T>
 __device__ __forceinline__ void store4(T* row, int64_t n, int64_t cols, f4 v) {
@@ -464,37 +540,28 @@ struct StoreEpi {
   int add;
 
   template <class Cfg>
-  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char*) const {
-    const int i16 = p.lane & 15, q4 = (p.lane >> 4) * 4;
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
     float a = alpha;
     if (scale[0]) a *= ldc(scale[0]);
     if (scale[1]) a *= ldc(scale[1]);
+    by_rows<Cfg>(acc, p, lds, [&](int, int64_t m, int64_t n, f4 v) {
+      if (m >= g.M || n >= g.N) return;
+      if (partial) {
+        float* to = partial + (p.part * g.M + m) * pitch;
+        if (add) {
+          float o[4];
+          load_row<float, 4>(to, n, g.N, o);
 #pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + Cfg::row(i) + i16;
-      if (m >= g.M) continue;
+          for (int e = 0; e < 4; ++e) v[e] += o[e];
+        }
+        store4(to, n, g.N, v);
+        return;
+      }
       const bool second = half > 0 && m >= half;
       const int64_t row = second ? m - half : m;
-      if (!partial && half > 0 && row >= rows) continue;
-#pragma unroll
-      for (int j = 0; j < Cfg::NJ; ++j) {
-        const int64_t n = p.n0 + Cfg::col(j) + q4;
-        if (n >= g.N) continue;
-        if (partial) {
-          float* to = partial + (p.part * g.M + m) * pitch;
-          f4 v = acc[i][j];
-          if (add) {
-            float o[4];
-            load_row<float, 4>(to, n, g.N, o);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += o[e];
-          }
-          store4(to, n, g.N, v);
-        } else {
-          store4_as(out[second], dtype, row, pitch, n, g.N, acc[i][j] * a);
-        }
-      }
-    }
+      if (half > 0 && row >= rows) return;
+      store4_as(out[second], dtype, row, pitch, n, g.N, v * a);
+    });
   }
 };
 

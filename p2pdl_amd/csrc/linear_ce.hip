@@ -204,58 +204,40 @@ struct GradEpi {
   int32_t dtype;
 
   template <class Cfg>
-  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char*) const {
-    const int64_t n0 = p.n0 + (p.lane >> 4) * 4;
-    const int cols = static_cast<int>(std::min<int64_t>(g.N - n0, Cfg::BN));
-    const int width = static_cast<int>(std::min<int64_t>(pitch - n0, Cfg::BN));  // with the padding
-    const bool whole = p.n0 + Cfg::HN + 32 <= g.N;
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
+    const int64_t own = row_of_lane<Cfg>(p);
+    const int64_t y = own < g.M ? ldg(target + own) : ignore;
+    const int counted = y != ignore;
+    const float l = !counted ? 0.f : y >= 0 && y < vocab ? ldg(lse + own) : NAN;
+    const int64_t n0 = static_cast<int64_t>(p.tn) * Cfg::BN;
+    const int at = y >= first + n0 && y < first + n0 + Cfg::BN ? static_cast<int>(y - first - n0) : -1;  // in the tile
+    by_rows<Cfg>(acc, p, lds, [&](int r, int64_t m, int64_t n, f4 v) {
+      const float lr = __shfl(l, r, 64);
+      const int t = __shfl(at, r, 64) - static_cast<int>(n - n0), c = __shfl(counted, r, 64);
+      if (m >= g.M || n >= pitch) return;
+      f4 d;
 #pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i) {
-      const int64_t m = p.m0 + Cfg::row(i) + (p.lane & 15);
-      const int64_t y = m < g.M ? ldg(target + m) : ignore, at = y - first - n0;
-      const bool counts = y != ignore;
-      const float l = !counts ? 0.f : y >= 0 && y < vocab ? ldg(lse + m) : NAN;
-      const int t = counts && at >= 0 && at < Cfg::BN ? static_cast<int>(at) : -1;
-#pragma unroll
-      for (int j = 0; j < Cfg::NJ; ++j)
+      for (int e = 0; e < 4; ++e) {
+        const float x = v[e] - lr;
+        d[e] = !c || n + e >= g.N ? 0.f : (dtype == P2P_DTYPE_F32 ? expf(x) : __expf(x)) - (e == t ? 1.f : 0.f);
+      }
+      uint16_t* to = this->d + m * pitch + n;
+      if (dtype == P2P_DTYPE_F32) {
+        Pack<uint16_t, 4> o[3];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = acc[i][j][e] - l;
-          acc[i][j][e] = counts ? (dtype == P2P_DTYPE_F32 ? expf(x) : __expf(x)) : 0.f;
+          const Planes s = split3(d[e]);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) o[q].v[e] = s.p[q];
         }
-      if (__any(t >= 0)) {  // few tiles hold a token's target
 #pragma unroll
-        for (int j = 0; j < Cfg::NJ; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] -= Cfg::col(j) + e == t ? 1.f : 0.f;
+        for (int q = 0; q < 3; ++q) store_pack<uint16_t, 4>(to + q * plane, o[q]);
+      } else if (dtype == P2P_DTYPE_F16) {
+        store4(reinterpret_cast<f16*>(to), 0, 4, d * kHalfScale);
+      } else {
+        store4(reinterpret_cast<bf16*>(to), 0, 4, d);
       }
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int j = 0; j < Cfg::NJ; ++j) {
-        if (!whole) {
-          if (Cfg::col(j) >= width) continue;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (Cfg::col(j) + e >= cols) acc[i][j][e] = 0.f;
-        }
-        uint16_t* to = d + m * pitch + n0 + Cfg::col(j);
-        if (dtype == P2P_DTYPE_F32) {
-          Pack<uint16_t, 4> o[3];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const Planes s = split3(acc[i][j][e]);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) o[q].v[e] = s.p[q];
-          }
-#pragma unroll
-          for (int q = 0; q < 3; ++q) store_pack<uint16_t, 4>(to + q * plane, o[q]);
-        } else if (dtype == P2P_DTYPE_F16) {
-          store4(reinterpret_cast<f16*>(to), 0, 4, acc[i][j] * kHalfScale);
-        } else {
-          store4(reinterpret_cast<bf16*>(to), 0, 4, acc[i][j]);
-        }
-      }
-    }
+    });
   }
 };
 
