@@ -56,8 +56,8 @@ typedef void *p2p_stream_t; /* hipStream_t */
 enum {
   P2P_OK = 0,
   P2P_ERR_INVALID = -1,     /* bad argument (null pointer, k < 1, n < 0, bad trim) */
-  P2P_ERR_UNSUPPORTED = -2, /* valid but unsupported here (robust rules need k <= 256) */
-  P2P_ERR_ALIGN = -3        /* a float pointer that is not 4-byte aligned */
+  P2P_ERR_UNSUPPORTED = -2, /* valid but unsupported here (robust rules: k <= 256; K7-K10: sizes past their limits) */
+  P2P_ERR_ALIGN = -3        /* a pointer that is not aligned to its elements */
 };
 
 /* P2P_RULE_FEDAVG: the reference's ops as torch runs them on CPU tensors

@@ -22,8 +22,8 @@ extern "C" const char* p2p_strerror(int32_t code) {
   switch (code) {
     case P2P_OK: return "ok";
     case P2P_ERR_INVALID: return "p2p: invalid argument";
-    case P2P_ERR_UNSUPPORTED: return "p2p: unsupported (robust rules need 1 <= k <= 256)";
-    case P2P_ERR_ALIGN: return "p2p: float pointer not 4-byte aligned";
+    case P2P_ERR_UNSUPPORTED: return "p2p: unsupported here (robust rules: 1 <= k <= 256; a trainer's operators: sizes past their limits)";
+    case P2P_ERR_ALIGN: return "p2p: pointer not aligned to its elements";
     default: break;
   }
   if (code > 0) return hipGetErrorString(static_cast<hipError_t>(code));
