@@ -22,6 +22,8 @@
 // sums of k-runs that a second kernel joins and activates (forward and
 // backward of 32 x 512 x 512 float32 82 us on tiles, 21 so; 1 x 512 x 1000
 // bfloat16 35, 22; direct.h has the sizes on both sides of the rule).
+#include <type_traits>
+
 #include "direct_tile.h"
 #include "gemm_tile.h"
 
@@ -42,10 +44,12 @@ __device__ __forceinline__ void activation(float g, float* a, float* da) {
     *da = g > 0.f ? 1.f : 0.f;
   }
 }
-__device__ __forceinline__ void activation(int act, float g, float* a, float* da) {
-  if (act == P2P_ACT_SILU) activation<P2P_ACT_SILU>(g, a, da);
-  else if (act == P2P_ACT_GELU) activation<P2P_ACT_GELU>(g, a, da);
-  else activation<P2P_ACT_RELU>(g, a, da);
+// f(the activation as a type): chosen once for many elements; a choice for each would compute them all.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, const F& f) {
+  if (act == P2P_ACT_SILU) f(std::integral_constant<int, P2P_ACT_SILU>());
+  else if (act == P2P_ACT_GELU) f(std::integral_constant<int, P2P_ACT_GELU>());
+  else f(std::integral_constant<int, P2P_ACT_RELU>());
 }
 
 struct GatedEpi {
@@ -56,13 +60,17 @@ struct GatedEpi {
 
   template <class Cfg>
   __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
+    with_activation(act, [&](auto kind) { tile<decltype(kind)::value, Cfg>(acc, p, g, lds); });
+  }
+  template <int ACT, class Cfg>
+  __device__ __forceinline__ void tile(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
     const auto put = [&](int64_t m, int64_t n, f4 gv, f4 uv) {
       if (m >= g.M || n >= units) return;
       f4 hv;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float a, da;
-        activation(act, gv[e], &a, &da);
+        activation<ACT>(gv[e], &a, &da);
         hv[e] = a * uv[e];
       }
       store4_as(h, dtype, m, units, n, units, hv);
@@ -164,12 +172,14 @@ __global__ __launch_bounds__(kBlock) void gated_join_kernel(const float* parts, 
     const float* row = parts + r * 2 * units;
     sum_runs<4>(row, rows * 2 * units, runs, c, units, g);
     sum_runs<4>(row + units, rows * 2 * units, runs, c, units, u);
+    with_activation(act, [&](auto kind) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float a, da;
-      activation(act, g[e], &a, &da);
-      o[e] = a * u[e];
-    }
+      for (int e = 0; e < 4; ++e) {
+        float a, da;
+        activation<decltype(kind)::value>(g[e], &a, &da);
+        o[e] = a * u[e];
+      }
+    });
     if (dtype == P2P_DTYPE_F32) store_row<float, 4>(static_cast<float*>(h) + r * units, c, units, o);
     else if (dtype == P2P_DTYPE_F16) store_row<f16, 4>(static_cast<f16*>(h) + r * units, c, units, o);
     else store_row<bf16, 4>(static_cast<bf16*>(h) + r * units, c, units, o);
@@ -289,12 +299,17 @@ struct GatedGrad {
   int64_t units;
   int act;
 
-  __device__ __forceinline__ float one(float g, float u, float d, bool second) const {
+  template <int ACT>
+  static __device__ __forceinline__ float one(float g, float u, float d, bool second) {
     float a, da;
-    activation(act, g, &a, &da);
+    activation<ACT>(g, &a, &da);
     return second ? d * a : d * u * da;
   }
   __device__ __forceinline__ void read(int64_t t, int64_t c, int64_t cols, float (&v)[4]) const {
+    with_activation(act, [&](auto kind) { read_as<decltype(kind)::value>(t, c, v); });
+  }
+  template <int ACT>
+  __device__ __forceinline__ void read_as(int64_t t, int64_t c, float (&v)[4]) const {
     const float *gr = gate + t * units, *ur = up + t * units;
     const T* dr = dh + t * lddh;
     const bool second = c >= units;
@@ -305,13 +320,13 @@ struct GatedGrad {
       load_row<float, 4>(ur, n, units, u);
       load_row<T, 4>(dr, n, units, d);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = one(g[e], u[e], d[e], second);
+      for (int e = 0; e < 4; ++e) v[e] = one<ACT>(g[e], u[e], d[e], second);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {  // from dg into du, or past both
         const bool s = c + e >= units;
         const int64_t m = s ? c + e - units : c + e;
-        v[e] = m < units ? one(ldg(gr + m), ldg(ur + m), static_cast<float>(ldg(dr + m)), s) : 0.f;
+        v[e] = m < units ? one<ACT>(ldg(gr + m), ldg(ur + m), static_cast<float>(ldg(dr + m)), s) : 0.f;
       }
     }
   }

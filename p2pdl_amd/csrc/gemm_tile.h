@@ -484,6 +484,13 @@ __device__ __forceinline__ int64_t row_of_lane(const Place& p) {
   }
 }
 
+// x of lane r, which in an image's rows is the wave's.
+template <class Cfg, typename T>
+__device__ __forceinline__ T from_lane(T x, int r) {
+  if constexpr (RowImage<Cfg>::USED) return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), r));
+  else return __shfl(x, r, 64);
+}
+
 // Four neighbours of one row, columns n .. n + 3 of `cols`, as T.
 template <typename T>
 __device__ __forceinline__ void store4(T* row, int64_t n, int64_t cols, f4 v) {

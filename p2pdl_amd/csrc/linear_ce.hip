@@ -53,45 +53,67 @@ struct StatsEpi {
     const int cols = static_cast<int>(std::min<int64_t>(g.N - n0, Cfg::BN));  // left from n0
     const bool whole = p.n0 + Cfg::HN + 32 <= g.N;  // of the wave's columns none is past the end
     float2* rows = reinterpret_cast<float2*>(lds);  // [WN][BM]
+    // in steps over all of the lane's rows, so that their loads and exchanges wait together
+    int t[Cfg::MI];  // the target among the lane's columns
 #pragma unroll
     for (int i = 0; i < Cfg::MI; ++i) {
       const int64_t m = p.m0 + Cfg::row(i) + i16;
       const int64_t y = m < g.M ? ldg(target + m) - first - n0 : -1;
-      const int t = y >= 0 && y < Cfg::BN ? static_cast<int>(y) : -1;
-      if (!whole) {
+      t[i] = y >= 0 && y < cols ? static_cast<int>(y) : -1;
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i)
 #pragma unroll
         for (int j = 0; j < Cfg::NJ; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (Cfg::col(j) + e >= cols) acc[i][j][e] = -INFINITY;
-      }
-      if (__any(t >= 0)) {  // few tiles hold a token's target
+    }
+    float top[Cfg::MI], s[Cfg::MI];
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+      top[i] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < Cfg::NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[i] = fmaxf(top[i], acc[i][j][e]);  // passes over a NaN, which the sum below takes up
+    }
+#pragma unroll
+    for (int o = 16; o <= 32; o *= 2)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) top[i] = fmaxf(top[i], __shfl_xor(top[i], o, 64));
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i) {
+      if (__any(t[i] >= 0)) {  // few tiles hold a token's target
 #pragma unroll
         for (int j = 0; j < Cfg::NJ; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (Cfg::col(j) + e == t && t < cols) stg(at_target + m, acc[i][j][e]);
+            if (Cfg::col(j) + e == t[i]) stg(at_target + p.m0 + Cfg::row(i) + i16, acc[i][j][e]);
       }
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < Cfg::NJ; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);  // passes over a NaN, which the sum below takes up
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float base = top == -INFINITY ? 0.f : top;  // -inf throughout: a sum of zeros
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < Cfg::NJ; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = acc[i][j][e] - base;  // a column past the end: exp(-inf)
-          s += precise ? expf(x) : __expf(x);
-        }
-      s += __shfl_xor(s, 16, 64);
-      s += __shfl_xor(s, 32, 64);
-      if (p.lane < 16) rows[p.wn * Cfg::BM + p.wm * Cfg::QM + Cfg::row(i) + i16] = make_float2(top, s);
     }
+    // (a choice of exponential for each element would compute both)
+    const auto sums = [&](auto exponential) {
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const float base = top[i] == -INFINITY ? 0.f : top[i];  // -inf throughout: a sum of zeros
+        s[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < Cfg::NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i] += exponential(acc[i][j][e] - base);  // a column past the end: exp(-inf)
+      }
+    };
+    if (precise) sums([](float x) { return expf(x); });
+    else sums([](float x) { return __expf(x); });
+#pragma unroll
+    for (int o = 16; o <= 32; o *= 2)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) s[i] += __shfl_xor(s[i], o, 64);
+    if (p.lane < 16)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) rows[p.wn * Cfg::BM + p.wm * Cfg::QM + Cfg::row(i) + i16] = make_float2(top[i], s[i]);
     __syncthreads();
     for (int r = threadIdx.x; r < Cfg::BM; r += Cfg::THREADS) {
       const int64_t m = static_cast<int64_t>(p.tm) * Cfg::BM + r;
@@ -211,33 +233,35 @@ struct GradEpi {
     const float l = !counted ? 0.f : y >= 0 && y < vocab ? ldg(lse + own) : NAN;
     const int64_t n0 = static_cast<int64_t>(p.tn) * Cfg::BN;
     const int at = y >= first + n0 && y < first + n0 + Cfg::BN ? static_cast<int>(y - first - n0) : -1;  // in the tile
-    by_rows<Cfg>(acc, p, lds, [&](int r, int64_t m, int64_t n, f4 v) {
-      const float lr = __shfl(l, r, 64);
-      const int t = __shfl(at, r, 64) - static_cast<int>(n - n0), c = __shfl(counted, r, 64);
-      if (m >= g.M || n >= pitch) return;
-      f4 d;
+    const auto rows = [&](auto exponential, auto put) {
+      by_rows<Cfg>(acc, p, lds, [&](int r, int64_t m, int64_t n, f4 v) {
+        const float lr = from_lane<Cfg>(l, r);
+        const int t = from_lane<Cfg>(at, r) - static_cast<int>(n - n0), c = from_lane<Cfg>(counted, r);
+        if (m >= g.M || n >= pitch) return;
+        f4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = v[e] - lr;
-        d[e] = !c || n + e >= g.N ? 0.f : (dtype == P2P_DTYPE_F32 ? expf(x) : __expf(x)) - (e == t ? 1.f : 0.f);
-      }
-      uint16_t* to = this->d + m * pitch + n;
-      if (dtype == P2P_DTYPE_F32) {
+        for (int e = 0; e < 4; ++e) x[e] = !c || n + e >= g.N ? 0.f : exponential(v[e] - lr) - (e == t ? 1.f : 0.f);
+        put(d + m * pitch + n, x);
+      });
+    };
+    const auto fast = [](float x) { return __expf(x); };
+    if (dtype == P2P_DTYPE_F32) {
+      rows([](float x) { return expf(x); }, [&](uint16_t* to, f4 x) {
         Pack<uint16_t, 4> o[3];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const Planes s = split3(d[e]);
+          const Planes s = split3(x[e]);
 #pragma unroll
           for (int q = 0; q < 3; ++q) o[q].v[e] = s.p[q];
         }
 #pragma unroll
         for (int q = 0; q < 3; ++q) store_pack<uint16_t, 4>(to + q * plane, o[q]);
-      } else if (dtype == P2P_DTYPE_F16) {
-        store4(reinterpret_cast<f16*>(to), 0, 4, d * kHalfScale);
-      } else {
-        store4(reinterpret_cast<bf16*>(to), 0, 4, d);
-      }
-    });
+      });
+    } else if (dtype == P2P_DTYPE_F16) {
+      rows(fast, [](uint16_t* to, f4 x) { store4(reinterpret_cast<f16*>(to), 0, 4, x * kHalfScale); });
+    } else {
+      rows(fast, [](uint16_t* to, f4 x) { store4(reinterpret_cast<bf16*>(to), 0, 4, x); });
+    }
   }
 };
 
