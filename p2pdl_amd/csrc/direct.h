@@ -26,22 +26,24 @@ struct DirectArgs {
 // 256 x 256 x 512 32 / 41, 90 x 512 x 1000 36 / 42, 128 x 512 x 1000 46 / 43, 512 x
 // 256 x 1024 53 / 46.  Loss, float32: 1024 x 1024 x 1024 136 / 246, 1024 x 1024 x
 // 2048 239 / 271, 1500 x 1500 x 1500 448 / 349; bfloat16: 128 x 512 x 1000 49 / 61,
-// 200 x 512 x 1000 61 / 62, 512 x 256 x 1024 61 / 61.  Few rows leave the tiles empty
-// and float32 pays for copies of all of B: 16 x 4096 x 8192 232 / 794.  Up to 2^24
-// rows and columns: its tiles and the rows of its epilogues then fit one
-// dimension of a grid.
+// 200 x 512 x 1000 61 / 62, 512 x 256 x 1024 61 / 61.  Up to 64 rows 16-bit tiles are
+// half empty: 64 x 1001 x 3001 float16 loss 70 / 78, gated layer 25 x 2119 x 1210 52 / 74,
+// 32 x 1024 x 4096 bfloat16 53 / 47.  Float32 pays for copies of all of B besides:
+// 16 x 4096 x 8192 232 / 794.  Up to 2^24 rows and columns: its tiles and the rows of
+// its epilogues then fit one dimension of a grid.
 static inline bool direct_pays(int64_t M, int64_t N, int64_t K, int32_t dtype) {
   const double size = static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
   if (M > 1 << 24 || N > 1 << 24) return false;
-  return dtype == P2P_DTYPE_F32 ? M <= 128 || size <= 2.6e9 : size <= 1.0e8;
+  return dtype == P2P_DTYPE_F32 ? M <= 128 || size <= 2.6e9 : size <= (M <= 64 ? 2.0e8 : 1.0e8);
 }
-// Its k-runs: enough blocks for every CU twice, at least two k-steps each, at
-// most `most`.  Forward as many as a lane's loads take at once (sum_runs):
-// 32 x 784 x 10 float32 19.1 us with up to 32 runs, 15.0 with 8, 16.9 with 4;
-// 8 x 2048 x 1000 23.2, 16.3, 20.5.  The gradients' long sums more: 64 x 512 x
-// 32000 backward 96 us with 32, 195 with 8.
-constexpr int kForwardRuns = 8, kGradRuns = 32;
-P2P_INTERNAL int direct_split(int64_t M, int64_t N, int64_t K, int most);
+// Its k-runs, at least two k-steps each.  The forward pass joins them anyway:
+// blocks for every CU four times, up to as many runs as a lane's loads take at
+// once (sum_runs; 32 x 784 x 10 float32 19.1 us with up to 32 runs, 15.0 with 8, 16.9
+// with 4; 632 x 1800 x 873 gated forward 89 us with two blocks per CU, 61 with four).
+// Gradients: blocks for every CU twice, or four times where a run would
+// still be 28 steps long (4 x 2608 x 96752 968 -> 830 us, but 512 x 1024 x 1024 60 ->
+// 64), up to 128 runs (1 x 108 x 6640 bfloat16 24 us with 32, 13 with 128).
+P2P_INTERNAL int direct_split(int64_t M, int64_t N, int64_t K, bool forward);
 
 // A B^T, both operands' lines their rows, of one type.
 P2P_INTERNAL int32_t direct_product(const DirectArgs& g, int32_t dtype, hipStream_t st);

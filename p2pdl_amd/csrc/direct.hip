@@ -12,9 +12,10 @@ __global__ __launch_bounds__(256) void direct_kernel(DirectArgs g) {
   direct_tile<DirectLines<T>, T, false, false, BM>(g, a, blockIdx.x, blockIdx.y, lds);
 }
 
-int direct_split(int64_t M, int64_t N, int64_t K, int most) {
+int direct_split(int64_t M, int64_t N, int64_t K, bool forward) {
   const int64_t tiles = direct_tiles(M, N), steps = ceil_div(K, kDirectK);
-  return static_cast<int>(std::max<int64_t>(1, std::min({512 / tiles, steps / 2, static_cast<int64_t>(most)})));
+  const int64_t blocks = forward || steps * tiles > 512 * 28 ? 1024 : 512, most = forward ? 8 : 128;
+  return static_cast<int>(std::max<int64_t>(1, std::min({blocks / tiles, steps / 2, most})));
 }
 
 template <typename T>

@@ -231,11 +231,11 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
     int64_t floats = 0;
     if (backward) {
       if (!gated_made_in_place(a)) s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 4));
-      const int sx = direct_split(a.tokens, a.hidden, rows2, kGradRuns), sw = direct_split(rows2, a.hidden, a.tokens, kGradRuns);
+      const int sx = direct_split(a.tokens, a.hidden, rows2, false), sw = direct_split(rows2, a.hidden, a.tokens, false);
       if (sx > 1) s->dx_parts = static_cast<float*>(c.take(sx * a.tokens * a.hidden * 4));
       if (sw > 1) floats = sw * rows2 * a.hidden;
     } else {
-      floats = direct_split(a.tokens, 2 * a.units, a.hidden, kForwardRuns) * a.tokens * 2 * a.units;
+      floats = direct_split(a.tokens, 2 * a.units, a.hidden, true) * a.tokens * 2 * a.units;
     }
     if (floats) s->parts = static_cast<float*>(c.take(floats * 4));
     return c.used;
@@ -278,7 +278,7 @@ static int32_t gated_operands(const p2p_gated_linear_t& a, const GatedSpace& s, 
 }
 
 static int32_t gated_direct_fwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
-  const int split = direct_split(a.tokens, 2 * a.units, a.hidden, kForwardRuns);
+  const int split = direct_split(a.tokens, 2 * a.units, a.hidden, true);
   const DirectArgs g{a.x, a.w_gate, a.w_up, a.ldx, a.ldg, a.ldu, a.units, a.tokens, 2 * a.units, a.hidden, split,
                      {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, s.parts};
   const int32_t rc = direct_product(g, a.dtype, st);
@@ -335,7 +335,7 @@ struct GatedGrad {
 template <typename T>
 static int32_t gated_direct_bwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
   const int64_t rows2 = 2 * a.units, nx = a.tokens * a.hidden, nw = a.units * a.hidden;
-  const int sx = direct_split(a.tokens, a.hidden, rows2, kGradRuns), sw = direct_split(rows2, a.hidden, a.tokens, kGradRuns);
+  const int sx = direct_split(a.tokens, a.hidden, rows2, false), sw = direct_split(rows2, a.hidden, a.tokens, false);
   // dx = [dg du] [Wg; Wu], [dWg; dWu] = [dg du]^T x
   const DirectArgs x{nullptr, a.w_gate, a.w_up, 0, a.ldg, a.ldu, a.units, a.tokens, a.hidden, rows2, sx,
                      {a.dx, nullptr}, INT64_MAX, {nullptr, nullptr}, sx > 1 ? s.dx_parts : nullptr};

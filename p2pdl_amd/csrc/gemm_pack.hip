@@ -66,37 +66,58 @@ int32_t pack_matrices(const PackJob* jobs, int n, int32_t dtype, hipStream_t st)
   return launch_status();
 }
 
-template <typename T>
+// GROUPS of a block's lanes each take a run of the parts; their sums are added in that order.  Many parts of a small
+// result are a long chain of loads otherwise (1 x 108 x 6640 bfloat16, 32 runs: loss backward 24.9 us, 23.4 so).
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(kBlock) void join_kernel(const float* parts, int nparts, int64_t stride, int64_t n, int64_t second,
                                                       const float* scale0, const float* scale1, float alpha, T* out0, T* out1) {
+  constexpr int LANES = kBlock / GROUPS;
+  __shared__ float sums[GROUPS > 1 ? GROUPS - 1 : 1][LANES * 4];
   if (scale0) alpha *= ldc(scale0);
   if (scale1) alpha *= ldc(scale1);
-  parts += blockIdx.y * second;
   T* out = blockIdx.y ? out1 : out0;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * 4; i < n;
-       i += static_cast<int64_t>(gridDim.x) * kBlock * 4) {
-    float s[4];
-    sum_runs<4>(parts, stride, nparts, i, n, s);
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int from = nparts * group / GROUPS, to = nparts * (group + 1) / GROUPS;
+  const float* mine = parts + blockIdx.y * second + from * stride;
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * (LANES * 4); i0 < n; i0 += static_cast<int64_t>(gridDim.x) * (LANES * 4)) {
+    const int64_t i = i0 + lane * 4;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i < n) sum_runs<4>(mine, stride, to - from, i, n, s);
+    if constexpr (GROUPS > 1) {
+      __syncthreads();  // the last ones have been read
+      if (group)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[group - 1][e * LANES + lane] = s[e];
+      __syncthreads();
+      if (group) continue;
+#pragma unroll
+      for (int q = 0; q < GROUPS - 1; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += sums[q][e * LANES + lane];
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] *= alpha;
-    store_row<T, 4>(out, i, n, s);
+    if (i < n) store_row<T, 4>(out, i, n, s);
   }
+}
+
+template <typename T>
+static int32_t join_typed(const float* parts, int nparts, int64_t stride, int64_t n, int64_t second, const float* scale0,
+                          const float* scale1, float alpha, void* out0, void* out1, hipStream_t st) {
+  const bool groups = nparts > 8 && n <= int64_t(1) << 20;
+  const dim3 grid(blocks_for(ceil_div(n, 4) * (groups ? 8 : 1)), out1 ? 2 : 1);
+  const auto kernel = groups ? join_kernel<T, 8> : join_kernel<T, 1>;
+  kernel<<<grid, dim3(kBlock), 0, st>>>(parts, nparts, stride, n, second, scale0, scale1, alpha, static_cast<T*>(out0),
+                                        static_cast<T*>(out1));
+  return launch_status();
 }
 
 int32_t join_parts(const float* parts, int nparts, int64_t stride, int64_t n, int64_t second, const float* scale0,
                    const float* scale1, float alpha, void* out0, void* out1, int32_t dtype, hipStream_t st) {
   if (n == 0) return P2P_OK;
-  const dim3 grid(blocks_for(ceil_div(n, 4)), out1 ? 2 : 1), block(kBlock);
-  if (dtype == P2P_DTYPE_F32)
-    join_kernel<float><<<grid, block, 0, st>>>(parts, nparts, stride, n, second, scale0, scale1, alpha,
-                                               static_cast<float*>(out0), static_cast<float*>(out1));
-  else if (dtype == P2P_DTYPE_F16)
-    join_kernel<f16><<<grid, block, 0, st>>>(parts, nparts, stride, n, second, scale0, scale1, alpha, static_cast<f16*>(out0),
-                                             static_cast<f16*>(out1));
-  else
-    join_kernel<bf16><<<grid, block, 0, st>>>(parts, nparts, stride, n, second, scale0, scale1, alpha,
-                                              static_cast<bf16*>(out0), static_cast<bf16*>(out1));
-  return launch_status();
+  if (dtype == P2P_DTYPE_F32) return join_typed<float>(parts, nparts, stride, n, second, scale0, scale1, alpha, out0, out1, st);
+  if (dtype == P2P_DTYPE_F16) return join_typed<f16>(parts, nparts, stride, n, second, scale0, scale1, alpha, out0, out1, st);
+  return join_typed<bf16>(parts, nparts, stride, n, second, scale0, scale1, alpha, out0, out1, st);
 }
 
 }  // namespace p2p

@@ -408,13 +408,13 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
   Carver c{static_cast<char*>(base)};
   if (ce_direct(a)) {
     *s = CeSpace{};
-    const int64_t runs = direct_split(a.tokens, a.vocab, a.hidden, kForwardRuns);
+    const int64_t runs = direct_split(a.tokens, a.vocab, a.hidden, true);
     s->d = static_cast<uint16_t*>(c.take(runs * a.tokens * a.vocab * 4));
     if (!backward) {
       s->row_loss = static_cast<float*>(c.take(a.tokens * 4));
       return c.used;
     }
-    const int64_t sx = direct_split(a.tokens, a.hidden, a.vocab, kGradRuns), sw = direct_split(a.vocab, a.hidden, a.tokens, kGradRuns);
+    const int64_t sx = direct_split(a.tokens, a.hidden, a.vocab, false), sw = direct_split(a.vocab, a.hidden, a.tokens, false);
     if (sx > 1) s->dx_parts = static_cast<float*>(c.take(sx * a.tokens * a.hidden * 4));
     if (sw > 1) s->dw_parts = static_cast<float*>(c.take(sw * a.vocab * a.hidden * 4));
     return c.used;
@@ -466,7 +466,7 @@ static LossOut ce_out(const p2p_linear_ce_t& a) {
 }
 
 static int32_t ce_direct_logits(const p2p_linear_ce_t& a, const CeSpace& s, int* runs, hipStream_t st) {
-  *runs = direct_split(a.tokens, a.vocab, a.hidden, kForwardRuns);
+  *runs = direct_split(a.tokens, a.vocab, a.hidden, true);
   const DirectArgs g{a.x, a.w, a.w, a.ldx, a.ldw, a.ldw, INT64_MAX, a.tokens, a.vocab, a.hidden, *runs,
                      {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, reinterpret_cast<float*>(s.d)};
   return direct_product(g, a.dtype, st);
@@ -495,7 +495,7 @@ static int32_t ce_direct_bwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStre
   int32_t rc = ce_direct_logits(a, s, &runs, st);
   if (rc != P2P_OK) return rc;
   const int64_t nx = a.tokens * a.hidden, nw = a.vocab * a.hidden;
-  const int sx = direct_split(a.tokens, a.hidden, a.vocab, kGradRuns), sw = direct_split(a.vocab, a.hidden, a.tokens, kGradRuns);
+  const int sx = direct_split(a.tokens, a.hidden, a.vocab, false), sw = direct_split(a.vocab, a.hidden, a.tokens, false);
   // dx = d W, dW = d^T x
   const DirectArgs x{nullptr, a.w, a.w, 0, a.ldw, a.ldw, INT64_MAX, a.tokens, a.hidden, a.vocab, sx,
                      {a.dx, nullptr}, INT64_MAX, {a.norm, a.dloss}, sx > 1 ? s.dx_parts : nullptr};
