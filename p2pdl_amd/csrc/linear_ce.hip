@@ -326,6 +326,40 @@ __global__ __launch_bounds__(1024) void ce_row_kernel(const float* parts, int ru
   }
 }
 
+// The same of few tokens with long rows: (maximum, sum) of 1024 logits of a token per block, joined by
+// ce_join_kernel (loss forward, a block per row / in chunks: 2 x 258 x 91984 float16 84 / 47 us, 64 x 512 x 32000
+// float32 50 / 40, 16 x 512 x 5000 18.6 / 16.1).
+constexpr int kChunk = 1024;
+__global__ __launch_bounds__(256) void ce_chunk_kernel(const float* parts, int runs, int64_t T, int64_t V, const int64_t* target,
+                                                       float2* stats, float* at_target) {
+  __shared__ float2 waves[4];
+  const int64_t t = blockIdx.y, n = static_cast<int64_t>(blockIdx.x) * kChunk + threadIdx.x * 4, y = ldg(target + t);
+  float z[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n < V && runs <= 2) add_runs<2, 4>(parts + t * V, T * V, runs, n, V, z);
+  else if (n < V) sum_runs<4>(parts + t * V, T * V, runs, n, V, z);
+  float2 a = make_float2(-INFINITY, 0.f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < V) {
+      a.x = fmaxf(a.x, z[e]);
+      if (n + e == y) stg(at_target + t, z[e]);
+    }
+#pragma unroll
+  for (int h = 32; h > 0; h >>= 1) a.x = fmaxf(a.x, __shfl_xor(a.x, h, 64));
+  const float base = a.x == -INFINITY ? 0.f : a.x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < V) a.y += expf(z[e] - base);
+  a.y = wave_sum(a.y);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x / 64] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 4; ++w) a = StatsEpi::join_stats(a, waves[w]);
+    stats[blockIdx.x * T + t] = a;
+  }
+}
+
 // d of the logits in k-runs, over the first run.
 __global__ __launch_bounds__(kBlock) void ce_grad_kernel(float* parts, int runs, int64_t T, int64_t V, const float* lse,
                                                          const int64_t* target, int64_t ignore) {
@@ -398,6 +432,8 @@ static Plan ce_dw_plan(const p2p_linear_ce_t& a, int64_t rows) {
 static bool ce_direct(const p2p_linear_ce_t& a) {
   return direct_pays(a.tokens, a.vocab, a.hidden, a.dtype) && a.tokens * a.vocab * 4 <= kPieceBytes;
 }
+// Whether the direct forward pass takes a token's row in chunks: rows of one block each would leave the chip idle.
+static bool ce_chunked(const p2p_linear_ce_t& a) { return a.tokens <= 64 && a.vocab > 4 * kChunk; }
 // Whether the direct gradients make d where they read it.  Backward, us, so /
 // out of the logits' buffer: 32 x 256 x 10 float32 9.4 / 12.5, 1 x 512 x 1000
 // bfloat16 13.8 / 14.8, 64 x 256 x 512 float32 17.7 / 17.2, 64 x 512 x 1000 22.0 / 19.7.
@@ -412,6 +448,10 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
     s->d = static_cast<uint16_t*>(c.take(runs * a.tokens * a.vocab * 4));
     if (!backward) {
       s->row_loss = static_cast<float*>(c.take(a.tokens * 4));
+      if (ce_chunked(a)) {
+        s->part = static_cast<float2*>(c.take(ceil_div(a.vocab, kChunk) * a.tokens * 8));
+        s->at_target = static_cast<float*>(c.take(a.tokens * 4));
+      }
       return c.used;
     }
     const int64_t sx = direct_split(a.tokens, a.hidden, a.vocab, false), sw = direct_split(a.vocab, a.hidden, a.tokens, false);
@@ -477,6 +517,15 @@ static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStre
   int32_t rc = ce_direct_logits(a, s, &runs, st);
   if (rc != P2P_OK) return rc;
   const float* z = reinterpret_cast<const float*>(s.d);
+  if (ce_chunked(a)) {
+    const int chunks = static_cast<int>(ceil_div(a.vocab, kChunk));
+    ce_chunk_kernel<<<dim3(chunks, static_cast<unsigned>(a.tokens)), dim3(256), 0, st>>>(z, runs, a.tokens, a.vocab, a.target,
+                                                                                         s.part, s.at_target);
+    if ((rc = launch_status()) != P2P_OK) return rc;
+    ce_join_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.part, chunks, nullptr, 1, 1, a.vocab, s.at_target, a.lse, s.row_loss,
+                                                   ce_out(a), 1);
+    return launch_status();
+  }
   // a token per 16 lanes, wave or block by the length of its row; few tokens in one block, which saves the launch
   // of the sum.  Forward, us: 32 x 784 x 10 float32 15.1 with a wave per token, 10.8 so; 32 x 512 x 512, of 131072
   // partial logits, 16.1 in one block, 13.3 in two; 64 x 128 x 100 17.5, 12.6.

@@ -116,35 +116,35 @@ __device__ __forceinline__ void store_row(T* row, int64_t c, int64_t cols, const
   }
 }
 
-// s[e] = p[c + e] + p[stride + c + e] + ... over `runs`, in that order; elements at and past `cols` are 0.  Loads
-// go out eight runs at a time, the last ones again in place of what is past them: a loop over a
-// remainder would wait for each.
+// s[e] += p[c + e] + p[stride + c + e] + ... over `runs` <= W, all loads before the first sum, those past the last
+// run again in its place (a loop over a remainder would wait for each).
+template <int W, int N>
+__device__ __forceinline__ void add_runs(const float* p, int64_t stride, int runs, int64_t c, int64_t cols, float (&s)[N]) {
+  float v[W][N];
+  if (c + N <= cols) {
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+      const Pack<float, N> q = load_pack<float, N>(p + (u < runs ? u : runs - 1) * stride + c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[u][e] = q.v[e];
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < W; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[u][e] = ldg(p + (u < runs ? u : runs - 1) * stride + (c + e < cols ? c + e : cols - 1));
+  }
+#pragma unroll
+  for (int u = 0; u < W; ++u)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] += u < runs && c + e < cols ? v[u][e] : 0.f;
+}
+// s[e] = p[c + e] + p[stride + c + e] + ... over `runs`, in that order, eight at a time; elements at and past `cols` are 0.
 template <int N>
 __device__ __forceinline__ void sum_runs(const float* p, int64_t stride, int runs, int64_t c, int64_t cols, float (&s)[N]) {
 #pragma unroll
   for (int e = 0; e < N; ++e) s[e] = 0.f;
-  const bool whole = c + N <= cols;
-  for (int r0 = 0; r0 < runs; r0 += 8) {
-    float v[8][N];
-    if (whole) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const Pack<float, N> q = load_pack<float, N>(p + (r0 + u < runs ? r0 + u : runs - 1) * stride + c);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[u][e] = q.v[e];
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          v[u][e] = ldg(p + (r0 + u < runs ? r0 + u : runs - 1) * stride + (c + e < cols ? c + e : cols - 1));
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int e = 0; e < N; ++e) s[e] += r0 + u < runs && c + e < cols ? v[u][e] : 0.f;
-  }
+  for (int r = 0; r < runs; r += 8) add_runs<8, N>(p + r * stride, stride, runs - r < 8 ? runs - r : 8, c, cols, s);
 }
 
 __device__ __forceinline__ float wave_sum(float v) {

@@ -833,6 +833,35 @@ def test_linear_cross_entropy_gradients_out_of_a_buffer(cuda, dtype, rows, cols,
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,vocab", [(1, 16, 40000), (3, 600, 4100), (64, 33, 5003), (17, 128, 9001)])
+def test_linear_cross_entropy_long_rows_of_few_tokens(cuda, dtype, rows, cols, vocab):
+    test_linear_cross_entropy(cuda, dtype, rows, cols, vocab, "mean")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_cross_entropy_long_rows_targets(cuda, dtype):
+    """Chunks of a row: classes at -inf in whole chunks, targets at a chunk's ends, ignored, outside."""
+    rows, vocab = 6, 5000
+    x = torch.ones(rows, 1, dtype=dtype, device="cuda")
+    w = torch.full((vocab, 1), float("-inf"), dtype=dtype, device="cuda")
+    w[[1023, 1024, 4999]] = torch.tensor([[1.0], [2.0], [3.0]], dtype=dtype, device="cuda")
+    t = torch.tensor([1023, 1024, 4999, -100, 4999, 1024], device="cuda")
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    want = math.log(math.exp(1) + math.exp(2) + math.exp(3))
+    assert (lse - want).abs().max().item() <= 32 * U * want
+    assert abs(loss.item() - (want - (1 + 2 + 3 + 3 + 2) / 5)) <= 64 * U * want and norm.item() == np.float32(1) / np.float32(5)
+    t[4] = vocab
+    assert math.isnan(T.linear_cross_entropy_forward(x, w, t)[0].item())
+    t[:] = -100
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    assert loss.item() == 0 and norm.item() == 0 and torch.isfinite(lse).all()
+    w[2000] = float("nan")
+    assert torch.isnan(T.linear_cross_entropy_forward(x, w, t)[1]).all()
+
+
+@gpu
 def test_long_sums_of_few_tiles(cuda):
     """Float32 on small tiles, the sum cut into runs in both gradients."""
     test_gated_linear_large_tiles(cuda, torch.float32, 200, 36000, 200)
