@@ -557,6 +557,32 @@ def test_gated_linear_float32_range(cuda):
     assert not torch.isfinite(gate[2]).any() and torch.isfinite(gate[[0, 1, 3]]).all()
 
 
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_activations_and_slopes(cuda, act):
+    """The activations alone (one feature, weights of 1, so g = u = x) from one tail to the other: off by
+    16 U of themselves and 4 U for each unit of their exponential's argument, the slopes by 32 U (1 + |g|)."""
+    x = torch.cat([torch.linspace(-12, 12, 200001, device="cuda"), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 80.0, -80.0, 3e38], device="cuda")])[:, None]
+    one = torch.ones(1, 1, device="cuda")
+    h, gate, up = T.gated_linear_forward(x, one, one, act)
+    assert torch.equal(gate, x)  # (a sum starts from +0: -0 comes out as 0)
+    g = x.double().cpu()
+    phi = 0.5 * torch.erfc(-g / math.sqrt(2)) if act == "gelu" else torch.sigmoid(g)  # with their lower tails
+    value = g * phi
+    slope = phi + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi) if act == "gelu" else phi * (1 + g * (1 - phi))
+    exponent = 0.5 * g * g if act == "gelu" else g.abs()
+    # h = act * u, u = g; products of two floats: the relative error is that of act and two roundings
+    got = h.double().cpu() / torch.where(g == 0, 1.0, g)
+    part = torch.where(g == 0, 0.0, value)
+    bound = U * (16 + 4 * exponent) * part.abs() + 1e-30
+    fine = torch.isfinite(h.cpu()) & (g.abs() < 1e18)
+    assert ((got - part).abs() <= bound)[fine].all()
+    dh = torch.ones_like(h)
+    dx = T.gated_linear_backward(dh, x, one, one, gate, up, act)[0].double().cpu()  # d(act(g) g) = slope g + act
+    want = slope * g + value
+    assert ((dx - want).abs()[fine] <= (32 * U * (1 + g.abs()) * (1 + g.abs()))[fine]).all()
+
+
 # ------------------------------------------------------------------ linear cross entropy
 def ce_reference(x, w, target, dloss, ignore, reduction):
     """Values and bounds (before the last rounding) of loss, dx, dw."""
