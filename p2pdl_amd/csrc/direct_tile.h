@@ -5,7 +5,8 @@
 // once.  A lane reads four neighbouring k of a row at once and feeds them to
 // four v_mfma_f32_16x16x4_f32; the order of k within a step is the same for both
 // operands.  The next step's elements are on their way to registers while
-// this one's are multiplied; four blocks share a CU.  Few tiles are cut along
+// this one's are multiplied (two steps ahead cost the fourth block of a CU its
+// registers: 1024 x 1024 x 1024 float32 loss backward 98 us, 114); four blocks share a CU.  Few tiles are cut along
 // k into runs, their sums joined in run order by the caller.
 #pragma once
 #include "direct.h"
@@ -17,44 +18,63 @@ using f4 = float __attribute__((ext_vector_type(4)));
 constexpr int kDirectN = 64, kDirectK = 32, kDirectPitch = kDirectK + 4;
 constexpr int kDirectLds = 2 * (64 + kDirectN) * kDirectPitch;  // floats
 
-// A matrix in memory, of up to two parts: elements c .. c + 3 of line i, 0 at and past `cols`.
+// A source of an operand: fetch(i, c, cols) requests elements c .. c + 3 of
+// line i (0 at and past `cols`), of(raw) makes them floats.  Between the two
+// lies a step's products: a conversion at the load would wait for it there.
+
+// A matrix in memory, of up to two parts.
 template <typename E>
 struct DirectLines {
   const E *p, *p2;
   int64_t ld, ld2, lines;  // lines of p; the further ones are p2's
-  __device__ __forceinline__ void read(int64_t i, int64_t c, int64_t cols, float (&v)[4]) const {
-    load_row<E, 4>(i < lines ? p + i * ld : p2 + (i - lines) * ld2, c, cols, v);
+  struct Raw4 {
+    uint32_t w[sizeof(E)];
+  };
+  __device__ __forceinline__ Raw4 fetch(int64_t i, int64_t c, int64_t cols) const {
+    const E* row = i < lines ? p + i * ld : p2 + (i - lines) * ld2;
+    if (c + 4 <= cols) return __builtin_bit_cast(Raw4, load_pack<E, 4>(row + c));
+    Pack<E, 4> v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.v[e] = c + e < cols ? ldg(row + c + e) : static_cast<E>(0.f);
+    return __builtin_bit_cast(Raw4, v);
+  }
+  __device__ __forceinline__ void of(const Raw4& r, float (&v)[4]) const {
+    const Pack<E, 4> q = __builtin_bit_cast(Pack<E, 4>, r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(q.v[e]);
   }
 };
 
-// EXT rows of an operand for one k-step: EXT / 8 floats per lane.  T: its lines are k, else rows.
+// EXT rows of an operand for one k-step: EXT / 8 elements per lane.  T: its lines are k, else rows.
 template <class Src, bool T, int EXT>
 struct DirectLoader {
   static constexpr int VECS = EXT / 32;  // vectors of four elements per lane
   const Src& src;
   int64_t rows, K;
-  float v[VECS][4];
+  typename Src::Raw4 raw[VECS];
 
   __device__ __forceinline__ DirectLoader(const Src& s, int64_t r, int64_t k) : src(s), rows(r), K(k) {}
   __device__ __forceinline__ void load(int64_t row0, int64_t k0) {
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int q = i * 256 + threadIdx.x;
-      const int64_t line = T ? k0 + q / (EXT / 4) : row0 + q / 8;
-      if (line < (T ? K : rows)) src.read(line, T ? row0 + q % (EXT / 4) * 4 : k0 + q % 8 * 4, T ? rows : K, v[i]);
-      else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+      const int64_t line = T ? k0 + q / (EXT / 4) : row0 + q / 8, c = T ? row0 + q % (EXT / 4) * 4 : k0 + q % 8 * 4;
+      raw[i] = typename Src::Raw4{};
+      if (line < (T ? K : rows)) raw[i] = src.fetch(line, c, T ? rows : K);
     }
   }
   __device__ __forceinline__ void store(float* image) const {
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int q = i * 256 + threadIdx.x;
+      float v[4];
+      src.of(raw[i], v);
       if constexpr (!T) {
-        *reinterpret_cast<f4*>(image + q / 8 * kDirectPitch + q % 8 * 4) = f4{v[i][0], v[i][1], v[i][2], v[i][3]};
+        *reinterpret_cast<f4*>(image + q / 8 * kDirectPitch + q % 8 * 4) = f4{v[0], v[1], v[2], v[3]};
       } else {
         float* to = image + q % (EXT / 4) * 4 * kDirectPitch + q / (EXT / 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[e * kDirectPitch] = v[i][e];
+        for (int e = 0; e < 4; ++e) to[e * kDirectPitch] = v[e];
       }
     }
   }

@@ -314,36 +314,51 @@ struct GatedGrad {
   int64_t units;
   int act;
 
-  template <int ACT>
-  static __device__ __forceinline__ float one(float g, float u, float d, bool second) {
-    float a, da;
-    activation<ACT>(g, &a, &da);
-    return second ? d * a : d * u * da;
-  }
-  __device__ __forceinline__ void read(int64_t t, int64_t c, int64_t cols, float (&v)[4]) const {
-    with_activation(act, [&](auto kind) { read_as<decltype(kind)::value>(t, c, v); });
-  }
-  template <int ACT>
-  __device__ __forceinline__ void read_as(int64_t t, int64_t c, float (&v)[4]) const {
+  struct Raw4 {
+    float g[4], u[4];
+    uint32_t d[sizeof(T)];
+    int first;  // how many of the four are dg's, the others du's
+  };
+  __device__ __forceinline__ Raw4 fetch(int64_t t, int64_t c, int64_t) const {
     const float *gr = gate + t * units, *ur = up + t * units;
     const T* dr = dh + t * lddh;
-    const bool second = c >= units;
-    const int64_t n = second ? c - units : c;
+    Raw4 r;
+    const int64_t n = c >= units ? c - units : c;
     if (n + 4 <= units) {
-      float g[4], u[4], d[4];
-      load_row<float, 4>(gr, n, units, g);
-      load_row<float, 4>(ur, n, units, u);
-      load_row<T, 4>(dr, n, units, d);
+      const Pack<float, 4> g = load_pack<float, 4>(gr + n), u = load_pack<float, 4>(ur + n);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = one<ACT>(g[e], u[e], d[e], second);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // from dg into du, or past both
-        const bool s = c + e >= units;
-        const int64_t m = s ? c + e - units : c + e;
-        v[e] = m < units ? one<ACT>(ldg(gr + m), ldg(ur + m), static_cast<float>(ldg(dr + m)), s) : 0.f;
-      }
+      for (int e = 0; e < 4; ++e) r.g[e] = g.v[e], r.u[e] = u.v[e];
+      const Pack<T, 4> d = load_pack<T, 4>(dr + n);
+      __builtin_memcpy(r.d, &d, sizeof(d));
+      r.first = c >= units ? 0 : 4;
+      return r;
     }
+    // from dg into du, or past both: zeros, of which 0 is made
+    Pack<T, 4> d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t m = c + e >= units ? c + e - units : c + e;
+      const bool in = m < units;
+      r.g[e] = in ? ldg(gr + m) : 0.f;
+      r.u[e] = in ? ldg(ur + m) : 0.f;
+      d.v[e] = in ? ldg(dr + m) : static_cast<T>(0.f);
+    }
+    __builtin_memcpy(r.d, &d, sizeof(d));
+    r.first = c >= units ? 0 : static_cast<int>(units - c);
+    return r;
+  }
+  __device__ __forceinline__ void of(const Raw4& r, float (&v)[4]) const {
+    Pack<T, 4> d;
+    __builtin_memcpy(&d, r.d, sizeof(d));
+    with_activation(act, [&](auto kind) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = static_cast<float>(d.v[e]);
+        float a, da;
+        activation<decltype(kind)::value>(r.g[e], &a, &da);
+        v[e] = e < r.first ? x * r.u[e] * da : x * a;
+      }
+    });
   }
 };
 

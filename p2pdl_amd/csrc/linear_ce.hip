@@ -387,13 +387,22 @@ struct CeGrad {
   const int64_t* target;
   int64_t ignore;
 
-  __device__ __forceinline__ void read(int64_t t, int64_t n, int64_t cols, float (&v)[4]) const {
+  struct Raw4 {
+    float z[4], l;
+    int at, in;  // the target among the four; how many of them are classes (0: the token does not count)
+  };
+  __device__ __forceinline__ Raw4 fetch(int64_t t, int64_t n, int64_t) const {
+    Raw4 r;
     const int64_t y = ldg(target + t);
-    const float l = y >= 0 && y < V ? ldg(lse + t) : NAN;
-    float z[4];
-    sum_runs<4>(parts + t * V, T * V, runs, n, V, z);
+    r.l = y >= 0 && y < V ? ldg(lse + t) : NAN;
+    sum_runs<4>(parts + t * V, T * V, runs, n, V, r.z);
+    r.at = y >= n && y < n + 4 ? static_cast<int>(y - n) : -1;
+    r.in = y == ignore || n >= V ? 0 : static_cast<int>(V - n < 4 ? V - n : 4);
+    return r;
+  }
+  __device__ __forceinline__ void of(const Raw4& r, float (&v)[4]) const {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = y == ignore || n + e >= V ? 0.f : expf(z[e] - l) - (n + e == y ? 1.f : 0.f);
+    for (int e = 0; e < 4; ++e) v[e] = e < r.in ? expf(r.z[e] - r.l) - (e == r.at ? 1.f : 0.f) : 0.f;
   }
 };
 
