@@ -6,8 +6,9 @@
 // four v_mfma_f32_16x16x4_f32; the order of k within a step is the same for both
 // operands.  The next step's elements are on their way to registers while
 // this one's are multiplied (two steps ahead cost the fourth block of a CU its
-// registers: 1024 x 1024 x 1024 float32 loss backward 98 us, 114); four blocks share a CU.  Few tiles are cut along
-// k into runs, their sums joined in run order by the caller.
+// registers: 1024 x 1024 x 1024 float32 loss backward 98 us, 114); four blocks
+// share a CU.  Few tiles are cut along k into runs, their sums joined in run
+// order by the caller.
 #pragma once
 #include "direct.h"
 

@@ -124,7 +124,7 @@ __global__ __launch_bounds__(kLnFwdBlock < TEAM ? TEAM : kLnFwdBlock) void layer
 // row of 2 * cols sums: dw, then db.  The next row's x and dy are requested
 // before this one is worked on (rows of up to 4096) and rows are held as they
 // lie, two registers per four 16-bit elements, so that two blocks fit a CU:
-// 16384 x 4096 bf16 in 143.6 us without either, 91 us (4.4 TB/s) with.
+// 16384 x 4096 bf16 in 143.6 us without either, 84 us (4.8 TB/s) with.
 template <typename T, int TEAM, int NV, Fit FIT>
 __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void layernorm_bwd_kernel(
     const T* dy, int64_t lddy, const T* x, int64_t ldx, const T* w, const float* mean_in, const float* rstd_in, int64_t rows,
