@@ -27,14 +27,17 @@ struct DirectArgs {
 // 256 x 1024 53 / 46.  Loss, float32: 1024 x 1024 x 1024 136 / 246, 1024 x 1024 x
 // 2048 239 / 271, 1500 x 1500 x 1500 448 / 349; bfloat16: 128 x 512 x 1000 49 / 61,
 // 200 x 512 x 1000 61 / 62, 512 x 256 x 1024 61 / 61.  Up to 64 rows 16-bit tiles are
-// half empty: 64 x 1001 x 3001 float16 loss 70 / 78, gated layer 25 x 2119 x 1210 52 / 74,
-// 32 x 1024 x 4096 bfloat16 53 / 47.  Float32 pays for copies of all of B besides:
-// 16 x 4096 x 8192 232 / 794.  Up to 2^24 rows and columns: its tiles and the rows of
-// its epilogues then fit one dimension of a grid.
+// half empty: 64 x 1001 x 3001 float16 loss 70 / 78.  Up to 32 rows the time of either
+// is the weight's: loss 16 x 1024 x 4096 47 / 62, 2 x 2048 x 8192 84 / 92, 4 x 512 x 32000
+// 84 / 84, 1 x 1024 x 32000 136 / 106; gated layer 25 x 2119 x 1210 float16 45 / 74, 8 x 1024 x
+// 4096 42 / 44, 2 x 2048 x 8192 105 / 81, 1 x 4096 x 11008 258 / 195.  Float32 pays for
+// copies of all of B besides: 16 x 4096 x 8192 210 / 794.  Up to 2^24 rows and columns:
+// its tiles and the rows of its epilogues then fit one dimension of a grid.
 static inline bool direct_pays(int64_t M, int64_t N, int64_t K, int32_t dtype) {
-  const double size = static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+  const double weight = static_cast<double>(N) * static_cast<double>(K), size = static_cast<double>(M) * weight;
   if (M > 1 << 24 || N > 1 << 24) return false;
-  return dtype == P2P_DTYPE_F32 ? M <= 128 || size <= 2.6e9 : size <= (M <= 64 ? 2.0e8 : 1.0e8);
+  if (dtype == P2P_DTYPE_F32) return M <= 128 || size <= 2.6e9;
+  return M <= 32 ? weight <= 2.0e7 : size <= (M <= 64 ? 2.0e8 : 1.0e8);
 }
 // Its k-runs, at least two k-steps each.  The forward pass joins them anyway:
 // blocks for every CU four times, up to as many runs as a lane's loads take at
