@@ -21,23 +21,23 @@ struct DirectArgs {
 
 // Whether a product of this size (N of the gated layer: 2 units) goes this
 // way.  Forward and backward together, direct / tiles, us.  Gated layer,
-// float32 (three planes in tiles): 1024 x 1024 x 512 103 / 168, 800 x 1024 x 1024
-// 160 / 186, 1024 x 1024 x 1024 174 / 200, 1024 x 1024 x 2048 341 / 244; bfloat16:
-// 256 x 256 x 512 32 / 41, 90 x 512 x 1000 36 / 42, 128 x 512 x 1000 46 / 43, 512 x
-// 256 x 1024 53 / 46.  Loss, float32: 1024 x 1024 x 1024 136 / 246, 1024 x 1024 x
-// 2048 239 / 271, 1500 x 1500 x 1500 448 / 349; bfloat16: 128 x 512 x 1000 49 / 61,
-// 200 x 512 x 1000 61 / 62, 512 x 256 x 1024 61 / 61.  Up to 64 rows 16-bit tiles are
-// half empty: 64 x 1001 x 3001 float16 loss 70 / 78.  Up to 32 rows the time of either
-// is the weight's: loss 16 x 1024 x 4096 47 / 62, 2 x 2048 x 8192 84 / 92, 4 x 512 x 32000
-// 84 / 84, 1 x 1024 x 32000 136 / 106; gated layer 25 x 2119 x 1210 float16 45 / 74, 8 x 1024 x
-// 4096 42 / 44, 2 x 2048 x 8192 105 / 81, 1 x 4096 x 11008 258 / 195.  Float32 pays for
-// copies of all of B besides: 16 x 4096 x 8192 210 / 794.  Up to 2^24 rows and columns:
-// its tiles and the rows of its epilogues then fit one dimension of a grid.
+// float32 (three planes in tiles): 1024 x 1024 x 512 105 / 108, 512 x 1024 x 1024
+// 101 / 112, 632 x 1800 x 873 195 / 164, 1024 x 1024 x 1024 180 / 147; bfloat16: 256 x
+// 256 x 512 32 / 38, 90 x 512 x 1000 34 / 40, 512 x 256 x 1024 53 / 46.  Loss, float32:
+// 632 x 1800 x 873 151 / 155, 1024 x 1024 x 1024 143 / 149, 384 x 1128 x 4734 259 / 215,
+// 4040 x 1560 x 389 328 / 242; bfloat16: 128 x 512 x 1000 49 / 57, 200 x 512 x 1000 61 /
+// 62, 512 x 256 x 1024 61 / 61.  Up to 64 rows 16-bit tiles are half empty: 64 x 1001
+// x 3001 loss 66 / 76.  Up to 32 rows the time of either is the weight's: loss 16 x 1024
+// x 4096 47 / 58, 8 x 2048 x 4096 60 / 60, 2 x 2048 x 8192 83 / 66; gated layer 25 x 2119 x
+// 1210 45 / 62, 16 x 1024 x 4096 43 / 43, 8 x 2048 x 4096 63 / 51.  Float32 pays for copies of
+// all of B besides, whatever the weight up to 128 rows: loss 128 x 4096 x 4096 226 / 258, 64
+// x 512 x 32000 136 / 303.  Up to 2^24 rows and columns: its tiles and the rows of its
+// epilogues then fit one dimension of a grid.
 static inline bool direct_pays(int64_t M, int64_t N, int64_t K, int32_t dtype) {
   const double weight = static_cast<double>(N) * static_cast<double>(K), size = static_cast<double>(M) * weight;
   if (M > 1 << 24 || N > 1 << 24) return false;
-  if (dtype == P2P_DTYPE_F32) return M <= 128 || size <= 2.6e9;
-  return M <= 32 ? weight <= 2.0e7 : size <= (M <= 64 ? 2.0e8 : 1.0e8);
+  if (dtype == P2P_DTYPE_F32) return M <= 128 || size <= 1.3e9;
+  return M <= 32 ? weight <= 9.0e6 : size <= (M <= 64 ? 2.0e8 : 1.0e8);
 }
 // Its k-runs, at least two k-steps each.  The forward pass joins them anyway:
 // blocks for every CU four times, up to as many runs as a lane's loads take at

@@ -116,6 +116,20 @@ struct GatedEpi {
   }
 };
 
+// The k-runs' g and u instead, [runs][T, 2 units] (the tile's columns: 16 units' g, then their u).
+struct GatedPartEpi {
+  float* partial;
+  int64_t units;
+
+  template <class Cfg>
+  __device__ __forceinline__ void finish(f4 (&acc)[Cfg::MI][Cfg::NJ], const Place& p, const GemmArgs& g, char* lds) const {
+    by_rows<Cfg>(acc, p, lds, [&](int, int64_t m, int64_t n, f4 v) {
+      const int64_t unit = n / 32 * 16 + n % 16;
+      if (m < g.M && unit < units) store4(partial + ((p.part * g.M + m) * 2 + n / 16 % 2) * units, unit, units, v);
+    });
+  }
+};
+
 // dg and du of 8 units per lane, into d [T, 2 * pitch]: dg, then du, zeros
 // in the columns past `units`; plane: elements from one plane to the next.
 // DIRECT: as float, with no columns past `units` (pitch == units).
@@ -176,7 +190,7 @@ static int32_t gated_grad(const p2p_gated_linear_t& a, int64_t pitch, uint16_t* 
   return launch_status();
 }
 
-// The direct product's runs [runs][T, 2 units] joined; gate, up and h.
+// A product's runs [runs][T, 2 units] joined; gate, up and h.
 __global__ __launch_bounds__(kBlock) void gated_join_kernel(const float* parts, int runs, int64_t rows, int64_t units, int act,
                                                             void* h, int32_t dtype, float* gate, float* up) {
   const int64_t per_row = (units + 3) / 4, all = rows * per_row;
@@ -213,6 +227,15 @@ static int32_t gated_check(const p2p_gated_linear_t* a) {
   const int s = dtype_bytes(a->dtype);
   if (!aligned_to(a->x, s) || !aligned_to(a->w_gate, s) || !aligned_to(a->w_up, s)) return P2P_ERR_ALIGN;
   return P2P_OK;
+}
+
+// The forward product's tile and runs: few tiles over a long sum are cut along k (their sums at most half a gigabyte),
+// joined and activated by the small product's kernel (whole / in runs, us: 64 x 4096 x 4096 bfloat16 47.4 / 24.1, 512 x
+// 4096 x 1024 49.0 / 26.0, 256 x 2048 x 2048 28.6 / 22.6, 512 x 4096 x 2048 float32 285 / 133).
+static Plan gated_fwd_plan(const p2p_gated_linear_t& a) {
+  const int64_t steps = ksteps(a.hidden, a.dtype == P2P_DTYPE_F32 ? 6 : 1);
+  const Plan p = gemm_plan(a.tokens, 2 * a.units, steps, true);
+  return p.split * a.tokens * 2 * a.units * 4 <= int64_t(512) << 20 ? p : gemm_plan(a.tokens, 2 * a.units, steps, false);
 }
 
 // The workspace, in the order in which both passes carve it.
@@ -269,7 +292,10 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
   }
   s->d = nullptr;
   s->parts = s->dx_parts = nullptr;
-  if (backward) {
+  if (!backward) {
+    const int64_t split = gated_fwd_plan(a).split;
+    if (split > 1) s->parts = static_cast<float*>(c.take(split * a.tokens * 2 * a.units * 4));
+  } else {
     const int64_t rows2 = 2 * gated_pitch(a);
     s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 2 * planes_of(a.dtype)));
     const Plan px = gated_dx_plan(a), pw = gated_dw_plan(a);
@@ -292,16 +318,19 @@ static int32_t gated_operands(const p2p_gated_linear_t& a, const GatedSpace& s, 
   return pack_matrices(jobs, 3, a.dtype, st);
 }
 
+static int32_t gated_join(const p2p_gated_linear_t& a, const GatedSpace& s, int split, hipStream_t st) {
+  const int64_t blocks = ceil_div(a.tokens * ceil_div(a.units, 4), kBlock);
+  gated_join_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
+      s.parts, split, a.tokens, a.units, a.activation, a.h, a.dtype, a.gate, a.up);
+  return launch_status();
+}
+
 static int32_t gated_direct_fwd(const p2p_gated_linear_t& a, const GatedSpace& s, hipStream_t st) {
   const int split = direct_split(a.tokens, 2 * a.units, a.hidden, true);
   const DirectArgs g{a.x, a.w_gate, a.w_up, a.ldx, a.ldg, a.ldu, a.units, a.tokens, 2 * a.units, a.hidden, split,
                      {nullptr, nullptr}, INT64_MAX, {nullptr, nullptr}, s.parts};
   const int32_t rc = direct_product(g, a.dtype, st);
-  if (rc != P2P_OK) return rc;
-  const int64_t blocks = ceil_div(a.tokens * ceil_div(a.units, 4), kBlock);
-  gated_join_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
-      s.parts, split, a.tokens, a.units, a.activation, a.h, a.dtype, a.gate, a.up);
-  return launch_status();
+  return rc == P2P_OK ? gated_join(a, s, split, st) : rc;
 }
 
 // [dg du] of a token, made where the gradients' products read it (again for
@@ -413,10 +442,13 @@ extern "C" int32_t p2p_gated_linear_fwd(const p2p_gated_linear_t* a, void* works
   add_pairs(&g, x, wg, &wu, a->dtype);
   g.lda = x.ld, g.ldb = wg.ld;
   g.M = a->tokens, g.N = 2 * a->units, g.K = a->hidden;
-  g.ksplit = 1;
-  const GatedEpi epi{a->h, a->gate, a->up, a->units, a->dtype, a->activation};
-  const bool big = gemm_plan(g.M, g.N, ksteps(g.K, g.nseg), false).big;
-  return gemm_launch<false, false, true>(g, a->dtype == P2P_DTYPE_F16, big, epi, st);
+  const Plan plan = gated_fwd_plan(*a);
+  g.ksplit = plan.split;
+  const bool f16_ = a->dtype == P2P_DTYPE_F16;
+  if (plan.split == 1)
+    return gemm_launch<false, false, true>(g, f16_, plan.big, GatedEpi{a->h, a->gate, a->up, a->units, a->dtype, a->activation}, st);
+  rc = gemm_launch<false, false, true>(g, f16_, plan.big, GatedPartEpi{s.parts, a->units}, st);
+  return rc == P2P_OK ? gated_join(*a, s, plan.split, st) : rc;
 }
 
 extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* workspace, int64_t workspace_bytes,

@@ -216,6 +216,24 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* part, int t
   }
 }
 
+// Four values of d as operands of type T: float32 in planes `plane` elements apart, float16 times kHalfScale.
+template <typename T>
+__device__ __forceinline__ void store_d(uint16_t* to, int64_t plane, f4 x) {
+  if constexpr (sizeof(T) == 4) {
+    Pack<uint16_t, 4> o[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Planes s = split3(x[e]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) o[q].v[e] = s.p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) store_pack<uint16_t, 4>(to + q * plane, o[q]);
+  } else {
+    store4(reinterpret_cast<T*>(to), 0, 4, std::is_same_v<T, f16> ? x * kHalfScale : x);
+  }
+}
+
 // d of a piece into its buffer [T, pitch] (planes `plane` elements apart).
 struct GradEpi {
   uint16_t* d;
@@ -245,23 +263,9 @@ struct GradEpi {
       });
     };
     const auto fast = [](float x) { return __expf(x); };
-    if (dtype == P2P_DTYPE_F32) {
-      rows([](float x) { return expf(x); }, [&](uint16_t* to, f4 x) {
-        Pack<uint16_t, 4> o[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const Planes s = split3(x[e]);
-#pragma unroll
-          for (int q = 0; q < 3; ++q) o[q].v[e] = s.p[q];
-        }
-#pragma unroll
-        for (int q = 0; q < 3; ++q) store_pack<uint16_t, 4>(to + q * plane, o[q]);
-      });
-    } else if (dtype == P2P_DTYPE_F16) {
-      rows(fast, [](uint16_t* to, f4 x) { store4(reinterpret_cast<f16*>(to), 0, 4, x * kHalfScale); });
-    } else {
-      rows(fast, [](uint16_t* to, f4 x) { store4(reinterpret_cast<bf16*>(to), 0, 4, x); });
-    }
+    if (dtype == P2P_DTYPE_F32) rows([](float x) { return expf(x); }, [&](uint16_t* to, f4 x) { store_d<float>(to, plane, x); });
+    else if (dtype == P2P_DTYPE_F16) rows(fast, [&](uint16_t* to, f4 x) { store_d<f16>(to, plane, x); });
+    else rows(fast, [&](uint16_t* to, f4 x) { store_d<bf16>(to, plane, x); });
   }
 };
 
@@ -377,6 +381,28 @@ __global__ __launch_bounds__(kBlock) void ce_grad_kernel(float* parts, int runs,
   }
 }
 
+// d as the tiles' gradient products read it: T, or three planes, [T, pitch], zeros past the last class.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void ce_d_kernel(const float* parts, int runs, int64_t tokens, int64_t V, const float* lse,
+                                                      const int64_t* target, int64_t ignore, uint16_t* d, int64_t pitch,
+                                                      int64_t plane) {
+  const int64_t per_row = pitch / 4, all = tokens * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
+       i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t t = i / per_row, n = (i - t * per_row) * 4;
+    const int64_t y = ldg(target + t);
+    const float l = y >= 0 && y < V ? ldg(lse + t) : NAN;
+    f4 x = {0.f, 0.f, 0.f, 0.f};
+    if (n < V && y != ignore) {
+      float z[4];
+      sum_runs<4>(parts + t * V, tokens * V, runs, n, V, z);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = n + e < V ? expf(z[e] - l) - (n + e == y ? 1.f : 0.f) : 0.f;
+    }
+    store_d<T>(d + t * pitch + n, plane, x);
+  }
+}
+
 // The same, made where the gradients' products read it (again for every 64
 // columns of x, against a launch).
 struct CeGrad {
@@ -426,6 +452,8 @@ struct CeSpace {
   // forward
   float2 *part, *state;
   float *at_target, *row_loss;
+  float* z;           // few tiles: the logits in k-runs
+  Plan z_plan;
   // backward
   uint16_t* d;
   float* dx_parts;
@@ -449,6 +477,21 @@ static bool ce_chunked(const p2p_linear_ce_t& a) { return a.tokens <= 64 && a.vo
 static bool ce_made_in_place(const p2p_linear_ce_t& a) {
   return static_cast<double>(a.tokens) * static_cast<double>(a.vocab) * static_cast<double>(a.hidden) <= 8.0e6;
 }
+// The logits' tile and runs.  Few tiles over a long sum are cut along k like the gradients; the runs are joined by the
+// kernel that reduces a token's row (forward) or makes d (backward).  Forward, whole / in runs, us: 64 x 4096 x 4096
+// bfloat16 52.6 / 24.6, 512 x 4096 x 1024 54.3 / 28.4, 1298 x 3618 x 920 60.1 / 41.8, 512 x 4096 x 2048 float32 274 / 95.
+static Plan ce_logits_plan(const p2p_linear_ce_t& a, int64_t piece) {
+  const int64_t steps = ksteps(a.hidden, a.dtype == P2P_DTYPE_F32 ? 6 : 1);
+  const Plan p = gemm_plan(a.tokens, piece, steps, piece == a.vocab);
+  return p.split * a.tokens * piece * 4 <= kPieceBytes ? p : gemm_plan(a.tokens, piece, steps, false);
+}
+// What the reduction of rows of logits needs besides them.
+static void ce_take_rows(const p2p_linear_ce_t& a, Carver* c, CeSpace* s) {
+  s->row_loss = static_cast<float*>(c->take(a.tokens * 4));
+  if (!ce_chunked(a)) return;
+  s->part = static_cast<float2*>(c->take(ceil_div(a.vocab, kChunk) * a.tokens * 8));
+  s->at_target = static_cast<float*>(c->take(a.tokens * 4));
+}
 static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeSpace* s) {
   Carver c{static_cast<char*>(base)};
   if (ce_direct(a)) {
@@ -456,11 +499,7 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
     const int64_t runs = direct_split(a.tokens, a.vocab, a.hidden, true);
     s->d = static_cast<uint16_t*>(c.take(runs * a.tokens * a.vocab * 4));
     if (!backward) {
-      s->row_loss = static_cast<float*>(c.take(a.tokens * 4));
-      if (ce_chunked(a)) {
-        s->part = static_cast<float2*>(c.take(ceil_div(a.vocab, kChunk) * a.tokens * 8));
-        s->at_target = static_cast<float*>(c.take(a.tokens * 4));
-      }
+      ce_take_rows(a, &c, s);
       return c.used;
     }
     const int64_t sx = direct_split(a.tokens, a.hidden, a.vocab, false), sw = direct_split(a.vocab, a.hidden, a.tokens, false);
@@ -479,6 +518,13 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
   s->piece = piece;
   s->x = x_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(a.tokens, a.hidden, a.dtype)));
   s->w = w_here ? nullptr : static_cast<uint16_t*>(c.take(packed_bytes(piece, a.hidden, a.dtype)));
+  s->z_plan = ce_logits_plan(a, piece);
+  s->z = s->z_plan.split > 1 ? static_cast<float*>(c.take(s->z_plan.split * a.tokens * a.vocab * 4)) : nullptr;
+  if (s->z && !backward) {
+    s->part = nullptr;
+    ce_take_rows(a, &c, s);
+    return c.used;
+  }
   if (!backward) {
     s->part = static_cast<float2*>(c.take(ceil_div(piece, Small::BN) * a.tokens * 8));
     s->state = static_cast<float2*>(c.take(a.tokens * 8));
@@ -521,11 +567,9 @@ static int32_t ce_direct_logits(const p2p_linear_ce_t& a, const CeSpace& s, int*
   return direct_product(g, a.dtype, st);
 }
 
-static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStream_t st) {
-  int runs;
-  int32_t rc = ce_direct_logits(a, s, &runs, st);
-  if (rc != P2P_OK) return rc;
-  const float* z = reinterpret_cast<const float*>(s.d);
+// lse and the loss out of the logits in k-runs.
+static int32_t ce_rows(const p2p_linear_ce_t& a, const CeSpace& s, const float* z, int runs, hipStream_t st) {
+  int32_t rc;
   if (ce_chunked(a)) {
     const int chunks = static_cast<int>(ceil_div(a.vocab, kChunk));
     ce_chunk_kernel<<<dim3(chunks, static_cast<unsigned>(a.tokens)), dim3(256), 0, st>>>(z, runs, a.tokens, a.vocab, a.target,
@@ -545,6 +589,30 @@ static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStre
   kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, st>>>(z, runs, a.vocab, a.lse, s.row_loss, ce_out(a));
   if ((rc = launch_status()) != P2P_OK || (blocks == 1 && a.tokens <= kAloneTokens)) return rc;
   ce_loss_kernel<<<dim3(1), dim3(1024), 0, st>>>(s.row_loss, ce_out(a));
+  return launch_status();
+}
+
+static int32_t ce_direct_fwd(const p2p_linear_ce_t& a, const CeSpace& s, hipStream_t st) {
+  int runs;
+  const int32_t rc = ce_direct_logits(a, s, &runs, st);
+  return rc == P2P_OK ? ce_rows(a, s, reinterpret_cast<const float*>(s.d), runs, st) : rc;
+}
+
+// The logits of all classes in k-runs, by tiles.
+static int32_t ce_tile_logits(const p2p_linear_ce_t& a, const CeSpace& s, const Mat& x, const Mat& w, hipStream_t st) {
+  GemmArgs g{};
+  add_pairs(&g, x, w, nullptr, a.dtype);
+  g.lda = x.ld, g.ldb = w.ld;
+  g.M = a.tokens, g.N = a.vocab, g.K = a.hidden;
+  g.ksplit = s.z_plan.split;
+  const StoreEpi e{{nullptr, nullptr}, 0, 0, a.vocab, a.dtype, {nullptr, nullptr}, 1.f, s.z, 0};
+  return gemm_launch<false, false, false>(g, a.dtype == P2P_DTYPE_F16, s.z_plan.big, e, st);
+}
+template <typename T>
+static int32_t ce_tile_d(const p2p_linear_ce_t& a, const CeSpace& s, int64_t pitch, int64_t plane, hipStream_t st) {
+  const int64_t blocks = ceil_div(a.tokens * (pitch / 4), kBlock);
+  ce_d_kernel<T><<<dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * 32))), dim3(kBlock), 0, st>>>(
+      s.z, s.z_plan.split, a.tokens, a.vocab, a.lse, a.target, a.ignore_index, s.d, pitch, plane);
   return launch_status();
 }
 
@@ -607,6 +675,11 @@ extern "C" int32_t p2p_linear_ce_fwd(const p2p_linear_ce_t* a, void* workspace, 
   if (!aligned_to(workspace, 16)) return P2P_ERR_ALIGN;
   if (ce_direct(*a)) return ce_direct_fwd(*a, s, st);
   Mat x, w;
+  if (s.z) {
+    if ((rc = ce_operands(*a, s, 0, a->vocab, &x, &w, st)) != P2P_OK) return rc;
+    if ((rc = ce_tile_logits(*a, s, x, w, st)) != P2P_OK) return rc;
+    return ce_rows(*a, s, s.z, s.z_plan.split, st);
+  }
   for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
     const int64_t rows = std::min(s.piece, a->vocab - v0);
     if ((rc = ce_operands(*a, s, v0, rows, &x, &w, st)) != P2P_OK) return rc;
@@ -648,7 +721,13 @@ extern "C" int32_t p2p_linear_ce_bwd(const p2p_linear_ce_t* a, void* workspace, 
   for (int64_t v0 = 0; v0 < a->vocab; v0 += s.piece) {
     const int64_t rows = std::min(s.piece, a->vocab - v0), pitch = line_pitch(rows), plane = a->tokens * pitch;
     if ((rc = ce_operands(*a, s, v0, rows, &x, &w, st)) != P2P_OK) return rc;
-    {
+    if (s.z) {
+      if ((rc = ce_tile_logits(*a, s, x, w, st)) != P2P_OK) return rc;
+      rc = a->dtype == P2P_DTYPE_F32 ? ce_tile_d<float>(*a, s, pitch, plane, st)
+           : f16_                    ? ce_tile_d<f16>(*a, s, pitch, plane, st)
+                                     : ce_tile_d<bf16>(*a, s, pitch, plane, st);
+      if (rc != P2P_OK) return rc;
+    } else {
       GemmArgs g{};
       add_pairs(&g, x, w, nullptr, a->dtype);
       g.lda = x.ld, g.ldb = w.ld;

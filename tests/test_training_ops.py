@@ -888,6 +888,25 @@ def test_linear_cross_entropy_long_rows_targets(cuda, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,rows,cols,units", [(torch.bfloat16, 200, 4000, 520), (torch.float16, 201, 3999, 517), (torch.bfloat16, 70, 3001, 1030),
+                                                   (torch.float32, 300, 9000, 1100), (torch.float32, 301, 8999, 1001)])
+def test_forward_in_runs(cuda, dtype, rows, cols, units):
+    """Few tiles over a long sum: the forward products cut along k."""
+    a, keep = T._ce_args(torch.empty(rows, cols, dtype=dtype, device="cuda"), torch.empty(units, cols, dtype=dtype, device="cuda"),
+                         torch.zeros(rows, dtype=torch.int64, device="cuda"), -100)
+    a.lse = a.norm = a.x
+    assert N.lib().p2p_linear_ce_workspace(a, 0) >= 2 * 4 * rows * units  # two runs of logits at least
+    test_gated_linear(cuda, dtype, rows, cols, units, "silu")
+    test_linear_cross_entropy(cuda, dtype, rows, cols, units, "mean")
+
+
+@gpu
+@pytest.mark.parametrize("dtype,cols", [(torch.bfloat16, 6000), (torch.float16, 5999)])
+def test_linear_cross_entropy_long_rows_in_runs(cuda, dtype, cols):
+    test_linear_cross_entropy(cuda, dtype, 40, cols, 5001, "sum")
+
+
+@gpu
 def test_long_sums_of_few_tiles(cuda):
     """Float32 on small tiles, the sum cut into runs in both gradients."""
     test_gated_linear_large_tiles(cuda, torch.float32, 200, 36000, 200)
