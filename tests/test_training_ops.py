@@ -929,6 +929,24 @@ def test_linear_cross_entropy_copied_pieces(cuda):
 
 
 @gpu
+def test_linear_cross_entropy_copied_pieces_on_tiles(cuda):
+    """The same with more rows, on tiles, forward and backward: float32 and float16 rows of an odd length."""
+    for rows, cols, vocab, dtype in ((260, 1000, 90000, torch.float32), (70, 1001, 280000, torch.float16)):
+        x, w, t = ce_inputs(rows, cols, vocab, dtype, 120)
+        a, keep = T._ce_args(x, w, t, -100)
+        a.lse = a.norm = x.data_ptr()
+        whole = vocab * cols * (6 if dtype == torch.float32 else 2)
+        assert N.lib().p2p_linear_ce_workspace(a, 0) < whole  # fewer bytes than the copy of all of w: equal pieces of it
+        loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+        dloss = torch.tensor(8.0 * rows, device="cuda")
+        got = T.linear_cross_entropy_backward(x, w, t, lse, norm, dloss)
+        want, err = ce_reference(x, w, t, 8.0 * rows, -100, "mean")
+        check(loss, want[0], rounded(want[0], err[0], torch.float32), "loss")
+        for o, v, e, name in zip(got, want[1:], err[1:], ("dx", "dw")):
+            check(o, v, rounded(v, e, dtype), name)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_tiled_layouts(cuda, dtype):
     """Pitches, bases at any element and strides on tiles: the bits of the dense call."""
