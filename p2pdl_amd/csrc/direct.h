@@ -32,8 +32,9 @@ struct DirectArgs {
 // 1210 45 / 62, 16 x 1024 x 4096 43 / 43, 8 x 2048 x 4096 63 / 51; rows that tiles have to
 // copy first: loss 2 x 258 x 91984 float16 130 / 200.  Float32 pays for copies of
 // all of B besides, whatever the weight up to 192 rows: loss 64 x 512 x 32000 136 / 303, 128
-// x 4096 x 4096 226 / 258, 192 x 1024 x 8192 182 / 189, 256 x 1024 x 8192 231 / 205.  Up to 2^24 rows and columns: its tiles and the rows of its
-// epilogues then fit one dimension of a grid.
+// x 4096 x 4096 226 / 258, 192 x 1024 x 8192 182 / 189, 256 x 1024 x 8192 231 / 205.
+// Up to 2^24 rows and columns: its tiles and the rows of its epilogues then fit one
+// dimension of a grid.
 static inline bool direct_pays(int64_t M, int64_t N, int64_t K, int32_t dtype) {
   const double weight = static_cast<double>(N) * static_cast<double>(K), size = static_cast<double>(M) * weight;
   if (M > 1 << 24 || N > 1 << 24) return false;
