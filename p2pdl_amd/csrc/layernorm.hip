@@ -178,10 +178,12 @@ __global__ __launch_bounds__(kLnBwdBlock, NV * Vec16<T>::N <= 8 ? 4 : 2) void la
     for (int i = 0; i < NV; ++i) {
       const Span<T, FIT> p(i * TEAM + lane, have);
       forget(wv[i]);
+      // past the row x and dy are 0 and so is what they add to the sums, if h is: (0 - mean) * rstd may be an infinity
+      const float mi = p.in ? mu : 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        // past the row dy is 0, and what it adds to sums with it
-        const float h = (raw_at<T>(xc[i], e) - mu) * rs;
+        float h = (raw_at<T>(xc[i], e) - mi) * rs;
+        if (FIT == SHORT) h = p.counts(e, have) ? h : 0.f;
         const float d = raw_at<T>(gc[i], e);
         float g = w ? d * raw_at<T>(wv[i], e) : d;
         dwv[i][e] += d * h;
