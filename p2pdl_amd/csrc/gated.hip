@@ -18,6 +18,14 @@
 // three planes), lie side by side in one [T, 2F] buffer, and feed dx as two
 // segments of one sum and dWg, dWu as one product of 2F rows.
 //
+// float16 holds them times a power of two that brings the largest of the call
+// to [2^14, 2^15), taken back from the 32-bit sums: without it gradients near
+// 1e-6 lay among its subnormal numbers (off by 3% in dx and dW; 0 below
+// 3e-8) and those past 65504 became infinities, which sums in 32 bits do not.
+// What is below 2^-28 of the largest is off by up to 2^-39 of it.  The largest
+// one takes a pass of its own over gate, up and dh (10 bytes a unit; backward, without /
+// with it, us: 1023 x 1001 x 2731 70 / 80, 8192 x 4096 x 16384 3852 / 4097).
+//
 // Small layers take the product of direct.h instead, forward into
 // sums of k-runs that a second kernel joins and activates (forward and
 // backward of 32 x 512 x 512 float32 82 us on tiles, 21 so; 1 x 512 x 1000
@@ -130,13 +138,86 @@ struct GatedPartEpi {
   }
 };
 
+template <int ACT>
+__device__ __forceinline__ void unit_grads(float g, float u, float dh, float* dg, float* du) {
+  float a, da;
+  activation<ACT>(g, &a, &da);
+  *dg = dh * u * da;
+  *du = dh * a;
+}
+
+// float16's power of two.  `largest`: the bits of the largest finite |dg|, |du|
+// of each block (as unsigned numbers they order as the values do), joined by
+// every block that scales; factor: what the sums are multiplied by.
+struct GradScale {
+  uint32_t* largest;
+  float* factor;
+  int blocks;
+};
+constexpr int kScaleBlocks = 4 * kBlock;  // four of them per lane
+
+// The block's largest; every lane calls it.
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  __shared__ uint32_t waves[kBlock / 64];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = std::max<uint32_t>(m, __shfl_xor(m, o, 64));
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x / 64] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kBlock / 64; ++w) m = std::max(m, waves[w]);
+  return m;
+}
+
+template <int ACT>
+__global__ __launch_bounds__(kBlock) void gated_largest_kernel(const f16* dh, int64_t lddh, const float* gate, const float* up,
+                                                               int64_t rows, int64_t units, uint32_t* largest) {
+  const int64_t per_row = (units + 7) / 8, all = rows * per_row;
+  uint32_t m = 0;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
+       i += static_cast<int64_t>(gridDim.x) * kBlock) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    float g[8], u[8], dhv[8];
+    load_row<float, 8>(gate + r * units, c, units, g);
+    load_row<float, 8>(up + r * units, c, units, u);
+    load_row<f16, 8>(dh + r * lddh, c, units, dhv);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // (0 past the units: their dh is)
+      float dg, du;
+      unit_grads<ACT>(g[e], u[e], dhv[e], &dg, &du);
+      const uint32_t a = __float_as_uint(fabsf(dg)), b = __float_as_uint(fabsf(du));
+      m = std::max(m, a < 0x7f800000u ? a : 0u);
+      m = std::max(m, b < 0x7f800000u ? b : 0u);
+    }
+  }
+  m = block_max(m);
+  if (threadIdx.x == 0) stg(largest + blockIdx.x, m);
+}
+
+// What to multiply by; the factor that undoes it is left by the first block.
+__device__ __forceinline__ float grad_scale(const GradScale& s) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < kScaleBlocks / kBlock; ++j) {
+    const int i = j * kBlock + threadIdx.x;
+    if (i < s.blocks) m = std::max(m, ldg(s.largest + i));
+  }
+  m = block_max(m);
+  // 2^e of the largest in [2^14, 2^15); both 2^e and 2^-e among the normal numbers
+  const int e = m == 0 ? 0 : std::min(14 - (static_cast<int>(m >> 23) - 127), 126);
+  if (blockIdx.x == 0 && threadIdx.x == 0) stg(s.factor, __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
+  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
 // dg and du of 8 units per lane, into d [T, 2 * pitch]: dg, then du, zeros
 // in the columns past `units`; plane: elements from one plane to the next.
 // DIRECT: as float, with no columns past `units` (pitch == units).
 template <typename T, int ACT, bool DIRECT>
 __global__ __launch_bounds__(kBlock) void gated_grad_kernel(const T* dh, int64_t lddh, const float* gate, const float* up,
                                                             int64_t rows, int64_t units, int64_t pitch, uint16_t* d,
-                                                            int64_t plane) {
+                                                            int64_t plane, GradScale scale) {
+  constexpr bool SCALED = std::is_same_v<T, f16> && !DIRECT;
+  float by = 1.f;
+  if constexpr (SCALED) by = grad_scale(scale);
   const int64_t per_row = (pitch + 7) / 8, all = rows * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < all;
        i += static_cast<int64_t>(gridDim.x) * kBlock) {
@@ -147,9 +228,9 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(const T* dh, int64_t
     load_row<T, 8>(dh + r * lddh, c, units, dhv);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float a, da;
-      activation<ACT>(g[e], &a, &da);
-      const float dg = dhv[e] * u[e] * da, du = dhv[e] * a;
+      float dg, du;
+      unit_grads<ACT>(g[e], u[e], dhv[e], &dg, &du);
+      if (SCALED) dg *= by, du *= by;
       g[e] = c + e < units ? dg : 0.f;
       u[e] = c + e < units ? du : 0.f;
     }
@@ -178,15 +259,28 @@ __global__ __launch_bounds__(kBlock) void gated_grad_kernel(const T* dh, int64_t
   }
 }
 
+static int32_t gated_largest(const p2p_gated_linear_t& a, const GradScale& scale, hipStream_t st) {
+  const auto kernel = a.activation == P2P_ACT_SILU   ? gated_largest_kernel<P2P_ACT_SILU>
+                      : a.activation == P2P_ACT_GELU ? gated_largest_kernel<P2P_ACT_GELU>
+                                                     : gated_largest_kernel<P2P_ACT_RELU>;
+  kernel<<<dim3(scale.blocks), dim3(kBlock), 0, st>>>(static_cast<const f16*>(a.dh), a.lddh, a.gate, a.up, a.tokens, a.units,
+                                                      scale.largest);
+  return launch_status();
+}
+
 template <typename T, bool DIRECT>
-static int32_t gated_grad(const p2p_gated_linear_t& a, int64_t pitch, uint16_t* d, hipStream_t st) {
+static int32_t gated_grad(const p2p_gated_linear_t& a, int64_t pitch, uint16_t* d, const GradScale& scale, hipStream_t st) {
+  if (std::is_same_v<T, f16> && !DIRECT) {
+    const int32_t rc = gated_largest(a, scale, st);
+    if (rc != P2P_OK) return rc;
+  }
   const int64_t items = a.tokens * ceil_div(pitch, 8), blocks = ceil_div(items, kBlock);
   const dim3 grid(static_cast<unsigned>(blocks < 256 * 32 ? blocks : 256 * 32)), block(kBlock);
   const auto kernel = a.activation == P2P_ACT_SILU   ? gated_grad_kernel<T, P2P_ACT_SILU, DIRECT>
                       : a.activation == P2P_ACT_GELU ? gated_grad_kernel<T, P2P_ACT_GELU, DIRECT>
                                                      : gated_grad_kernel<T, P2P_ACT_RELU, DIRECT>;
   kernel<<<grid, block, 0, st>>>(static_cast<const T*>(a.dh), a.lddh, a.gate, a.up, a.tokens, a.units, pitch, d,
-                                 a.tokens * 2 * pitch);
+                                 a.tokens * 2 * pitch, scale);
   return launch_status();
 }
 
@@ -241,6 +335,7 @@ static Plan gated_fwd_plan(const p2p_gated_linear_t& a) {
 // The workspace, in the order in which both passes carve it.
 struct GatedSpace {
   uint16_t *x, *wg, *wu, *d;
+  GradScale scale;  // float16 on tiles
   float* parts;
   float* dx_parts;  // of direct.h's product, whose gradients are made side by side
 };
@@ -291,6 +386,7 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
     s->wu = static_cast<uint16_t*>(c.take(packed_bytes(a.units, a.hidden, a.dtype)));
   }
   s->d = nullptr;
+  s->scale = GradScale{};
   s->parts = s->dx_parts = nullptr;
   if (!backward) {
     const int64_t split = gated_fwd_plan(a).split;
@@ -298,6 +394,11 @@ static int64_t gated_carve(const p2p_gated_linear_t& a, bool backward, void* bas
   } else {
     const int64_t rows2 = 2 * gated_pitch(a);
     s->d = static_cast<uint16_t*>(c.take(a.tokens * rows2 * 2 * planes_of(a.dtype)));
+    if (a.dtype == P2P_DTYPE_F16) {
+      s->scale.blocks = static_cast<int>(std::min<int64_t>(ceil_div(a.tokens * ceil_div(a.units, 8), kBlock), kScaleBlocks));
+      s->scale.largest = static_cast<uint32_t*>(c.take(kScaleBlocks * 4));
+      s->scale.factor = static_cast<float*>(c.take(4));
+    }
     const Plan px = gated_dx_plan(a), pw = gated_dw_plan(a);
     int64_t floats = 0;
     if (px.split > 1) floats = px.split * a.tokens * a.hidden;
@@ -402,7 +503,7 @@ static int32_t gated_direct_bwd(const p2p_gated_linear_t& a, const GatedSpace& s
                      {a.dw_gate, a.dw_up}, a.units, {nullptr, nullptr}, sw > 1 ? s.parts : nullptr};
   int32_t rc;
   if (s.d) {
-    if ((rc = gated_grad<T, true>(a, a.units, s.d, st)) != P2P_OK) return rc;
+    if ((rc = gated_grad<T, true>(a, a.units, s.d, s.scale, st)) != P2P_OK) return rc;
     const float* d = reinterpret_cast<const float*>(s.d);
     rc = direct_grads<DirectLines<float>, T>(x, w, {d, d, rows2, rows2, INT64_MAX}, st);
   } else {
@@ -473,9 +574,9 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
   Mat x, wg, wu;
   if ((rc = gated_operands(*a, s, &x, &wg, &wu, st)) != P2P_OK) return rc;
   const int64_t pitch = gated_pitch(*a), plane = a->tokens * 2 * pitch;
-  rc = a->dtype == P2P_DTYPE_F32 ? gated_grad<float, false>(*a, pitch, s.d, st)
-       : f16_                    ? gated_grad<f16, false>(*a, pitch, s.d, st)
-                                 : gated_grad<bf16, false>(*a, pitch, s.d, st);
+  rc = a->dtype == P2P_DTYPE_F32 ? gated_grad<float, false>(*a, pitch, s.d, s.scale, st)
+       : f16_                    ? gated_grad<f16, false>(*a, pitch, s.d, s.scale, st)
+                                 : gated_grad<bf16, false>(*a, pitch, s.d, s.scale, st);
   if (rc != P2P_OK) return rc;
   Mat dg{{s.d, s.d + plane, s.d + 2 * plane}, 2 * pitch};
   Mat du{{s.d + pitch, s.d + plane + pitch, s.d + 2 * plane + pitch}, 2 * pitch};
@@ -488,10 +589,10 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
     g.M = a->tokens, g.N = a->hidden, g.K = a->units;
     const Plan plan = gated_dx_plan(*a);
     g.ksplit = plan.split;
-    StoreEpi e{{a->dx, nullptr}, 0, 0, a->hidden, a->dtype, {nullptr, nullptr}, 1.f, plan.split > 1 ? s.parts : nullptr, 0};
+    StoreEpi e{{a->dx, nullptr}, 0, 0, a->hidden, a->dtype, {s.scale.factor, nullptr}, 1.f, plan.split > 1 ? s.parts : nullptr, 0};
     if ((rc = gemm_launch<false, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
-    if (plan.split > 1 && (rc = join_parts(s.parts, plan.split, g.M * g.N, g.M * g.N, 0, nullptr, nullptr, 1.f, a->dx, nullptr,
-                                           a->dtype, st)) != P2P_OK)
+    if (plan.split > 1 && (rc = join_parts(s.parts, plan.split, g.M * g.N, g.M * g.N, 0, s.scale.factor, nullptr, 1.f, a->dx,
+                                           nullptr, a->dtype, st)) != P2P_OK)
       return rc;
   }
   {  // dWg = dg^T x, dWu = du^T x: one product of 2 pitch rows
@@ -501,11 +602,11 @@ extern "C" int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t* a, void* works
     g.M = 2 * pitch, g.N = a->hidden, g.K = a->tokens;
     const Plan plan = gated_dw_plan(*a);
     g.ksplit = plan.split;
-    StoreEpi e{{a->dw_gate, a->dw_up}, pitch, a->units, a->hidden, a->dtype, {nullptr, nullptr}, 1.f,
+    StoreEpi e{{a->dw_gate, a->dw_up}, pitch, a->units, a->hidden, a->dtype, {s.scale.factor, nullptr}, 1.f,
                plan.split > 1 ? s.parts : nullptr, 0};
     if ((rc = gemm_launch<true, true, false>(g, f16_, plan.big, e, st)) != P2P_OK) return rc;
     if (plan.split > 1)
-      return join_parts(s.parts, plan.split, g.M * g.N, a->units * a->hidden, pitch * a->hidden, nullptr, nullptr, 1.f,
+      return join_parts(s.parts, plan.split, g.M * g.N, a->units * a->hidden, pitch * a->hidden, s.scale.factor, nullptr, 1.f,
                         a->dw_gate, a->dw_up, a->dtype, st);
   }
   return P2P_OK;

@@ -44,3 +44,62 @@ def test_layer_norm_backward_of_large_constant_rows(cuda, dtype, cols):
     strict(dw, torch.zeros(cols), torch.zeros(cols), "dw")
     total = dy.double().cpu().sum(0)
     strict(db, total, rounded(total, 16 * U * dy.double().cpu().abs().sum(0), dtype), "db")
+
+
+# ------------------------------------------------------------------ gated linear layer
+GATED_RANGE = [(30, 64, 40), (600, 264, 500), (257, 2041, 1100), (1500, 512, 300)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,units", GATED_RANGE)
+@pytest.mark.parametrize("grad,up", [(2.0 ** -22, 1.0), (2.0 ** -22, 64.0), (2.0 ** -17, 1.0), (100.0, 300.0)])
+def test_gated_linear_small_and_large_gradients(cuda, monkeypatch, dtype, rows, cols, units, grad, up):
+    """dg and du next to either end of float16's range, on the small path and on tiles: their rounding is half a step
+    of the type, or of float16's smallest one scaled (the largest is held in [2^14, 2^15): 2^-25 * 2^-14 of it)."""
+    x, dh = randn((rows, cols), dtype, 72), randn((rows, units), dtype, 73, grad)
+    wg, wu = randn((units, cols), dtype, 74, cols ** -0.5), randn((units, cols), dtype, 75, cols ** -0.5 * up)
+    h, gate, u_ = T.gated_linear_forward(x, wg, wu)
+    got = T.gated_linear_backward(dh, x, wg, wu, gate, u_)
+    a, da = ops.act64("silu", x.double().cpu() @ wg.double().cpu().t())
+    d64 = dh.double().cpu()
+    largest = max((d64 * da * (x.double().cpu() @ wu.double().cpu().t())).abs().max(), (d64 * a).abs().max()).item()
+
+    def scaled(want, err, t):
+        floor = 2.0 ** -39 * 1.01 * largest if t == torch.float16 else ops.tiny(t)
+        return err + ops.u(t) * (want.abs() + err) + floor
+
+    with monkeypatch.context() as m:
+        m.setattr(ops, "rounded", scaled)  # of dg and du; the results' own roundings are the type's
+        want, err = ops.gated_reference(x, wg, wu, dh, "silu")
+    for o, v, e, name in zip(got, want[1:], err[1:], ("dx", "dwg", "dwu")):
+        bound = rounded(v, e, dtype)
+        # rounded to the type: what is past its largest value is an infinity; at that border either may come
+        limit = torch.finfo(dtype).max
+        clear = ((v.abs() + bound) < limit) | ((v.abs() - bound) > limit * (1 + ops.u(dtype)))
+        v = torch.where(v.abs() > limit, torch.copysign(torch.tensor(float("inf"), dtype=v.dtype), v), v)
+        strict(torch.where(clear, o.double().cpu(), 0.0), torch.where(clear, v, 0.0), bound, (name, largest))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,units", GATED_RANGE[:2])
+def test_gated_linear_gradients_that_are_not_finite(cuda, dtype, rows, cols, units):
+    """A NaN and an infinity in one token's dh stay with that token's dx; the other tokens' dx have the bits they have
+    without them (the power of two of float16 goes by the finite ones)."""
+    x, dh = randn((rows, cols), dtype, 76), randn((rows, units), dtype, 77)
+    wg, wu = randn((units, cols), dtype, 78, cols ** -0.5), randn((units, cols), dtype, 79, cols ** -0.5)
+    h, gate, up = T.gated_linear_forward(x, wg, wu)
+    clean = T.gated_linear_backward(dh, x, wg, wu, gate, up)[0]
+    bad = dh.clone()
+    bad[3, 5], bad[7, 9] = float("nan"), float("inf")
+    dx, dwg, dwu = T.gated_linear_backward(bad, x, wg, wu, gate, up)
+    rest = [i for i in range(rows) if i not in (3, 7)]
+    assert same_bits(dx[rest], clean[rest]) and not torch.isfinite(dx[[3, 7]]).any()
+    assert not torch.isfinite(dwg[[5, 9]]).any() and not torch.isfinite(dwu[[5, 9]]).any()
+    others = [i for i in range(units) if i not in (5, 9)]
+    assert torch.isfinite(dwg[others]).all() and torch.isfinite(dwu[others]).all()
+    # nothing to scale by: no gradient, and none that is finite
+    zero = T.gated_linear_backward(torch.zeros_like(dh), x, wg, wu, gate, up)
+    assert not any(t.any() for t in zero)
+    assert torch.isnan(T.gated_linear_backward(torch.full_like(dh, float("nan")), x, wg, wu, gate, up)[0]).all()
