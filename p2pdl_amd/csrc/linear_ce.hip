@@ -509,9 +509,11 @@ static int64_t ce_carve(const p2p_linear_ce_t& a, bool backward, void* base, CeS
   }
   const int planes = planes_of(a.dtype);
   const bool x_here = in_place(a.x, a.ldx, a.hidden, a.dtype), w_here = in_place(a.w, a.ldw, a.hidden, a.dtype);
-  // pieces: the buffers that grow with one stay under kPieceBytes (one tile's columns at least)
+  // pieces: the buffers that grow with one stay under kPieceBytes (one tile's columns at least).  By shape and type alone,
+  // since the sums over pieces are rounded piece by piece: a weight that is copied for its address or pitch only is
+  // copied whole with its piece, however large
   int64_t per_row = backward ? a.tokens * 2 * planes : ceil_div(a.tokens * 8, Small::BN);
-  if (!w_here) per_row = std::max(per_row, line_pitch(a.hidden) * 2 * planes);
+  if (a.dtype == P2P_DTYPE_F32 || a.hidden % 8) per_row = std::max(per_row, line_pitch(a.hidden) * 2 * planes);
   int64_t piece = std::max<int64_t>(1, kPieceBytes / per_row / Big::BN) * Big::BN;
   if (piece >= a.vocab) piece = a.vocab;
   else piece = round_up(ceil_div(a.vocab, ceil_div(a.vocab, piece)), Big::BN);  // pieces of about one size

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import test_training_ops as ops
+from p2pdl_amd import _native as N
 from p2pdl_amd import training as T
 from test_training_ops import DTYPES, U, gpu, randn, rounded, same_bits
 
@@ -103,3 +104,40 @@ def test_gated_linear_gradients_that_are_not_finite(cuda, dtype, rows, cols, uni
     zero = T.gated_linear_backward(torch.zeros_like(dh), x, wg, wu, gate, up)
     assert not any(t.any() for t in zero)
     assert torch.isnan(T.gated_linear_backward(torch.full_like(dh, float("nan")), x, wg, wu, gate, up)[0]).all()
+
+
+# ------------------------------------------------------------------ linear cross entropy
+@pytest.mark.parametrize("dtype", [N.P2P_DTYPE_F16, N.P2P_DTYPE_BF16])
+@pytest.mark.parametrize("tokens,hidden,vocab", [(256, 4096, 70000), (1024, 4096, 131072), (2048, 4096, 131072), (512, 2048, 400000)])
+@pytest.mark.parametrize("backward", [0, 1])
+def test_linear_ce_pieces_do_not_depend_on_the_weights_place(dtype, tokens, hidden, vocab, backward):
+    """A weight that cannot be read where it lies costs its copy; the pieces, whose sums are rounded one by one, stay."""
+    L = N.load_library()
+    here = ops.ce_args(tokens=tokens, hidden=hidden, vocab=vocab, ldx=hidden, ldw=hidden, dtype=dtype)
+    need = L.p2p_linear_ce_workspace(here, backward)
+    for other in ({"w": here.w + 2}, {"ldw": hidden + 1}):
+        there = ops.ce_args(tokens=tokens, hidden=hidden, vocab=vocab, ldx=hidden, ldw=hidden, dtype=dtype)
+        for k, v in other.items():
+            setattr(there, k, v)
+        assert L.p2p_linear_ce_workspace(there, backward) - need == vocab * hidden * 2, other
+
+
+@gpu
+def test_linear_cross_entropy_bits_do_not_depend_on_the_weights_place(cuda):
+    """256 x 4096 x 70000: the copy of a weight that lies one element off, or has an odd pitch, is 573 MB."""
+    rows, cols, vocab = 256, 4096, 70000
+    g = torch.Generator("cuda").manual_seed(80)
+    w = torch.randn((vocab, cols), generator=g, device="cuda", dtype=torch.bfloat16) * 0.03
+    x = torch.randn((rows, cols), generator=g, device="cuda", dtype=torch.bfloat16)
+    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    dloss = torch.tensor(256.0, device="cuda")
+
+    def step(weight):
+        loss, lse, norm = T.linear_cross_entropy_forward(x, weight, t)
+        return (loss, lse) + T.linear_cross_entropy_backward(x, weight, t, lse, norm, dloss)
+
+    want = step(w)
+    off = torch.empty(vocab * cols + 1, device="cuda", dtype=w.dtype)[1:].view(vocab, cols).copy_(w)
+    pitched = torch.empty((vocab, cols + 1), device="cuda", dtype=w.dtype)[:, :cols].copy_(w)
+    for other in (off, pitched):
+        assert all(same_bits(a, b) for a, b in zip(step(other), want))
