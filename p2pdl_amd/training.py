@@ -98,6 +98,11 @@ def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+def _pair(shape, dtype: torch.dtype, dev: torch.device):
+    """Two tensors of their own (a view of a common one could not be changed in place once autograd returns it)."""
+    return torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+
+
 def _stat(t: torch.Tensor, x: torch.Tensor, name: str, shape) -> None:
     """A dense float32 tensor that a forward pass left for its backward pass."""
     if t.shape == shape and t.dtype is torch.float32 and t.device == x.device and t.is_contiguous():
@@ -171,7 +176,7 @@ def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias
     dev, cols = x.device, x.shape[-1]
     rows = x.numel() // cols
     y = _new(x)
-    mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=dev).unbind(0)
+    mean, rstd = _pair(x.shape[:-1], torch.float32, dev)
     if rows:
         xr, ld = _rows(x)
         w = None if weight is None else weight.contiguous()
@@ -196,7 +201,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     dx = _new(x)
     dw = db = None
     if weight is not None:
-        dw, db = (torch.empty if rows else torch.zeros)((2, cols), dtype=x.dtype, device=dev).unbind(0)
+        dw, db = _pair((cols,), x.dtype, dev)
     if rows:
         L = N.lib()
         xr, ldx = _rows(x)
@@ -209,6 +214,9 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
             ws = _workspace(nbytes, dev, "p2p_layernorm_bwd_workspace")
         _call(L.p2p_layernorm_bwd, "p2p_layernorm_bwd", dev, dyr.data_ptr(), lddy, xr.data_ptr(), ldx, _ptr(w),
               mean.data_ptr(), rstd.data_ptr(), rows, cols, dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), nbytes, dt)
+    elif weight is not None:
+        dw.zero_()
+        db.zero_()
     return dx, dw, db
 
 
@@ -355,7 +363,7 @@ def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
     h = torch.empty(shape, dtype=x.dtype, device=dev)
     gate = up = None
     if save:
-        gate, up = torch.empty((2,) + shape, dtype=torch.float32, device=dev).unbind(0)
+        gate, up = _pair(shape, torch.float32, dev)
     if x.numel():
         L = N.lib()
         a, keep = _gated_args(x, w_gate, w_up, dt, act)
@@ -461,7 +469,7 @@ def linear_cross_entropy_forward(x: torch.Tensor, weight: torch.Tensor, target: 
         return done
     a, keep = _ce_args(x, weight, target, ignore_index)
     dev = x.device
-    loss, norm = torch.empty(2, dtype=torch.float32, device=dev).unbind(0)
+    loss, norm = _pair((), torch.float32, dev)
     lse = torch.empty(target.shape, dtype=torch.float32, device=dev)
     a.mean = reduction == "mean"
     a.loss, a.lse, a.norm = loss.data_ptr(), lse.data_ptr(), norm.data_ptr()

@@ -141,3 +141,54 @@ def test_linear_cross_entropy_bits_do_not_depend_on_the_weights_place(cuda):
     pitched = torch.empty((vocab, cols + 1), device="cuda", dtype=w.dtype)[:, :cols].copy_(w)
     for other in (off, pitched):
         assert all(same_bits(a, b) for a, b in zip(step(other), want))
+
+
+# ------------------------------------------------------------------ both host paths
+def host_paths(monkeypatch):
+    """'C++', then 'Python': the path that a dense call takes, and the one that copies and explains."""
+    yield "C++"
+    with monkeypatch.context() as m:
+        m.setattr(T, "_host", type("NoHost", (), {"__getattr__": lambda self, name: lambda *a: None})())
+        yield "Python"
+
+
+@gpu
+@pytest.mark.parametrize("pitched", [False, True])
+def test_a_loss_may_be_changed_in_place(cuda, monkeypatch, pitched):
+    """loss /= steps before backward(), whichever path made the loss."""
+    wide = randn((12, 40), torch.float32, 81)
+    x = wide[:, 3:35] if pitched else wide[:, :32].contiguous()
+    t = (torch.arange(12) % 7).cuda()
+    grads = []
+    for path in host_paths(monkeypatch):
+        w = randn((7, 32), torch.float32, 82).requires_grad_()
+        loss = T.linear_cross_entropy(x, w, t)
+        loss /= 4
+        loss.mul_(2)
+        loss.backward()
+        grads.append(w.grad)
+    assert same_bits(*grads)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_results_are_tensors_of_their_own(cuda, monkeypatch, dtype):
+    """No result is a view, or shares its memory with another one, and both paths have the same bits."""
+    x, dy = randn((9, 24), dtype, 83), randn((9, 24), dtype, 84)
+    w, wide, dh = randn((24,), dtype, 85), randn((16, 24), dtype, 86), randn((9, 16), dtype, 87)
+    t = (torch.arange(9) % 16).cuda()
+    found = []
+    for path in host_paths(monkeypatch):
+        y, mean, rstd = T.layer_norm_forward(x, w, w)
+        h, gate, up = T.gated_linear_forward(x, wide, wide)
+        loss, lse, norm = T.linear_cross_entropy_forward(x, wide, t)
+        out = [y, mean, rstd, h, gate, up, loss, lse, norm, T.dropout_forward(x, 0.5, 3, residual=x)]
+        out += T.layer_norm_backward(dy, x, mean, rstd, w)
+        out += T.gated_linear_backward(dh, x, wide, wide, gate, up)
+        out += T.linear_cross_entropy_backward(x, wide, t, lse, norm)
+        out += T.layer_norm_backward(dy[:0], x[:0], mean[:0], rstd[:0], w)[1:]
+        assert all(o._base is None for o in out), path
+        assert len({o.untyped_storage().data_ptr() for o in out}) == len(out), path
+        found.append(out)
+    assert all(same_bits(a, b) for a, b in zip(*found))
+    assert not found[0][-1].any() and not found[0][-2].any()
