@@ -251,7 +251,7 @@ struct Gated : Call {
     args.ldx = args.ldg = args.ldu = cols;
     args.tokens = rows, args.hidden = cols, args.units = wg.size(0);
     args.activation = static_cast<int32_t>(integer(act)), args.dtype = dtype;
-    if (cols > (1 << 22) - 8 || args.units > (1 << 21) - 4) throw OtherPath{};
+    if (cols > (1 << 22) - 8 || args.units > (1 << 21) - 8) throw OtherPath{};
   }
 };
 

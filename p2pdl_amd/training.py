@@ -45,7 +45,8 @@ _bound = False
 DTYPES = {torch.float32: N.P2P_DTYPE_F32, torch.float16: N.P2P_DTYPE_F16, torch.bfloat16: N.P2P_DTYPE_BF16}
 ACTIVATIONS = {"silu": N.P2P_ACT_SILU, "gelu": N.P2P_ACT_GELU, "relu": N.P2P_ACT_RELU}
 MAX_NORM_COLS = 16384
-MAX_FEATURES = (1 << 22) - 8
+MAX_FEATURES = (1 << 22) - 8  # of a product
+MAX_UNITS = (1 << 21) - 8
 
 
 def _bind() -> None:
@@ -331,8 +332,8 @@ def _gated_inputs(x, w_gate, w_up, activation):
         raise ValueError(f"w_gate: expected a [units, features] weight, got shape {tuple(w_gate.shape)}")
     _like(w_gate, x, "w_gate", (w_gate.shape[0], x.shape[-1]))
     _like(w_up, x, "w_up", w_gate.shape)
-    if x.shape[-1] > MAX_FEATURES or w_gate.shape[0] > MAX_FEATURES // 2:
-        raise ValueError(f"at most {MAX_FEATURES} features and {MAX_FEATURES // 2} units, got {tuple(w_gate.shape)}")
+    if x.shape[-1] > MAX_FEATURES or w_gate.shape[0] > MAX_UNITS:
+        raise ValueError(f"at most {MAX_FEATURES} features and {MAX_UNITS} units, got {tuple(w_gate.shape)}")
     return dt, act
 
 

@@ -192,3 +192,37 @@ def test_results_are_tensors_of_their_own(cuda, monkeypatch, dtype):
         found.append(out)
     assert all(same_bits(a, b) for a, b in zip(*found))
     assert not found[0][-1].any() and not found[0][-2].any()
+
+
+# ------------------------------------------------------------------ limits
+def test_limits_are_the_librarys():
+    """The wrappers' limits are the library's own, on either side of each."""
+    L = N.load_library()
+    n, f = T.MAX_UNITS, T.MAX_FEATURES
+    assert L.p2p_gated_linear_workspace(ops.gated_args(units=n), 1) >= 0
+    assert L.p2p_gated_linear_workspace(ops.gated_args(units=n + 1), 1) == -2
+    wide = {"hidden": f, "ldx": f, "ldg": f, "ldu": f}
+    assert L.p2p_gated_linear_workspace(ops.gated_args(**wide), 1) >= 0
+    assert L.p2p_gated_linear_workspace(ops.gated_args(**{k: v + 1 for k, v in wide.items()}), 1) == -2
+    wide = {"hidden": f, "ldx": f, "ldw": f}
+    assert L.p2p_linear_ce_workspace(ops.ce_args(**wide), 1) >= 0
+    assert L.p2p_linear_ce_workspace(ops.ce_args(**{k: v + 1 for k, v in wide.items()}), 1) == -2
+    c = T.MAX_NORM_COLS
+    assert L.p2p_layernorm_bwd_workspace(1, c, 0) >= 0 and L.p2p_layernorm_bwd_workspace(1, c + 1, 0) < 0
+
+
+@gpu
+def test_more_units_than_the_limit_are_refused(cuda):
+    """2^21 - 8 units run; past them, up to 2^21 - 4 and more, both passes say what the limit is."""
+    x = torch.ones(1, 1, device="cuda")
+    for n in (T.MAX_UNITS, T.MAX_UNITS + 1, T.MAX_UNITS + 4, T.MAX_UNITS + 5):
+        w = torch.ones(n, 1, device="cuda")
+        row = torch.ones(1, n, device="cuda")
+        if n == T.MAX_UNITS:
+            h, gate, up = T.gated_linear_forward(x, w, w, "relu")
+            assert (h == 1).all() and T.gated_linear_backward(row, x, w, w, gate, up, "relu")[0].item() == 2 * n
+            continue
+        for call in (lambda: T.gated_linear_forward(x, w, w, "relu"),
+                     lambda: T.gated_linear_backward(row, x, w, w, row, row, "relu")):
+            with pytest.raises(ValueError, match=str(T.MAX_UNITS)):
+                call()
