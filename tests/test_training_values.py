@@ -226,3 +226,60 @@ def test_more_units_than_the_limit_are_refused(cuda):
                      lambda: T.gated_linear_backward(row, x, w, w, row, row, "relu")):
             with pytest.raises(ValueError, match=str(T.MAX_UNITS)):
                 call()
+
+
+# ------------------------------------------------------------------ the forms in 64 bits, infinities and NaN compared too
+def reruns():
+    for dtype in DTYPES:
+        for shape in ops.NORM_SHAPES:
+            yield ops.test_layer_norm, (dtype, *shape)
+        for shape in ops.GATED_SHAPES:
+            yield ops.test_gated_linear, (dtype, *shape, "silu")
+        for shape in ops.CE_SHAPES:
+            yield ops.test_linear_cross_entropy, (dtype, *shape, "mean")
+        for args in ((1000, 0.1, 0xDEADBEEFCAFEF00D, (1 << 32) - 3), (2051, 1 - 2.0 ** -33, 3, 4)):
+            yield ops.test_dropout, (dtype, *args)
+
+
+@gpu
+@pytest.mark.parametrize("test,args", [pytest.param(t, a, id=f"{t.__name__[5:]}-{'-'.join(str(v) for v in a)}") for t, a in reruns()])
+def test_values_that_are_not_finite_too(cuda, monkeypatch, test, args):
+    """ops.check lets a value pass where the form in 64 bits has a NaN or an infinity; here none does."""
+    monkeypatch.setattr(ops, "check", strict)
+    test(cuda, *args)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,units", [(30, 64, 40), (600, 264, 500)])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_gated_linear_inputs_that_are_not_finite(cuda, dtype, rows, cols, units, act):
+    """A NaN and an infinity in x: what the form in 64 bits makes of them, in every place.  (An infinity among
+    the float32 operands of a product on tiles may come out as NaN.)"""
+    x, dh = randn((rows, cols), dtype, 88), randn((rows, units), dtype, 89)
+    wg, wu = randn((units, cols), dtype, 90, cols ** -0.5), randn((units, cols), dtype, 91, cols ** -0.5)
+    x[3, 5] = float("nan")
+    if dtype != torch.float32 or rows <= 192:
+        x[7, 9] = float("inf")
+    h, gate, up = T.gated_linear_forward(x, wg, wu, act)
+    got = (h,) + T.gated_linear_backward(dh, x, wg, wu, gate, up, act)
+    want, err = ops.gated_reference(x, wg, wu, dh, act)
+    for o, v, e, name in zip(got, want, err, ("h", "dx", "dwg", "dwu")):
+        strict(o, v, rounded(v, e, dtype), name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols,vocab", [(30, 64, 100), (600, 264, 900)])
+def test_linear_cross_entropy_inputs_that_are_not_finite(cuda, dtype, rows, cols, vocab):
+    """A NaN in a token that counts: the loss, that token's dx and all of dW; no other token's dx."""
+    x, w, t = ops.ce_inputs(rows, cols, vocab, dtype, 92)
+    t[3] = 5
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    clean = T.linear_cross_entropy_backward(x, w, t, lse, norm)[0]
+    x[3, 6] = float("nan")
+    loss, lse, norm = T.linear_cross_entropy_forward(x, w, t)
+    dx, dw = T.linear_cross_entropy_backward(x, w, t, lse, norm)
+    rest = [i for i in range(rows) if i != 3]
+    assert torch.isnan(loss) and torch.isnan(lse[3]) and torch.isfinite(lse[rest]).all()
+    assert torch.isnan(dx[3]).all() and same_bits(dx[rest], clean[rest]) and torch.isnan(dw).all()
