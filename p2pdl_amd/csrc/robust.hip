@@ -58,18 +58,16 @@ __device__ __forceinline__ float special_floats(const uint32_t (&v)[KP], uint64_
       c[j].x = at(2 * Q + j);
       d[j].x = at(3 * Q + j);
     }
-    // PAD: lists c and d (slots KP/2..KP-1) may hold pad rows
-    constexpr int S = PAD ? 0 : 1 << 20;
     sort_full<Q>(a, NanHook<>{nan});
     sort_full<Q>(b, NanHook<>{nan});
-    sort_full<Q>(c, NanHook<1, 0, S>{nan});
-    sort_full<Q>(d, NanHook<1, 0, S>{nan});
+    sort_full<Q>(c, NanHook<>{nan});
+    sort_full<Q>(d, NanHook<>{nan});
     return four_list_median<Q>(a, b, c, d).x;
   } else {
     fx x[KP];
 #pragma unroll
     for (int j = 0; j < KP; ++j) x[j].x = at(j);
-    run_special<KP, 2>(x, NanHook<1, 0, PAD ? KP / 32 : 1 << 20>{nan});  // PAD: blocks of slots >= KP/2
+    run_special<KP, 2>(x, NanHook<>{nan});
     constexpr int b = (KP * 2) / 10;
     float acc = 0.f;
     if constexpr (PAD) {  // padded ranks b..b+m-1

@@ -67,20 +67,6 @@ __device__ __forceinline__ float div_const(float a) {
   return div_const_fast<D>(a);
 }
 
-// Lanes for which any of the N values at(0) .. at(N-1) is NaN.  NaN
-// propagates through v_pk_fma_f32 (a * b + c on float pairs), so each
-// instruction folds four more values into a running pair: the first takes
-// six, the rest four, and one v_cmp_u_f32 tests the final pair -- about N/4 + 1
-// instructions where one compare per two values takes N/2 (the loaded
-// values already sit in register pairs: no moves).  An overflowing product,
-// inf * 0 or inf - inf also ends in NaN: a false alarm only sends the tile
-// to the exact uint32-key network.  Fewer than six values: compares.
-typedef float f2v __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ f2v pk_fma(f2v a, f2v b, f2v c) {
-  f2v d;
-  asm volatile("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-  return d;
-}
 // v_maximum3_f32 (IEEE 754-2019 maximum, gfx950): NaN in, NaN out, and no
 // NaN from infinities.
 __device__ __forceinline__ float maximum3(float a, float b, float c) {
@@ -100,33 +86,30 @@ __device__ __forceinline__ float maximum3_nv(float a, float b, float c) {
   asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
   return d;
 }
-// INF_SAFE: the test of a padded network's slots, whose +-inf pad rows meet
-// (inf - inf in the FMA chain would send every tile to the key path): two
-// v_maximum3 chains, two values per instruction.
-template <int N, bool INF_SAFE = false, typename F>
+// Lanes for which any of the N values at(0) .. at(N-1) is NaN: two chains of
+// v_maximum3_f32, two values per instruction, and one v_cmp_u_f32 over both --
+// about N/2 instructions, in asm that -fno-honor-nans cannot fold; infinities
+// (pad rows of the padded networks) are no alarm.  Fewer than six values:
+// compares.  (Four values per v_pk_fma_f32 are half the instructions and no
+// faster, K = 128 median of 16.8M 1.388 / 1.382 ms; packed 32-bit float
+// instructions are not used in this library.)
+template <int N, typename F>
 __device__ __forceinline__ uint64_t nan_lanes(F&& at) {
   static_assert(N % 2 == 0, "pairs");
-  if constexpr (INF_SAFE && N >= 6) {
+  if constexpr (N >= 6) {
     float a = maximum3(at(0), at(1), at(2)), b = maximum3(at(3), at(4), at(5));
-    int j = 6;
 #pragma unroll
-    for (; j + 3 < N; j += 4) {
+    for (int j = 6; j + 3 < N; j += 4) {
       a = maximum3(a, at(j), at(j + 1));
       b = maximum3(b, at(j + 2), at(j + 3));
     }
     if constexpr ((N - 6) % 4 == 2) a = maximum3(a, at(N - 2), at(N - 1));
     return unordered_mask(a, b);
-  } else if constexpr (N < 6) {
+  } else {
     uint64_t m = 0;
 #pragma unroll
     for (int j = 0; j < N / 2; ++j) m |= unordered_mask(at(j), at(j + N / 2));
     return m;
-  } else {
-    f2v acc = pk_fma(f2v{at(0), at(1)}, f2v{at(2), at(3)}, f2v{at(4), at(5)});
-#pragma unroll
-    for (int j = 6; j + 3 < N; j += 4) acc = pk_fma(f2v{at(j), at(j + 1)}, f2v{at(j + 2), at(j + 3)}, acc);
-    if constexpr ((N - 6) % 4 == 2) acc = pk_fma(f2v{at(N - 2), at(N - 1)}, f2v{1.f, 1.f}, acc);
-    return unordered_mask(acc.x, acc.y);
   }
 }
 
@@ -201,21 +184,19 @@ struct NoHook {
 __device__ __forceinline__ float bits_f(uint32_t k) { return __uint_as_float(k); }
 __device__ __forceinline__ float bits_f(fk x) { return x.x; }
 __device__ __forceinline__ float bits_f(fx x) { return x.x; }
-// The NaN test of the float networks (nan_lanes: packed FMAs), block by
+// The NaN test of the float networks (nan_lanes), block by
 // block as the network first reads it: the test waits only for that
 // block's loads (a whole-wave test up front waited for every load before the
 // first comparator: median256 -3.5% time without it).
-// G blocks per test, blocks from FIRST on; blocks from SAFE on may hold pad
-// rows (nan_lanes INF_SAFE).
-template <int G = 1, int FIRST = 0, int SAFE = 1 << 20>
+// G blocks per test, blocks from FIRST on.
+template <int G = 1, int FIRST = 0>
 struct NanHook {
   uint64_t& m;
   template <typename T, int KP>
   __device__ __forceinline__ void operator()(T (&v)[KP], int blk) const {
     if (blk % G != 0 || blk < FIRST) return;
     constexpr int N = 16 * G < KP ? 16 * G : KP;
-    if (blk >= SAFE) m |= nan_lanes<N, true>([&](int j) { return bits_f(v[16 * blk + j]); });
-    else m |= nan_lanes<N>([&](int j) { return bits_f(v[16 * blk + j]); });
+    m |= nan_lanes<N>([&](int j) { return bits_f(v[16 * blk + j]); });
   }
 };
 __device__ __forceinline__ uint32_t umed3(uint32_t a, uint32_t b, uint32_t c) {
