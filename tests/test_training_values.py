@@ -106,6 +106,38 @@ def test_gated_linear_gradients_that_are_not_finite(cuda, dtype, rows, cols, uni
     assert torch.isnan(T.gated_linear_backward(torch.full_like(dh, float("nan")), x, wg, wu, gate, up)[0]).all()
 
 
+@gpu
+def test_captured_float16_gradients_are_scaled_by_their_own(cuda):
+    """A captured backward pass finds the power of two of the values that it is replayed on: gradients 2^30 apart, an
+    infinity, zeros and the first ones again, with eager passes of other sizes between the replays."""
+    rows, cols, units = 600, 264, 500
+    x, base = randn((rows, cols), torch.float16, 93), randn((rows, units), torch.float16, 94)
+    wg, wu = (randn((units, cols), torch.float16, s, cols ** -0.5) for s in (95, 96))
+    h, gate, up = T.gated_linear_forward(x, wg, wu)
+    dh = base.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        T.gated_linear_backward(dh, x, wg, wu, gate, up)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = T.gated_linear_backward(dh, x, wg, wu, gate, up)
+    for factor in (1.0, 2.0 ** -18, 4096.0, float("inf"), 0.0, 1.0):
+        dh.copy_(base)
+        if factor != float("inf"):
+            dh.mul_(factor)
+        else:
+            dh[3, 5] = factor
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        T.gated_linear_backward(base[:300], x[:300], wg, wu, gate[:300], up[:300])
+        want = T.gated_linear_backward(dh, x, wg, wu, gate, up)
+        assert all(same_bits(a, b) for a, b in zip(got, want)), factor
+
+
 # ------------------------------------------------------------------ linear cross entropy
 @pytest.mark.parametrize("dtype", [N.P2P_DTYPE_F16, N.P2P_DTYPE_BF16])
 @pytest.mark.parametrize("tokens,hidden,vocab", [(256, 4096, 70000), (1024, 4096, 131072), (2048, 4096, 131072), (512, 2048, 400000)])
