@@ -286,9 +286,15 @@ int32_t p2p_digest_accept(const uint8_t *digests, const uint8_t *expected,
  * nothing between calls, and two calls that may run at once need one each.
  * K9 and K10 take at most 2^22 - 8 features, 2^21 - 8 units and, as far as
  * their tiles fit one launch, 2^31 - 256 tokens or classes
- * (P2P_ERR_UNSUPPORTED past that).  An infinity in a float32 operand of
- * theirs may come out as NaN: larger float32 products are sums of products of
- * three 16-bit parts of each operand.
+ * (P2P_ERR_UNSUPPORTED past that).  Larger float32 products are sums of
+ * products of three 16-bit parts of each operand: an infinity among the
+ * operands may come out as NaN, operands below 2^-110 lose digits.  Larger
+ * 16-bit gradients read dg, du (K9) and d (K10) rounded to the type once;
+ * float16 holds K9's times a power of two found per call, so that what is
+ * below 2^-28 of the largest is off by up to 2^-39 of it.  No result depends on
+ * where operands lie; a workspace's size does, since what cannot be read in
+ * place (16-bit rows or addresses not in whole 16 bytes; float32 in larger
+ * products) is copied into it.
  *
  * K7, layer norm.  y = (x - mean) * rstd * w + b per row, w / b nullable;
  * mean and rstd (float, one per row) feed the backward pass, which writes dx
@@ -332,14 +338,15 @@ int32_t p2p_gated_linear_fwd(const p2p_gated_linear_t *args, void *workspace, in
 int32_t p2p_gated_linear_bwd(const p2p_gated_linear_t *args, void *workspace, int64_t workspace_bytes,
                              p2p_stream_t stream);
 
-/* K10, softmax cross entropy of the logits x w^T (never stored), x [tokens,
- * hidden], w [vocab, hidden], over the tokens whose target is not
- * ignore_index: their mean (mean != 0; 0 where there are none) or sum.  The
- * forward pass writes loss, lse [tokens] and norm (1 / count, or 1), the
- * backward pass reads lse and norm and writes dx and dw, times *dloss
- * (nullable: 1).  A target outside [0, vocab) that is not ignore_index makes
- * the loss and both gradients NaN.  With tokens = 0 the forward pass writes a
- * loss of 0, the backward pass launches nothing. */
+/* K10, softmax cross entropy of the logits x w^T (kept by neither pass; a small
+ * head's stand in the workspace, at most half a gigabyte), x [tokens, hidden],
+ * w [vocab, hidden], over the tokens whose target is not ignore_index: their
+ * mean (mean != 0; 0 where there are none) or sum.  The forward pass writes
+ * loss, lse [tokens] and norm (1 / count, or 1), the backward pass reads lse
+ * and norm and writes dx and dw, times *dloss (nullable: 1).  A target outside
+ * [0, vocab) that is not ignore_index makes the loss and both gradients NaN.
+ * With tokens = 0 the forward pass writes a loss of 0, the backward pass
+ * launches nothing. */
 typedef struct p2p_linear_ce_t {
   const void *x, *w;
   const int64_t *target;

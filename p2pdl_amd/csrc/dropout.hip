@@ -2,7 +2,7 @@
 //
 //   y[i] = (keep(i) ? x[i] / (1 - p) : 0) (+ residual[i])
 //   keep(i): word i % 4 of Philox4x32-10's block offset + i / 4 under the key
-//   `seed` is at least p * 2^32
+//   `seed` is at least floor(p * 2^32)
 // (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3",
 // SC 2011: ten rounds over the counter (block mod 2^32, block / 2^32, 0, 0)).
 // The mask is a function of (seed, offset, i) alone: the backward pass is

@@ -16,7 +16,10 @@
 // unit against 16 more bytes moved).  dg and du are rounded to the type of x
 // once, as the operands of the matrix instructions (float32: not rounded,
 // three planes), lie side by side in one [T, 2F] buffer, and feed dx as two
-// segments of one sum and dWg, dWu as one product of 2F rows.
+// segments of one sum and dWg, dWu as one product of 2F rows.  That rounding
+// and the results' own make 1.4 times the RMS error of the latter alone (1023
+// x 1001 x 2731 float16 2.9e-4, 8192 x 4096 x 16384 bfloat16 2.3e-3; with d in 32
+// bits 2.1e-4, 1.7e-3); a second plane of d would double two of three products.
 //
 // float16 holds them times a power of two that brings the largest of the call
 // to [2^14, 2^15), taken back from the 32-bit sums: without it gradients near

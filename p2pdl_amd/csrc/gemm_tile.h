@@ -11,7 +11,8 @@
 // shape, its segments: the two halves of the gated layer's dx, and float32.
 //
 // float32.  x = hi + mid + lo exactly, three bf16 values of 8 bits each,
-// rounded to nearest: |mid| <= 2^-8 |x|, |lo| <= 2^-16 |x|.  Of the nine
+// rounded to nearest: |mid| <= 2^-8 |x|, |lo| <= 2^-16 |x| (below 2^-110 they
+// meet bf16's smallest step, 2^-133: off by half of it).  Of the nine
 // products the six of order 2^-16 and above are kept, the small ones first;
 // what is left out is at most 2^-23 + 2^-32 of |a| |b|, the size of one
 // rounding of a 32-bit sum.  Six bf16 products take 6/16 of the time of one on

@@ -9,16 +9,18 @@ gradient:
   layer_norm            normalisation of rows, weight and bias
   dropout               mask from a counter-based generator, never stored; adds a residual
   gated_linear          act(x w_gate^T) * (x w_up^T), a feed-forward block's first half
-  linear_cross_entropy  loss of a linear head over a large vocabulary, logits never stored
+  linear_cross_entropy  loss of a linear head (no bias) over a large vocabulary, logits never kept
 
 Every operator has a differentiable form (above) and a pair ``*_forward`` /
 ``*_backward`` that a hand-written or captured step calls directly.  Types:
 float32, float16, bfloat16, one per call; sums and statistics are held in 32
-bits, float32 products are float32 products (an infinity among their operands
-may come out as NaN: larger ones are sums over 16-bit parts).  No result depends on the order
-of atomics and a dropout mask depends on (seed, offset) alone, so a step run
-again on the same inputs gives the same bits, and a local update the same
-digest.
+bits.  Of 16-bit types the last two operators' gradients are rounded to the type
+once, as operands of their products (small sizes keep them in 32 bits).  float32
+products are float32 products (larger ones are sums over 16-bit parts: an
+infinity among their operands may come out as NaN, operands below 2^-110 lose
+digits).  No result depends on the order of atomics or on where a tensor lies, and
+a dropout mask depends on (seed, offset) alone, so a step run again on the same
+inputs gives the same bits, and a local update the same digest.
 
 Tensors are [..., features]; rows may have a pitch (a slice of a wider
 tensor is read in place), other layouts are copied.  Work is launched on the
@@ -288,7 +290,7 @@ def dropout_forward(x: torch.Tensor, p: float, seed: int, offset: int | torch.Te
     divided by 1 - p, plus ``residual`` if given.
 
     Element i (in row-major order) is kept if word i % 4 of Philox4x32-10's
-    block ``offset`` + i // 4 under the key ``seed`` is at least p * 2^32: the
+    block ``offset`` + i // 4 under the key ``seed`` is at least floor(p * 2^32): the
     mask is a function of (seed, offset) and is not stored.  ``offset`` may be a
     one-element int64 tensor on x's device, read when the kernel runs: a captured
     step advances it (by dropout_blocks) between replays."""
@@ -455,9 +457,9 @@ def _ce_args(x, weight, target, ignore_index):
 
 def linear_cross_entropy_forward(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
                                  reduction: str = "mean"):
-    """Softmax cross entropy of the logits x weight^T against ``target``, without
-    the logits: x [..., features], weight [vocabulary, features], target int64 of
-    x's leading shape.  Tokens whose target is ``ignore_index`` do not count;
+    """Softmax cross entropy of the logits x weight^T against ``target``; neither
+    pass keeps the logits (a small head's stand in its workspace during a call).  x
+    [..., features], weight [vocabulary, features], target int64 of x's leading shape.  Tokens whose target is ``ignore_index`` do not count;
     ``reduction`` is "mean" over the others (0 where there are none) or "sum".  A
     target outside the vocabulary gives NaN.
 
