@@ -174,6 +174,12 @@ int64_t integer(PyObject* o) {
   return v;
 }
 
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Raised{};
+  return v;
+}
+
 // layer_norm_forward(x, weight, bias, eps) -> (y, mean, rstd)
 PyObject* layer_norm_forward(PyObject* const* a) {
   const Call c(a[0]);
@@ -258,7 +264,7 @@ struct Gated : Call {
 // gated_linear_forward(x, w_gate, w_up, activation, save) -> (h, gate, up)
 PyObject* gated_linear_forward(PyObject* const* a) {
   Gated c(a[0], a[1], a[2], a[3]);
-  const int save = PyObject_IsTrue(a[4]);
+  const bool save = truth(a[4]);
   const Shape shape(c.lead(), 0, c.args.units);
   at::Tensor h = at::empty(shape, c.x.options()), gate, up;
   if (save) {
@@ -307,7 +313,7 @@ struct Ce : Call {
 // linear_cross_entropy_forward(x, weight, target, ignore_index, mean) -> (loss, lse, norm)
 PyObject* linear_cross_entropy_forward(PyObject* const* a) {
   Ce c(a[0], a[1], a[2], a[3]);
-  c.args.mean = PyObject_IsTrue(a[4]);
+  c.args.mean = truth(a[4]);
   at::Tensor loss = at::empty({}, c.options(at::kFloat)), norm = at::empty({}, c.options(at::kFloat));
   at::Tensor lse = at::empty(c.lead(), c.options(at::kFloat));
   c.args.loss = loss.data_ptr<float>(), c.args.norm = norm.data_ptr<float>(), c.args.lse = lse.data_ptr<float>();

@@ -315,3 +315,13 @@ def test_linear_cross_entropy_inputs_that_are_not_finite(cuda, dtype, rows, cols
     rest = [i for i in range(rows) if i != 3]
     assert torch.isnan(loss) and torch.isnan(lse[3]) and torch.isfinite(lse[rest]).all()
     assert torch.isnan(dx[3]).all() and same_bits(dx[rest], clean[rest]) and torch.isnan(dw).all()
+
+
+@gpu
+def test_an_error_inside_a_call_is_the_callers(cuda):
+    """What `save` raises when it is asked for its truth comes out as it is, and the next call is as before."""
+    x, w = torch.ones(2, 8, device="cuda"), torch.ones(4, 8, device="cuda")
+    want = T.gated_linear_forward(x, w, w)
+    with pytest.raises(RuntimeError, match="[Bb]oolean"):
+        T.gated_linear_forward(x, w, w, save=torch.ones(2))
+    assert all(same_bits(a, b) for a, b in zip(T.gated_linear_forward(x, w, w, save=torch.ones(())), want))
